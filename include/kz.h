@@ -297,6 +297,89 @@ int kz_gemm_i8_allgather(const int8_t* A, int8_t* const* peer_A, uint32_t* const
                          uint32_t* absmax_partials, uint32_t* flags, uint32_t token, int64_t flag_rows, int copy_ctas,
                          kz_stream_t stream);
 
+/* ------------------------------------------------ int8 K/V cache, serving
+ * No reference counterpart (the reference's attention, python/kansai/nn.py:
+ * 410-427, runs over whole sequences and keeps nothing).  A cache is a pool of
+ * pages the caller owns: codes int8 [pages][kv_heads][page_size][head_dim] and
+ * scales fp32 [pages][kv_heads][page_size], for K and for V, 16-byte aligned;
+ * head_dim in {32, 64, 128}, page_size in {16, 32, 64, 128}, pages * kv_heads *
+ * page_size < 2^31.  Position p of sequence b is slot p % page_size of page
+ * table[b * table_cols + p / page_size] (int32, device memory).  lengths[b]
+ * (int32, device) is the number of tokens the sequence has in the cache before
+ * the call; counts[b] (int32, device, NULL: all) the number of its rows that
+ * are tokens, the rest being padding.  A page number outside the pool, or a
+ * position the table has no column for, is not read or written: the row is
+ * left out and the device status word set to KZ_ERR_INVALID_ARGUMENT.
+ *
+ * A row (one token, one head) is quantized by quantize.py:66-70's rule on its
+ * own: scale = max|x| / 127 in double (1 for zeros), codes rounded half to
+ * even; fl32(scale) is kept, and a cached value stands for
+ * fl32(code * fl32(scale)).  A row with NaN/Inf keeps codes 0 and scale NaN
+ * and sets KZ_ERR_NONFINITE. */
+typedef struct kz_cache {
+    int8_t* k_codes;
+    float* k_scale;
+    int8_t* v_codes;
+    float* v_scale;
+    int64_t pages, kv_heads, page_size, head_dim;
+} kz_cache;
+
+/* Nodes a tree of drafted tokens may have in kz_cache_attention_f32. */
+#define KZ_TREE_MAX_NODES 256
+
+/* Quantizes k and v [batch, tokens, kv_heads * head_dim] (element (b, t, i) at
+ * b * batch_stride + t * row_stride + i, floats; 16-byte aligned, strides
+ * multiples of 4) into positions lengths[b] + t.  k_values / v_values (may be
+ * NULL): what the codes stand for, [batch, tokens, kv_heads * head_dim]
+ * contiguous, 0 in padding rows. */
+int kz_cache_write_f32(const kz_cache* cache, const float* k, const float* v, int64_t batch, int64_t tokens,
+                       int64_t k_batch_stride, int64_t k_row_stride, int64_t v_batch_stride, int64_t v_row_stride,
+                       const int32_t* table, int64_t table_cols, const int32_t* lengths, const int32_t* counts,
+                       float* k_values, float* v_values, kz_stream_t stream);
+
+/* The first lengths[b] tokens of each sequence as fp32, k_out and v_out
+ * [batch, most, kv_heads * head_dim] contiguous; rows at or past lengths[b] are
+ * 0, tokens past `most` are left out. */
+int kz_cache_read_f32(const kz_cache* cache, const int32_t* table, int64_t table_cols, const int32_t* lengths,
+                      int64_t batch, int64_t most, float* k_out, float* v_out, kz_stream_t stream);
+
+/* Moves position lengths[b] + path[b * nodes + i] to lengths[b] + i for
+ * i < count[b]: the accepted path of a tree to the front of its new tokens.  A
+ * path that is not strictly increasing within [0, nodes) moves nothing and
+ * sets KZ_ERR_INVALID_ARGUMENT. */
+int kz_cache_keep(const kz_cache* cache, const int32_t* table, int64_t table_cols, const int32_t* lengths,
+                  const int32_t* path, const int32_t* count, int64_t batch, int64_t nodes, kz_stream_t stream);
+
+/* softmax(q k^T * scale) v per head over the cached values, fp32 results: q
+ * [batch, tokens, heads * head_dim] with strides as above, heads a multiple of
+ * kv_heads (head h reads key head h / (heads / kv_heads)).  The new tokens'
+ * K/V are in the cache already, at positions lengths[b] + t.  New token t sees
+ * every position before lengths[b], and of the new ones its ancestors and
+ * itself in the tree (parents[b * parents_batch_stride + t], -1 or anything
+ * that is not below t: none; tokens <= KZ_TREE_MAX_NODES) or, parents NULL,
+ * every one up to itself.  out [batch, tokens, heads * head_dim] contiguous;
+ * rows past counts[b], and rows that see no key, are 0. */
+int kz_cache_attention_f32(const kz_cache* cache, const float* q, int64_t batch, int64_t tokens, int64_t heads,
+                           int64_t q_batch_stride, int64_t q_row_stride, const int32_t* table, int64_t table_cols,
+                           const int32_t* lengths, const int32_t* counts, const int32_t* parents,
+                           int64_t parents_batch_stride, float scale, float* out, kz_stream_t stream);
+
+/* Verifies a tree of drafted tokens (node 0 the root, parents[n] < n; other
+ * values make no child) against the target's probabilities target[batch, nodes,
+ * vocab], with draft[batch, nodes, vocab] the probabilities the children of each
+ * node were drawn from (NULL: drafts without probabilities, one-hot rows) and
+ * accept_u[batch, nodes], sample_u[batch] uniform in [0, 1).  With r the
+ * target's row at the current node, its children are tried in index order:
+ * accepted where accept_u * q(x) < r(x) (the walk goes on there), else
+ * r = (r - q)+ / sum (r - q)+ (r unchanged where that sum is 0).  path
+ * [batch, nodes]: the accepted nodes from the root on, then -1; count[batch];
+ * next[batch]: the smallest token whose running sum of r passes
+ * sample_u * sum r.  All decisions in double.  nodes 1 to 1024, vocab below 2^24. */
+int kz_verify_tree_f32(const int64_t* tokens, const int32_t* parents, int64_t parents_batch_stride,
+                       const float* target, const float* draft, const float* accept_u, const float* sample_u,
+                       int64_t batch, int64_t nodes, int64_t vocab, int32_t* path, int32_t* count, int64_t* next,
+                       kz_stream_t stream);
+
 /* ------------------------------------------------- peer exchange buffers
  * No reference counterpart (the reference's DTensor moves shards through host
  * lists, python/kansai/distributed.py:157-176).  One process per GPU: a rank

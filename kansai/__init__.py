@@ -4,7 +4,7 @@ A user's quantized model keeps its imports as they are -- ``from kansai.quantize
 import QLinear``, ``from kansai import nn``, ``kansai.distributed.DTensor``,
 ``kansai.tensor([[...]])`` -- and runs on libkz.  Every name here is the
 kansaiml_b200 object itself, and ``kansai.quantize`` / ``nn`` /
-``distributed`` / ``serialize`` are the same module objects as
+``distributed`` / ``serialize`` / ``cache`` are the same module objects as
 ``kansaiml_b200.*``: one implementation, one set of per-device state.
 
 The reference package's other top-level names on this path: ``where``
@@ -17,9 +17,10 @@ import contextlib
 import sys
 
 from kansaiml_b200 import Tensor, cat, from_flat, from_numpy, ones, randn, tensor, zeros
-from kansaiml_b200 import distributed, nn, quantize, serialize
+from kansaiml_b200 import cache, distributed, nn, quantize, serialize
 
-for _name, _module in (("quantize", quantize), ("nn", nn), ("distributed", distributed), ("serialize", serialize)):
+for _name, _module in (("quantize", quantize), ("nn", nn), ("distributed", distributed), ("serialize", serialize),
+                       ("cache", cache)):
     sys.modules[f"{__name__}.{_name}"] = _module
 del _name, _module
 
@@ -35,4 +36,4 @@ def no_grad():
 
 
 __all__ = ["Tensor", "cat", "from_flat", "from_numpy", "ones", "randn", "tensor", "zeros", "where", "no_grad",
-           "quantize", "nn", "distributed", "serialize"]
+           "quantize", "nn", "distributed", "serialize", "cache"]

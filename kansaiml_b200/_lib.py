@@ -23,9 +23,17 @@ KZ_ERR_DEVICE_TIMEOUT = 5
 KZ_ACT_NONE, KZ_ACT_RELU, KZ_ACT_GELU = 0, 1, 2
 KZ_PARTIALS_WORDS = 1024
 KZ_IPC_HANDLE_BYTES = 64
+KZ_TREE_MAX_NODES = 256
 
 _P, _I64, _I, _D, _F, _U64, _SZ = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_double,
                                     ctypes.c_float, ctypes.c_uint64, ctypes.c_size_t)
+
+
+class KzCache(ctypes.Structure):
+    """kz_cache: the buffers and sizes of a paged int8 K/V cache."""
+    _fields_ = [("k_codes", _P), ("k_scale", _P), ("v_codes", _P), ("v_scale", _P),
+                ("pages", _I64), ("kv_heads", _I64), ("page_size", _I64), ("head_dim", _I64)]
+
 
 # name -> (restype, argtypes); mirrors include/kz.h
 SIGNATURES = {
@@ -56,6 +64,13 @@ SIGNATURES = {
                               ctypes.c_uint32, _I, _I64, _P]),
     "kz_gemm_i8_allgather": (_I, [_P, _P, _P, _I, _I, _P, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P,
                                   ctypes.c_uint32, _I64, _I, _P]),
+    "kz_cache_write_f32": (_I, [ctypes.POINTER(KzCache), _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P,
+                                _P, _P, _P]),
+    "kz_cache_read_f32": (_I, [ctypes.POINTER(KzCache), _P, _I64, _P, _I64, _I64, _P, _P, _P]),
+    "kz_cache_keep": (_I, [ctypes.POINTER(KzCache), _P, _I64, _P, _P, _P, _I64, _I64, _P]),
+    "kz_cache_attention_f32": (_I, [ctypes.POINTER(KzCache), _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _P,
+                                    _I64, _F, _P, _P]),
+    "kz_verify_tree_f32": (_I, [_P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P]),
     "kz_peer_alloc": (_I, [_SZ, ctypes.POINTER(_P), _P]),
     "kz_peer_open": (_I, [_P, ctypes.POINTER(_P)]),
     "kz_peer_close": (_I, [_P]),

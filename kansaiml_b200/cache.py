@@ -1,0 +1,300 @@
+"""An int8 K/V cache for generation: quantized as it is written, read back,
+attended over, and the verification of drafted tokens.
+
+The reference recomputes attention over the whole sequence for every token
+(MultiHeadAttention.forward, nn.py:410-427) and keeps nothing; here its keys
+and values stay on the GPU as int8 codes, quantized by quantize_symmetric's
+rule (quantize.py:66-70) with one scale per token and key head:
+
+* ``QCache``: one attention layer's pages.  ``write`` quantizes new tokens into
+  it, ``read`` gives tokens back as fp32, ``attention`` attends over it (one new
+  token a sequence, a chunk of a prompt, or a tree of drafted tokens, with
+  grouped heads), ``keep`` moves the accepted path of a tree to the front.
+* ``PagePool``: which pages each sequence has (one pool serves every layer).
+* ``verify_tree``: which drafted tokens stand, and the next token, from the
+  target's probabilities and given uniform numbers.  A tree of one node draws
+  the next token of plain sampling.
+
+Common arguments: ``table`` int32 [batch, columns], the page numbers of each
+sequence; ``lengths`` int32 [batch], its tokens in the cache before the call;
+``counts`` int32 [batch] or None, how many of its rows are tokens (None: all;
+the rest is padding); ``parents`` int32 [batch, tokens] or [tokens], each new
+token's parent in its tree (-1: none; a parent comes before its child).  All
+are CUDA tensors, read on the device: nothing here waits for the GPU.  A page
+number or position that a cache does not have is left out and recorded in the
+device status word (quantize.device_status), as NaN/Inf in a written row is.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .tensor import Tensor, _as_device, ptr, require_cuda, stream_handle
+
+
+def _raw(t, what):
+    """The fp32 CUDA tensor of a Tensor or torch tensor."""
+    x = t.data if isinstance(t, Tensor) else t
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{what} must be a Tensor or a torch tensor, not {type(t).__name__}")
+    require_cuda(x, what)
+    return x if x.dtype == torch.float32 else x.float()
+
+
+def _rows(x, what, width):
+    """(x, batch stride, row stride) of a [batch, tokens, width] tensor whose
+    rows a kernel can read in 16-byte pieces; any other is copied first."""
+    if x.dim() != 3 or x.shape[2] != width:
+        raise ValueError(f"{what} must be [batch, tokens, {width}], not {list(x.shape)}")
+    bs, rs, fs = x.stride()
+    if (x.data_ptr() & 15) or ((bs | rs) & 3) or fs != 1 or bs < 0 or (x.shape[1] > 1 and rs < width):
+        x = x.contiguous()
+        if x.data_ptr() & 15:
+            x = x.clone()
+        bs, rs, _ = x.stride()
+    return x, bs, rs
+
+
+def _ints(t, what, shape, device, dtype=torch.int32):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must be a {str(dtype)[6:]} tensor {list(shape)}, not "
+                         f"{list(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}"
+                         f"{' ' + str(t.dtype)[6:] if isinstance(t, torch.Tensor) else ''}")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, not on {device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _parents(parents, batch, nodes, device):
+    """(parents, batch stride): one tree for every sequence, or one each."""
+    if isinstance(parents, torch.Tensor) and parents.dim() == 1:
+        return _ints(parents, "parents", (nodes,), device), 0
+    return _ints(parents, "parents", (batch, nodes), device), nodes
+
+
+def _on(device, name, *args):
+    """Calls libkz with `device` current, on torch's current stream there."""
+    if torch.cuda.current_device() == device.index:
+        _lib.call(name, *args, stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, stream_handle(device))
+
+
+class QCache:
+    """One attention layer's int8 K/V pages: codes [pages, kv_heads, page_size,
+    head_dim] and fp32 scales [pages, kv_heads, page_size], for K and for V."""
+
+    __slots__ = ("k_codes", "k_scale", "v_codes", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "_c", "_ref")
+
+    def __init__(self, pages, kv_heads, head_dim, page_size=64, device=None):
+        dev = _as_device(device)
+        shape = (int(pages), int(kv_heads), int(page_size))
+        if min(shape) < 0:
+            raise ValueError(f"QCache: negative size {shape}")
+        self._bind(*(torch.empty(shape + d, dtype=t, device=dev)
+                     for _ in range(2) for d, t in (((int(head_dim),), torch.int8), ((), torch.float32))))
+
+    @classmethod
+    def wrap(cls, k_codes, k_scale, v_codes, v_scale):
+        """A cache over buffers the caller has."""
+        obj = cls.__new__(cls)
+        obj._bind(k_codes, k_scale, v_codes, v_scale)
+        return obj
+
+    def _bind(self, k_codes, k_scale, v_codes, v_scale):
+        if k_codes.dim() != 4:
+            raise ValueError(f"QCache: codes must be [pages, kv_heads, page_size, head_dim], not {list(k_codes.shape)}")
+        self.pages, self.kv_heads, self.page_size, self.head_dim = k_codes.shape
+        if self.head_dim not in (32, 64, 128):
+            raise ValueError(f"QCache: head_dim must be 32, 64 or 128 (got {self.head_dim})")
+        if self.page_size not in (16, 32, 64, 128):
+            raise ValueError(f"QCache: page_size must be 16, 32, 64 or 128 (got {self.page_size})")
+        if self.kv_heads < 1:
+            raise ValueError("QCache: kv_heads must be at least 1")
+        for t, dtype, shape in ((k_codes, torch.int8, k_codes.shape), (v_codes, torch.int8, k_codes.shape),
+                                (k_scale, torch.float32, k_codes.shape[:3]),
+                                (v_scale, torch.float32, k_codes.shape[:3])):
+            if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.device != k_codes.device:
+                raise ValueError("QCache: codes are int8 [pages, kv_heads, page_size, head_dim], scales float32 "
+                                 "[pages, kv_heads, page_size], contiguous and on one device")
+        self.k_codes, self.k_scale, self.v_codes, self.v_scale = k_codes, k_scale, v_codes, v_scale
+        self._c = _lib.KzCache(ptr(k_codes), ptr(k_scale), ptr(v_codes), ptr(v_scale), *k_codes.shape)
+        self._ref = ctypes.byref(self._c)
+
+    @property
+    def device(self):
+        return self.k_codes.device
+
+    def nbytes(self):
+        """Bytes held: one per code and four per scale."""
+        return 2 * (self.k_codes.numel() + 4 * self.k_scale.numel())
+
+    def __repr__(self):
+        return (f"QCache(pages={self.pages}, kv_heads={self.kv_heads}, head_dim={self.head_dim}, "
+                f"page_size={self.page_size}, device={self.device})")
+
+    def _sequences(self, table, lengths, counts=None):
+        dev = self.device
+        require_cuda(self.k_codes, "QCache")
+        if not isinstance(table, torch.Tensor) or table.dim() != 2:
+            raise ValueError("table must be an int32 tensor [batch, columns]")
+        batch, cols = table.shape
+        return (batch, cols, _ints(table, "table", (batch, cols), dev), _ints(lengths, "lengths", (batch,), dev),
+                None if counts is None else _ints(counts, "counts", (batch,), dev))
+
+    def _input(self, t, what, heads, batch):
+        x = _raw(t, what)
+        if x.device != self.device:
+            raise ValueError(f"{what} is on {x.device}, the cache on {self.device}")
+        if x.dim() != 3 or x.shape[0] != batch:
+            raise ValueError(f"{what} must be [{batch}, tokens, {heads * self.head_dim}], not {list(x.shape)}")
+        return _rows(x, what, heads * self.head_dim)
+
+    def write(self, k, v, table, lengths, counts=None, values=False):
+        """Quantizes new tokens' k and v [batch, tokens, kv_heads * head_dim]
+        (strided rows allowed, e.g. slices of a fused projection) into positions
+        lengths + 0, 1, ...  With ``values``, returns what the codes stand for,
+        two Tensors like k and v (0 in padding rows): the K/V a later pass sees."""
+        batch, cols, table, lengths, counts = self._sequences(table, lengths, counts)
+        k, kb, kr = self._input(k, "k", self.kv_heads, batch)
+        v, vb, vr = self._input(v, "v", self.kv_heads, batch)
+        if v.shape != k.shape:
+            raise ValueError(f"k {list(k.shape)} and v {list(v.shape)} do not match")
+        ko = vo = None
+        if values:
+            ko, vo = (torch.empty(k.shape, dtype=torch.float32, device=k.device) for _ in range(2))
+        _on(self.device, "kz_cache_write_f32", self._ref, ptr(k), ptr(v), batch, k.shape[1], kb, kr, vb, vr, ptr(table),
+            cols, ptr(lengths), ptr(counts), ptr(ko), ptr(vo))
+        return (Tensor(ko), Tensor(vo)) if values else None
+
+    def read(self, table, lengths, most):
+        """The first ``lengths`` tokens of each sequence, dequantized: two
+        Tensors [batch, most, kv_heads * head_dim], 0 past a sequence's length
+        (tokens past ``most`` are left out)."""
+        batch, cols, table, lengths, _ = self._sequences(table, lengths)
+        if most < 0:
+            raise ValueError(f"read: most must not be negative (got {most})")
+        shape = (batch, int(most), self.kv_heads * self.head_dim)
+        k, v = (torch.empty(shape, dtype=torch.float32, device=self.device) for _ in range(2))
+        _on(self.device, "kz_cache_read_f32", self._ref, ptr(table), cols, ptr(lengths), batch, shape[1], ptr(k), ptr(v))
+        return Tensor(k), Tensor(v)
+
+    def attention(self, q, heads, table, lengths, counts=None, parents=None, scale=None):
+        """softmax(q k^T * scale) v over the cached tokens and the new ones
+        (written before): q [batch, tokens, heads * head_dim], heads a multiple
+        of kv_heads; scale 1 / sqrt(head_dim) by default.  A new token sees every
+        token before the new ones and, of these, its ancestors and itself in the
+        tree ``parents`` (at most 256 nodes), or without one all up to itself.
+        Returns [batch, tokens, heads * head_dim], 0 in padding rows."""
+        batch, cols, table, lengths, counts = self._sequences(table, lengths, counts)
+        if heads < 1 or heads % self.kv_heads:
+            raise ValueError(f"attention: heads ({heads}) must be a multiple of kv_heads ({self.kv_heads})")
+        q, qb, qr = self._input(q, "q", heads, batch)
+        tokens, pb = q.shape[1], 0
+        if parents is not None:
+            if tokens > _lib.KZ_TREE_MAX_NODES:
+                raise ValueError(f"attention: a tree has at most {_lib.KZ_TREE_MAX_NODES} nodes (got {tokens})")
+            parents, pb = _parents(parents, batch, tokens, self.device)
+        out = torch.empty((batch, tokens, heads * self.head_dim), dtype=torch.float32, device=self.device)
+        _on(self.device, "kz_cache_attention_f32", self._ref, ptr(q), batch, tokens, heads, qb, qr, ptr(table), cols,
+            ptr(lengths), ptr(counts), ptr(parents), pb, 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
+            ptr(out))
+        return Tensor(out)
+
+    def keep(self, table, lengths, path, count):
+        """Moves the new tokens path[b, 0 .. count[b] - 1] (strictly increasing,
+        int32 [batch, nodes], as verify_tree returns it) to positions lengths +
+        0, 1, ...: the cache then holds lengths + count tokens of each sequence."""
+        batch, cols, table, lengths, count = self._sequences(table, lengths, count)
+        if not isinstance(path, torch.Tensor) or path.dim() != 2:
+            raise ValueError("path must be an int32 tensor [batch, nodes]")
+        path = _ints(path, "path", (batch, path.shape[1]), self.device)
+        if count is None:
+            raise ValueError("count must be an int32 tensor [batch]")
+        _on(self.device, "kz_cache_keep", self._ref, ptr(table), cols, ptr(lengths), ptr(path), ptr(count), batch,
+            path.shape[1])
+
+
+class PagePool:
+    """Hands out page numbers 0 .. pages - 1 to ``batch`` sequences.  ``table``
+    (int32 [batch, columns] on the device, -1 where a sequence has no page) is
+    what every layer's QCache takes; a change is one small copy to the device."""
+
+    def __init__(self, pages, batch, columns, page_size=64, device=None):
+        self.page_size, self.columns = int(page_size), int(columns)
+        self._free = list(range(int(pages) - 1, -1, -1))
+        self._held = [[] for _ in range(int(batch))]
+        self.table = torch.full((int(batch), self.columns), -1, dtype=torch.int32, device=_as_device(device))
+
+    @property
+    def free(self):
+        return len(self._free)
+
+    def reserve(self, tokens, sequence=None):
+        """Pages for ``tokens`` positions of one sequence, or of each; raises,
+        and changes nothing, where the pool or the table is too small."""
+        need = -(-int(tokens) // self.page_size)
+        if need > self.columns:
+            raise ValueError(f"PagePool: {tokens} tokens need {need} pages a sequence, the table has {self.columns}")
+        which = range(len(self._held)) if sequence is None else [sequence]
+        short = sum(max(0, need - len(self._held[i])) for i in which)
+        if short > len(self._free):
+            raise RuntimeError(f"PagePool: {short} pages needed, {len(self._free)} free")
+        for i in which:
+            at = len(self._held[i])
+            if need > at:
+                new = [self._free.pop() for _ in range(need - at)]
+                self._held[i] += new
+                self.table[i, at:need] = torch.tensor(new, dtype=torch.int32)
+
+    def release(self, sequence):
+        """Gives a sequence's pages back."""
+        self._free += reversed(self._held[sequence])
+        self._held[sequence] = []
+        self.table[sequence] = -1
+
+
+def verify_tree(tokens, parents, target, draft, accept_u, sample_u):
+    """Which nodes of a drafted tree stand (speculative sampling).
+
+    tokens int64 [batch, nodes], node 0 the root (a token already drawn);
+    parents int32 [batch, nodes] or [nodes]; target fp32 [batch, nodes, vocab],
+    the model's probabilities after each node; draft, the same shape, the
+    probabilities each node's children were drawn from, or None where drafts
+    have none; accept_u fp32 [batch, nodes] and sample_u [batch] uniform in
+    [0, 1).  With r the target's row at the current node, its children x are
+    tried in index order: accepted where accept_u * q(x) < r(x), and the walk
+    goes on there; else r = (r - q)+ / sum (r - q)+.  Returns path int32
+    [batch, nodes] (the accepted nodes from the root on, then -1), count int32
+    [batch], and the next token int64 [batch], drawn from r by sample_u: it is
+    distributed as the target's own, whatever was drafted."""
+    target = _raw(target, "target")
+    if target.dim() != 3 or target.shape[1] < 1 or target.shape[2] < 1:
+        raise ValueError(f"target must be [batch, nodes, vocab], not {list(target.shape)}")
+    batch, nodes, vocab = target.shape
+    if nodes > 1024:
+        raise ValueError(f"verify_tree: at most 1024 nodes (got {nodes})")
+    dev = target.device
+
+    def floats(t, what, shape):
+        x = _raw(t, what)
+        if tuple(x.shape) != tuple(shape) or x.device != dev:
+            raise ValueError(f"{what} must be {list(shape)} on {dev}, not {list(x.shape)} on {x.device}")
+        return x.contiguous()
+
+    target = target.contiguous()
+    draft = None if draft is None else floats(draft, "draft", target.shape)
+    accept_u, sample_u = floats(accept_u, "accept_u", (batch, nodes)), floats(sample_u, "sample_u", (batch,))
+    tokens = _ints(tokens, "tokens", (batch, nodes), dev, torch.int64)
+    parents, pb = _parents(parents, batch, nodes, dev)
+    path = torch.empty((batch, nodes), dtype=torch.int32, device=dev)
+    count = torch.empty(batch, dtype=torch.int32, device=dev)
+    token = torch.empty(batch, dtype=torch.int64, device=dev)
+    _on(dev, "kz_verify_tree_f32", ptr(tokens), ptr(parents), pb, ptr(target), ptr(draft), ptr(accept_u), ptr(sample_u),
+        batch, nodes, vocab, ptr(path), ptr(count), ptr(token))
+    return path, count, token
+
+
+__all__ = ["QCache", "PagePool", "verify_tree"]

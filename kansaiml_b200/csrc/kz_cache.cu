@@ -1,0 +1,407 @@
+// The paged int8 K/V cache: writing new tokens, reading tokens back, moving
+// the accepted path of a drafted tree to the front.
+//
+// A token's head (d values) is one row with its own scale, quantized by the
+// framework's rule (kz_quant_math.cuh): scale = max|x| / 127 in double (1 for
+// a row of zeros), code = rint(x / scale) half to even.  What is kept is the
+// code and fl32(scale); a cached value stands for fl32(code * fl32(scale)).
+//
+// All three kernels move each byte once and are bound by HBM (small calls by
+// the launch).  A page keeps each head's slots together ([page][head][slot][d]),
+// so attention and the read-back stream whole pages; a written row is d
+// contiguous bytes.
+#include <algorithm>
+
+#include "kz_cache.cuh"
+#include "kz_quant_math.cuh"
+
+namespace kz {
+namespace {
+
+constexpr int kCacheThreads = 256;
+
+// x / d and x % d for 0 <= x < 2^31 by one multiply-high (the rows of a call
+// are numbered through and split into sequence, token and head by each lane).
+struct FastDiv {
+    uint32_t d, m, l;
+};
+FastDiv fast_div(uint32_t d) {
+    FastDiv f{d, 0, 0};
+    while ((1ull << f.l) < d) ++f.l;
+    f.m = (uint32_t)(((1ull << 32) * ((1ull << f.l) - d)) / d + 1);
+    return f;
+}
+__device__ __forceinline__ uint32_t div_by(uint32_t x, const FastDiv& f) { return (__umulhi(f.m, x) + x) >> f.l; }
+
+struct WriteArgs {
+    CacheView c;
+    SeqView s;
+    const float* x[2];                 // K, V
+    int64_t bs[2], rs[2];              // batch and row strides (floats)
+    float* values[2];                  // what the codes stand for, [batch, tokens, heads * d], or NULL
+    const int32_t* counts;
+    uint32_t tokens, rows;             // rows = batch * tokens * heads
+    FastDiv by_heads, by_tokens;
+    int* status;
+};
+
+// Four codes (a packed word) as floats times a scale, one rounding each: the
+// byte, offset by 128, in the mantissa of 2^23, less 2^23 + 128, is the code.
+__device__ __forceinline__ float4 codes_times(uint32_t w, float s) {
+    w ^= 0x80808080u;
+    float4 v;
+    v.x = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)) - 8388736.0f, s);
+    v.y = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441)) - 8388736.0f, s);
+    v.z = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)) - 8388736.0f, s);
+    v.w = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443)) - 8388736.0f, s);
+    return v;
+}
+
+// One group of D / 4 lanes holds a row (16 bytes a lane); a warp works on
+// kU x 2 such row sets at a time (K and V of kU consecutive rows a group), so
+// 2 kU 16-byte loads are in flight a lane.  The rows' scales need two double
+// divisions each: they are handed to one lane a row and back by shuffles, so a
+// warp divides once for all its rows instead of once a row set.
+template <int D, int kU>
+__global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(WriteArgs a) {
+    constexpr int L = D / 4, G = 32 / L, N = 2 * kU * G;   // lanes a row, groups a warp, rows a warp
+    static_assert(N <= 32, "a lane for each row's scale");
+    griddep_launch_dependents();
+    griddep_wait();
+    const int lane = threadIdx.x & 31, sub = lane / L, col = 4 * (lane % L);
+    const uint32_t first = (blockIdx.x * (kCacheThreads / 32) + (threadIdx.x >> 5)) * (uint32_t)(kU * G);
+    if (first >= a.rows) return;
+    float4 x[2 * kU];
+    int64_t row_at[kU];      // the row's place in the cache, -1: none
+    int64_t out_at[kU];      // and in the returned values, -1: past the last row
+    uint32_t bits[2 * kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+        const uint32_t r = first + u * G + sub;
+        const uint32_t bt = div_by(r, a.by_heads), h = r - bt * a.by_heads.d;
+        const uint32_t b = div_by(bt, a.by_tokens), t = bt - b * a.by_tokens.d;
+        row_at[u] = -1;
+        out_at[u] = r < a.rows ? (int64_t)r * D + col : -1;
+        x[2 * u] = x[2 * u + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < a.rows && (!a.counts || (int)t < a.counts[b])) {
+            x[2 * u] = __ldcs(reinterpret_cast<const float4*>(a.x[0] + b * a.bs[0] + t * a.rs[0] + h * D + col));
+            x[2 * u + 1] = __ldcs(reinterpret_cast<const float4*>(a.x[1] + b * a.bs[1] + t * a.rs[1] + h * D + col));
+            const int page = page_of(a.c, a.s, b, (int64_t)a.s.lengths[b] + t);
+            if (page >= 0)
+                row_at[u] = ((int64_t)page * a.c.heads + h) * a.c.page + ((a.s.lengths[b] + (int)t) & (a.c.page - 1));
+            else if (lane % L == 0)
+                record_status(a.status, KZ_ERR_INVALID_ARGUMENT);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * kU; ++i) {
+        uint32_t m = max(max(abs_bits(x[i].x), abs_bits(x[i].y)), max(abs_bits(x[i].z), abs_bits(x[i].w)));
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        bits[i] = m;
+    }
+    // lane i * G + g: the scale of row set i of group g
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < 2 * kU; ++i) {
+        const uint32_t m = __shfl_sync(0xffffffffu, bits[i], (lane % G) * L);
+        if (lane / G == i) mine = m;
+    }
+    const ScaleInfo si = scale_from_absmax_bits(mine);
+    const float s32 = si.finite ? __double2float_rn(si.scale) : __uint_as_float(0x7FC00000u);
+#pragma unroll
+    for (int i = 0; i < 2 * kU; ++i) {
+        const int u = i >> 1, kv = i & 1;
+        const float s = __shfl_sync(0xffffffffu, s32, i * G + sub);
+        const float rcp = __shfl_sync(0xffffffffu, si.rcp, i * G + sub);
+        if (out_at[u] < 0) continue;
+        uint32_t w = 0;
+        if (bits[i] < kInfBits) {
+            const bool fast = bits[i] >= __float_as_uint(7.8886090522101181e-31f);   // as scale_from_absmax_bits has it
+            float near;
+            w = pack4_fast(x[i], rcp, near);
+            if (!fast || near > kTieGuardFma)
+                w = pack4_repair(x[i], w, scale_from_absmax_bits(bits[i]).scale, rcp, fast);
+        }
+        if (row_at[u] >= 0) {
+            *reinterpret_cast<uint32_t*>(a.c.codes[kv] + row_at[u] * D + col) = w;
+            if (col == 0) {
+                a.c.scale[kv][row_at[u]] = s;
+                if (bits[i] >= kInfBits) record_status(a.status, KZ_ERR_NONFINITE);
+            }
+        }
+        if (a.values[kv]) __stcs(reinterpret_cast<float4*>(a.values[kv] + out_at[u]), codes_times(w, s));
+    }
+}
+
+struct ReadArgs {
+    CacheView c;
+    SeqView s;
+    float* out[2];                     // [batch, most, heads * d]
+    uint32_t most, chunks, items;      // items = batch * chunks (pages up to `most`) * heads
+    FastDiv by_heads, by_chunks;
+    int* status;
+};
+
+// A warp a (sequence, page, head): streams the page's K and V slots of that
+// head (contiguous) and writes rows of d floats; rows past the sequence's
+// length are written as zeros.  Four code words of K and four of V in flight.
+template <int D>
+__global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(ReadArgs a) {
+    constexpr int L = D / 4, G = 32 / L;
+    griddep_launch_dependents();
+    griddep_wait();
+    const int lane = threadIdx.x & 31, sub = lane / L, col = 4 * (lane % L);
+    const uint32_t item = blockIdx.x * (kCacheThreads / 32) + (threadIdx.x >> 5);
+    if (item >= a.items) return;
+    const uint32_t bc = div_by(item, a.by_heads), h = item - bc * a.by_heads.d;
+    const uint32_t b = div_by(bc, a.by_chunks), chunk = bc - b * a.by_chunks.d;
+    const int64_t first = (int64_t)chunk * a.c.page;
+    const int rows = (int)min((int64_t)a.c.page, (int64_t)a.most - first);          // output rows of this page
+    int held = (int)min((int64_t)rows, max((int64_t)0, (int64_t)a.s.lengths[b] - first));
+    int64_t base = 0;
+    if (held > 0) {
+        const int page = page_of(a.c, a.s, b, first);
+        if (page < 0) {
+            if (lane == 0) record_status(a.status, KZ_ERR_INVALID_ARGUMENT);
+            held = 0;
+        }
+        base = ((int64_t)page * a.c.heads + h) * a.c.page;
+    }
+    const int64_t width = (int64_t)a.c.heads * D;
+    const int64_t out_at = ((int64_t)b * a.most + first) * width + h * D + col;
+    for (int r0 = 0; r0 < rows; r0 += 4 * G) {
+        uint32_t w[2][4];
+        float s[2][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int r = r0 + u * G + sub;
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                const bool there = r < held;
+                w[kv][u] = there ? __ldcs(reinterpret_cast<const uint32_t*>(a.c.codes[kv] + (base + r) * D + col)) : 0u;
+                s[kv][u] = there ? __ldg(a.c.scale[kv] + base + r) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int r = r0 + u * G + sub;
+            if (r < rows) {
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv)
+                    __stcs(reinterpret_cast<float4*>(a.out[kv] + out_at + r * width), codes_times(w[kv][u], s[kv][u]));
+            }
+        }
+    }
+}
+
+struct KeepArgs {
+    CacheView c;
+    SeqView s;
+    const int32_t* path;               // [batch, nodes]
+    const int32_t* count;              // [batch]
+    int batch, nodes;
+    int* status;
+};
+
+// A warp a (sequence, head): slot length + path[i] moves to length + i.  A
+// path is strictly increasing (a node comes after its parent), so path[i] >= i
+// and a row's new slot is never the old slot of a later row: passes of whole
+// rows, every load of a pass before its stores, move in place without a copy.
+// A path that is not strictly increasing within [0, nodes) moves nothing.
+template <int D>
+__global__ void __launch_bounds__(kCacheThreads) cache_keep_kernel(KeepArgs a) {
+    constexpr int L = D / 16, G = 32 / L;    // 16 codes a lane
+    griddep_launch_dependents();
+    griddep_wait();
+    const int lane = threadIdx.x & 31, sub = lane / L, col = 16 * (lane % L);
+    const int64_t item = (int64_t)blockIdx.x * (kCacheThreads / 32) + (threadIdx.x >> 5);
+    if (item >= (int64_t)a.batch * a.c.heads) return;
+    const int b = (int)(item / a.c.heads), h = (int)(item % a.c.heads);
+    const int32_t* path = a.path + (int64_t)b * a.nodes;
+    const int n = a.count[b];
+    const int64_t len = a.s.lengths[b];
+    bool good = n >= 0 && n <= a.nodes;
+    if (good)
+        for (int i = lane; i < n; i += 32)
+            good = good && path[i] >= (i > 0 ? path[i - 1] + 1 : 0) && path[i] < a.nodes &&
+                   page_of(a.c, a.s, b, len + i) >= 0 && page_of(a.c, a.s, b, len + path[i]) >= 0;
+    if (!__all_sync(0xffffffffu, good)) {
+        if (lane == 0) record_status(a.status, KZ_ERR_INVALID_ARGUMENT);
+        return;
+    }
+    for (int i0 = 0; i0 < n; i0 += G) {
+        const int i = i0 + sub;
+        const bool moves = i < n && path[i] != i;
+        int64_t from = 0, to = 0;
+        uint4 w[2];
+        float s[2];
+        if (moves) {
+            const int64_t p = len + path[i], q = len + i;
+            from = ((int64_t)page_of(a.c, a.s, b, p) * a.c.heads + h) * a.c.page + (p & (a.c.page - 1));
+            to = ((int64_t)page_of(a.c, a.s, b, q) * a.c.heads + h) * a.c.page + (q & (a.c.page - 1));
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                w[kv] = *reinterpret_cast<const uint4*>(a.c.codes[kv] + from * D + col);
+                s[kv] = a.c.scale[kv][from];
+            }
+        }
+        __syncwarp();
+        if (moves) {
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                *reinterpret_cast<uint4*>(a.c.codes[kv] + to * D + col) = w[kv];
+                if (col == 0) a.c.scale[kv][to] = s[kv];
+            }
+        }
+        __syncwarp();
+    }
+}
+
+template <int D>
+int launch_write(const WriteArgs& a, cudaStream_t s) {
+    constexpr int kU = 4;
+    const uint32_t per_block = (kCacheThreads / 32) * kU * (128 / D);
+    KZ_CHECK_CUDA(launch_pdl(cache_write_kernel<D, kU>, dim3((a.rows + per_block - 1) / per_block),
+                             dim3(kCacheThreads), 0, s, a));
+    return KZ_OK;
+}
+
+}  // namespace
+
+int cache_view(const kz_cache* c, const char* who, CacheView* v) {
+    KZ_REQUIRE(c, std::string(who) + ": cache is NULL");
+    KZ_REQUIRE(c->head_dim == 32 || c->head_dim == 64 || c->head_dim == 128, std::string(who) + ": head_dim must be 32, 64 or 128");
+    KZ_REQUIRE(c->page_size == 16 || c->page_size == 32 || c->page_size == 64 || c->page_size == 128,
+               std::string(who) + ": page_size must be 16, 32, 64 or 128");
+    KZ_REQUIRE(c->pages >= 0 && c->kv_heads > 0 && c->kv_heads < (1 << 16) &&
+                   c->pages * c->kv_heads < (int64_t)INT32_MAX / c->page_size,
+               std::string(who) + ": cache size out of range (pages * kv_heads * page_size must be below 2^31)");
+    KZ_REQUIRE(c->pages == 0 || (c->k_codes && c->v_codes && c->k_scale && c->v_scale), std::string(who) + ": NULL cache buffer");
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes) |
+                           reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale);
+    KZ_REQUIRE((bits & 15u) == 0, std::string(who) + ": cache buffers must be 16-byte aligned");
+    v->codes[0] = c->k_codes;
+    v->codes[1] = c->v_codes;
+    v->scale[0] = c->k_scale;
+    v->scale[1] = c->v_scale;
+    v->pages = (int)c->pages;
+    v->heads = (int)c->kv_heads;
+    v->page = (int)c->page_size;
+    v->shift = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
+    return KZ_OK;
+}
+
+int seq_view(const int32_t* table, int64_t cols, const int32_t* lengths, int64_t batch, const char* who, SeqView* v) {
+    KZ_REQUIRE(batch >= 0 && batch < (1 << 24) && cols >= 0 && cols < (1 << 24), std::string(who) + ": batch or table size out of range");
+    KZ_REQUIRE(batch == 0 || ((table || cols == 0) && lengths), std::string(who) + ": table or lengths is NULL");
+    v->table = table;
+    v->lengths = lengths;
+    v->cols = (int)cols;
+    return KZ_OK;
+}
+
+}  // namespace kz
+
+using namespace kz;
+
+extern "C" int kz_cache_write_f32(const kz_cache* cache, const float* k, const float* v, int64_t batch, int64_t tokens,
+                                  int64_t k_batch_stride, int64_t k_row_stride, int64_t v_batch_stride,
+                                  int64_t v_row_stride, const int32_t* table, int64_t table_cols,
+                                  const int32_t* lengths, const int32_t* counts, float* k_values, float* v_values,
+                                  kz_stream_t stream) {
+    WriteArgs a;
+    int st = cache_view(cache, "kz_cache_write_f32", &a.c);
+    if (!st) st = seq_view(table, table_cols, lengths, batch, "kz_cache_write_f32", &a.s);
+    if (st) return st;
+    const int64_t width = cache->kv_heads * cache->head_dim;
+    KZ_REQUIRE(tokens >= 0 && tokens < (1 << 24), "kz_cache_write_f32: tokens out of range");
+    KZ_REQUIRE(batch * tokens < (int64_t)INT32_MAX / cache->kv_heads, "kz_cache_write_f32: batch * tokens * kv_heads out of range");
+    if (batch * tokens == 0) return KZ_OK;
+    KZ_REQUIRE(k && v, "kz_cache_write_f32: k or v is NULL");
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                           reinterpret_cast<uintptr_t>(k_values) | reinterpret_cast<uintptr_t>(v_values);
+    KZ_REQUIRE((bits & 15u) == 0 && ((k_batch_stride | k_row_stride | v_batch_stride | v_row_stride) & 3) == 0,
+               "kz_cache_write_f32: k, v and the values must be 16-byte aligned, strides multiples of 4 floats");
+    KZ_REQUIRE(tokens == 1 || (k_row_stride >= width && v_row_stride >= width),
+               "kz_cache_write_f32: a row stride is shorter than kv_heads * head_dim");
+    KZ_REQUIRE(k_batch_stride >= 0 && v_batch_stride >= 0, "kz_cache_write_f32: negative batch stride");
+    st = check_device();
+    if (st) return st;
+    a.x[0] = k;
+    a.x[1] = v;
+    a.bs[0] = k_batch_stride;
+    a.bs[1] = v_batch_stride;
+    a.rs[0] = k_row_stride;
+    a.rs[1] = v_row_stride;
+    a.values[0] = k_values;
+    a.values[1] = v_values;
+    a.counts = counts;
+    a.tokens = (uint32_t)tokens;
+    a.rows = (uint32_t)(batch * tokens * cache->kv_heads);
+    a.by_heads = fast_div((uint32_t)cache->kv_heads);
+    a.by_tokens = fast_div((uint32_t)tokens);
+    a.status = device_status_ptr();
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    return cache->head_dim == 32 ? launch_write<32>(a, s) : cache->head_dim == 64 ? launch_write<64>(a, s)
+                                                                                  : launch_write<128>(a, s);
+}
+
+extern "C" int kz_cache_read_f32(const kz_cache* cache, const int32_t* table, int64_t table_cols,
+                                 const int32_t* lengths, int64_t batch, int64_t most, float* k_out, float* v_out,
+                                 kz_stream_t stream) {
+    ReadArgs a;
+    int st = cache_view(cache, "kz_cache_read_f32", &a.c);
+    if (!st) st = seq_view(table, table_cols, lengths, batch, "kz_cache_read_f32", &a.s);
+    if (st) return st;
+    KZ_REQUIRE(most >= 0 && most < (int64_t)INT32_MAX, "kz_cache_read_f32: most out of range");
+    if (batch * most == 0) return KZ_OK;
+    const int64_t chunks = (most + cache->page_size - 1) / cache->page_size;
+    KZ_REQUIRE(batch * chunks < (int64_t)INT32_MAX / cache->kv_heads, "kz_cache_read_f32: batch * most * kv_heads out of range");
+    KZ_REQUIRE(k_out && v_out, "kz_cache_read_f32: k_out or v_out is NULL");
+    KZ_REQUIRE(((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15u) == 0,
+               "kz_cache_read_f32: k_out and v_out must be 16-byte aligned");
+    st = check_device();
+    if (st) return st;
+    a.out[0] = k_out;
+    a.out[1] = v_out;
+    a.most = (uint32_t)most;
+    a.chunks = (uint32_t)chunks;
+    a.items = (uint32_t)(batch * chunks * cache->kv_heads);
+    a.by_heads = fast_div((uint32_t)cache->kv_heads);
+    a.by_chunks = fast_div((uint32_t)chunks);
+    a.status = device_status_ptr();
+    const dim3 grid((a.items + kCacheThreads / 32 - 1) / (kCacheThreads / 32));
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    auto kernel = cache->head_dim == 32 ? cache_read_kernel<32> : cache->head_dim == 64 ? cache_read_kernel<64>
+                                                                                       : cache_read_kernel<128>;
+    KZ_CHECK_CUDA(launch_pdl(kernel, grid, dim3(kCacheThreads), 0, s, a));
+    return KZ_OK;
+}
+
+extern "C" int kz_cache_keep(const kz_cache* cache, const int32_t* table, int64_t table_cols, const int32_t* lengths,
+                             const int32_t* path, const int32_t* count, int64_t batch, int64_t nodes,
+                             kz_stream_t stream) {
+    KeepArgs a;
+    int st = cache_view(cache, "kz_cache_keep", &a.c);
+    if (!st) st = seq_view(table, table_cols, lengths, batch, "kz_cache_keep", &a.s);
+    if (st) return st;
+    KZ_REQUIRE(nodes >= 0 && nodes < (1 << 24), "kz_cache_keep: nodes out of range");
+    KZ_REQUIRE(batch < (int64_t)INT32_MAX / cache->kv_heads, "kz_cache_keep: batch * kv_heads out of range");
+    if (batch * nodes == 0) return KZ_OK;
+    KZ_REQUIRE(path && count, "kz_cache_keep: path or count is NULL");
+    st = check_device();
+    if (st) return st;
+    a.path = path;
+    a.count = count;
+    a.batch = (int)batch;
+    a.nodes = (int)nodes;
+    a.status = device_status_ptr();
+    const int64_t warps = batch * cache->kv_heads;
+    const dim3 grid((unsigned)((warps + kCacheThreads / 32 - 1) / (kCacheThreads / 32)));
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    auto kernel = cache->head_dim == 32 ? cache_keep_kernel<32> : cache->head_dim == 64 ? cache_keep_kernel<64>
+                                                                                       : cache_keep_kernel<128>;
+    KZ_CHECK_CUDA(launch_pdl(kernel, grid, dim3(kCacheThreads), 0, s, a));
+    return KZ_OK;
+}

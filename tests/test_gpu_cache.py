@@ -1,0 +1,529 @@
+"""The int8 K/V cache on the GPU against plain implementations in 64 bits:
+writing (codes and scales bit for bit), reading back, moving an accepted path,
+attention for tokens, chunks and trees, verification of drafted trees, and the
+whole of it as a generation loop uses it.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import cpu as ocpu
+
+pytestmark = pytest.mark.gpu
+
+
+def _dev(a, dtype=None):
+    return torch.from_numpy(np.ascontiguousarray(a)).to("cuda", dtype)
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def _status():
+    from kansaiml_b200 import quantize as kq
+    return kq.device_status()
+
+
+class Book:
+    """A cache with the pages of some sequences, in random order, and the same
+    tokens' codes and scales kept on the host, position by position."""
+
+    def __init__(self, totals, kv_heads=2, d=64, page=32, seed=0, spare=2):
+        from kansaiml_b200.cache import QCache
+        rs = self.rs = np.random.RandomState(seed)
+        need = [-(-n // page) for n in totals]
+        order = rs.permutation(sum(need) + spare)
+        table = np.full((len(totals), max(need + [1]) + 1), -1, np.int32)
+        at = 0
+        for i, n in enumerate(need):
+            table[i, :n] = order[at:at + n]
+            at += n
+        self.table_h, self.table = table, _dev(table)
+        self.page, self.d, self.kv, self.batch = page, d, kv_heads, len(totals)
+        self.cache = QCache(len(order), kv_heads, d, page, device="cuda")
+        for t, fill in ((self.cache.k_codes, 77), (self.cache.v_codes, -77), (self.cache.k_scale, math.nan),
+                        (self.cache.v_scale, math.inf)):
+            t.fill_(fill)      # what nothing has written: never to be seen
+
+    def fill(self, lengths, seed=1, spread=1.0):
+        """Random codes and scales at positions below lengths; returns (k, v) lists of float64 [n, kv, d]."""
+        rs = np.random.RandomState(seed)
+        out = []
+        for codes, scale in ((self.cache.k_codes, self.cache.k_scale), (self.cache.v_codes, self.cache.v_scale)):
+            c, s = codes.cpu().numpy(), scale.cpu().numpy()
+            vals = []
+            for b, n in enumerate(lengths):
+                cc = rs.randint(-127, 128, (n, self.kv, self.d)).astype(np.int8)
+                ss = (np.exp(rs.uniform(-spread, spread, (n, self.kv))) / 127).astype(np.float32)
+                pos = np.arange(n)
+                c[self.table_h[b, pos // self.page], :, pos % self.page] = cc
+                s[self.table_h[b, pos // self.page], :, pos % self.page] = ss
+                vals.append(cc.astype(np.float64) * ss[..., None].astype(np.float64))
+            codes.copy_(torch.from_numpy(c))
+            scale.copy_(torch.from_numpy(s))
+            out.append(vals)
+        return out
+
+    def held(self):
+        return [t.cpu().numpy().copy() for t in (self.cache.k_codes, self.cache.k_scale, self.cache.v_codes,
+                                                 self.cache.v_scale)]
+
+
+# -------------------------------------------------------------------- write
+
+def _quantized(x):
+    """quantize.py:66-70 of each row of x [.., d]: codes, double scales."""
+    q, s = ocpu.quantize_rows(np.ascontiguousarray(x.reshape(-1, x.shape[-1])))
+    return q.reshape(x.shape), s.reshape(x.shape[:-1])
+
+
+@pytest.mark.parametrize("d,kv,page,lengths,counts,tokens", [
+    (64, 4, 64, [0, 63, 64, 200], None, 1),                # single tokens, first and last slots of pages
+    (128, 2, 16, [0, 5, 31], [37, 0, 9], 37),              # ragged, pages that end inside the rows, none at all
+    (32, 3, 32, [7], None, 65),                            # an odd number of heads
+    (128, 1, 128, [1, 100], [3, 130], 130),
+    (64, 8, 64, [0], None, 300),
+])
+@pytest.mark.parametrize("values", [False, True])
+def test_write_is_bit_exact(cuda_device, d, kv, page, lengths, counts, tokens, values):
+    """Codes and scales equal the reference's rule row by row; every other slot
+    and the rows past a count stay as they were; the values are the codes times
+    the kept scale, one fp32 rounding; k and v are strided columns."""
+    n = [tokens] * len(lengths) if counts is None else counts
+    book = Book([a + b for a, b in zip(lengths, n)], kv, d, page, seed=d + page)
+    before = book.held()
+    rs = np.random.RandomState(tokens)
+    x = rs.standard_normal((len(lengths), tokens, 3 * kv * d)).astype(np.float32)
+    x[0, 0, kv * d:kv * d + d] = 0                          # a row of zeros: scale 1
+    x[-1, -1, 2 * kv * d:2 * kv * d + d] = np.arange(d) - d / 2 + 0.5   # ties
+    x[:, :, kv * d + 1] *= 30
+    xd = _dev(x)
+    got = book.cache.write(xd[:, :, kv * d:2 * kv * d], xd[:, :, 2 * kv * d:], book.table, _i32(lengths),
+                           None if counts is None else _i32(counts), values=values)
+    after = book.held()
+    for part in range(2):
+        rows = x[:, :, (1 + part) * kv * d:(2 + part) * kv * d].reshape(len(lengths), tokens, kv, d)
+        codes, scales = _quantized(rows)
+        c, s = before[2 * part], before[2 * part + 1]
+        stood = np.zeros(rows.shape, np.float32)
+        for b, m in enumerate(n):
+            pos = lengths[b] + np.arange(m)
+            c[book.table_h[b, pos // page], :, pos % page] = codes[b, :m]
+            s[book.table_h[b, pos // page], :, pos % page] = scales[b, :m].astype(np.float32)
+            stood[b, :m] = codes[b, :m].astype(np.float32) * scales[b, :m, :, None].astype(np.float32)
+        np.testing.assert_array_equal(after[2 * part], c)
+        assert after[2 * part + 1].tobytes() == s.tobytes()
+        if values:
+            np.testing.assert_array_equal(got[part].numpy(), stood.reshape(len(lengths), tokens, kv * d))
+    assert values or got is None
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_write_marks_rows_that_are_not_finite(cuda_device, bad):
+    from kansaiml_b200 import _lib
+    book = Book([4], 2, 32, 16)
+    k = torch.randn(1, 4, 64, device="cuda")
+    v = torch.randn(1, 4, 64, device="cuda")
+    k[0, 2, 40] = bad
+    book.cache.write(k, v, book.table, _i32([0]))
+    assert _status() == _lib.KZ_ERR_NONFINITE
+    codes, scale = book.cache.k_codes[book.table_h[0, 0]], book.cache.k_scale[book.table_h[0, 0]]
+    assert torch.isnan(scale[1, 2]) and not codes[1, 2].any()
+    assert torch.isfinite(scale[:, :4]).sum() == 7
+
+
+@pytest.mark.parametrize("scale", [1e-42, 1e-33, 1e-30, 3e38])
+def test_write_at_the_ends_of_the_range(cuda_device, scale):
+    """Rows whose absmax is subnormal, below and above the fast path's border, and near the largest float."""
+    book = Book([50], 1, 64, 64)
+    x = (np.random.RandomState(3).uniform(-1, 1, (1, 50, 64)) * scale).astype(np.float32)
+    book.cache.write(_dev(x), _dev(x), book.table, _i32([0]))
+    codes, scales = _quantized(x.reshape(50, 64))
+    np.testing.assert_array_equal(book.cache.v_codes[book.table_h[0, 0], 0, :50].cpu().numpy(), codes)
+    np.testing.assert_array_equal(book.cache.k_scale[book.table_h[0, 0], 0, :50].cpu().numpy(), scales.astype(np.float32))
+    assert _status() == 0
+
+
+def test_write_copies_views_a_kernel_cannot_read(cuda_device):
+    """Odd offsets, transposed and broadcast inputs, and another dtype give the same codes."""
+    base = torch.randn(2, 5, 131, device="cuda")
+    want = Book([5, 5], 2, 64, 16)
+    x = base[:, :, 3:131].contiguous()
+    want.cache.write(x, x, want.table, _i32([0, 0]))
+    for k in (base[:, :, 3:131], x.transpose(1, 2).contiguous().transpose(1, 2), x.double()):
+        book = Book([5, 5], 2, 64, 16)
+        book.cache.write(k, x, book.table, _i32([0, 0]))
+        for a, b in zip(book.held(), want.held()):
+            assert a.tobytes() == b.tobytes()
+    one = Book([5, 5], 2, 64, 16)
+    one.cache.write(x[:, :1].expand(2, 5, 128), x[:1].expand(2, 5, 128), one.table, _i32([0, 0]))
+    full = Book([5, 5], 2, 64, 16)
+    full.cache.write(x[:, :1].repeat(1, 5, 1), x[:1].repeat(2, 1, 1), full.table, _i32([0, 0]))
+    for a, b in zip(one.held(), full.held()):
+        assert a.tobytes() == b.tobytes()
+
+
+# --------------------------------------------------------------------- read
+
+@pytest.mark.parametrize("d,kv,page,lengths,most", [
+    (64, 4, 32, [33, 0, 64, 1], 64), (128, 1, 128, [300, 129], 300), (32, 3, 16, [5], 200), (128, 8, 64, [70, 65], 66),
+    (32, 1, 16, [0, 0], 3), (64, 2, 64, [10], 0),
+])
+def test_read_back(cuda_device, d, kv, page, lengths, most):
+    """fl32(code * scale) of every token, zeros past a length, nothing past `most`."""
+    book = Book(lengths, kv, d, page, seed=page)
+    vals = book.fill(lengths)
+    got = book.cache.read(book.table, _i32(lengths), most)
+    for part in range(2):
+        want = np.zeros((len(lengths), most, kv * d), np.float32)
+        for b, n in enumerate(lengths):
+            n = min(n, most)
+            want[b, :n] = vals[part][b][:n].reshape(n, kv * d).astype(np.float32)
+        np.testing.assert_array_equal(got[part].numpy(), want)
+    assert _status() == 0
+
+
+# --------------------------------------------------------------------- keep
+
+@pytest.mark.parametrize("d,kv,page", [(32, 3, 16), (64, 4, 64), (128, 2, 32)])
+def test_keep_moves_paths_in_place(cuda_device, d, kv, page):
+    """Long, short, unmoved and empty paths; other slots stay as they were."""
+    lengths, nodes = [14, 0, 63, 5, 30], 70
+    paths = [[0, 2, 5, 6, 9], [0], [], list(range(0, 70, 2)) + [69], list(range(1, 70))]
+    book = Book([n + nodes for n in lengths], kv, d, page, seed=5)
+    book.fill([n + nodes for n in lengths])
+    want = book.held()
+    path = np.full((5, nodes), -1, np.int32)
+    for b, p in enumerate(paths):
+        path[b, :len(p)] = p
+        for i, j in enumerate(p):
+            new, old = lengths[b] + i, lengths[b] + j
+            for x in want:
+                x[book.table_h[b, new // page], :, new % page] = x[book.table_h[b, old // page], :, old % page].copy()
+    book.cache.keep(book.table, _i32(lengths), _dev(path), _i32([len(p) for p in paths]))
+    for a, b in zip(book.held(), want):
+        assert a.tobytes() == b.tobytes()
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("path,count", [([0, 2, 2, -1], 3), ([0, 4, -1, -1], 2), ([-1, 1, 2, 3], 2), ([1, 0, 2, 3], 4),
+                                        ([0, 1, 2, 3], 5), ([0, 1, 2, 3], -1)])
+def test_keep_refuses_paths_that_are_none(cuda_device, path, count):
+    from kansaiml_b200 import _lib
+    book = Book([8, 8], 1, 32, 16)
+    book.fill([8, 8])
+    before = book.held()
+    book.cache.keep(book.table, _i32([4, 4]), _i32([path, [0, 1, 2, 3]]), _i32([count, 4]))
+    assert _status() == _lib.KZ_ERR_INVALID_ARGUMENT
+    for a, b in zip(book.held(), before):
+        assert a.tobytes() == b.tobytes()
+
+
+# ---------------------------------------------------------------- attention
+
+def _sees(parents, tokens, t):
+    if parents is None:
+        return list(range(t + 1))
+    out = []
+    while t >= 0:
+        out.append(t)
+        up = int(parents[t])
+        t = up if 0 <= up < t else -1
+    return out
+
+
+def _attention_64(q, kvals, vvals, length, count, heads, parents, scale):
+    """One sequence in float64: output [tokens, heads * d] and the bound on a
+    32-bit kernel's error.  A product q . k of d terms whose factors are held to
+    22 bits or more and summed in 32 bits, each addition off by at most
+    2^-23 of the terms' absolute sum, is off by (d + 4) 2^-23 sum |q k|; a
+    weight's relative error is twice that (its own and the largest's) plus the
+    exponential's and its own 22 bits; the weighted sum of n values adds
+    2^-23 for each 16 keys that a partial sum covers, and 32 for the joining."""
+    tokens, kv, d = q.shape[0], kvals.shape[1], kvals.shape[2]
+    out, bound = np.zeros((tokens, heads * d)), np.zeros((tokens, heads * d))
+    for t in range(count):
+        seen = np.array(list(range(length)) + [length + j for j in _sees(parents, tokens, t)])
+        for h in range(heads):
+            k, v = kvals[seen, h * kv // heads], vvals[seen, h * kv // heads]
+            qq = q[t, h * d:(h + 1) * d].astype(np.float64)
+            s = k @ qq * scale
+            e = np.exp(s - s.max())
+            w = e / e.sum()
+            out[t, h * d:(h + 1) * d] = w @ v
+            off = 2 * (d + 4) * (np.abs(k) @ np.abs(qq)).max() * scale + 16 + len(seen) / 16 + 32
+            bound[t, h * d:(h + 1) * d] = off * 2.0**-23 * (w @ np.abs(v))
+    return out, bound
+
+
+def _check_attention(book, lengths, counts, tokens, heads, parents=None, seed=9, spread=1.0, strong=1.5, view=False,
+                     scale=None):
+    n = [tokens] * len(lengths) if counts is None else counts
+    kvals, vvals = book.fill([a + b for a, b in zip(lengths, n)], seed=seed, spread=spread)
+    q = (np.random.RandomState(seed).standard_normal((len(lengths), tokens, heads * book.d)) * strong).astype(np.float32)
+    qd = _dev(q)
+    if view:     # columns of a fused projection
+        wide = torch.full((len(lengths), tokens, heads * book.d + 64), math.nan, device="cuda")
+        wide[:, :, 32:-32] = qd
+        qd = wide[:, :, 32:-32]
+    pd = None if parents is None else _dev(np.asarray(parents, np.int32))
+    y = book.cache.attention(qd, heads, book.table, _i32(lengths), None if counts is None else _i32(counts), pd,
+                             scale).numpy()
+    for b in range(len(lengths)):
+        par = None if parents is None else np.asarray(parents) if np.ndim(parents) == 1 else np.asarray(parents)[b]
+        want, bound = _attention_64(q[b], kvals[b], vvals[b], lengths[b], n[b], heads, par,
+                                    1 / math.sqrt(book.d) if scale is None else scale)
+        off = np.abs(y[b] - want)
+        assert np.all(off <= bound), (b, (off - bound).max(), (off / np.maximum(bound, 1e-300)).max())
+        assert not y[b, n[b]:].any()
+    assert _status() == 0
+    return y
+
+
+@pytest.mark.parametrize("d,kv,heads,page", [(64, 4, 4, 64), (128, 2, 8, 16), (128, 1, 32, 128), (32, 3, 9, 32),
+                                             (64, 2, 14, 32), (128, 2, 2, 64)])
+def test_attention_single_tokens(cuda_device, d, kv, heads, page):
+    """One new token a sequence, lengths from none to several tiles and their neighbours."""
+    lengths = [0, 1, 15, 16, 31, 63, 64, 127, 128, 255, 300, 1030]
+    book = Book([n + 1 for n in lengths], kv, d, page, seed=heads)
+    _check_attention(book, lengths, None, 1, heads, view=heads == kv)
+
+
+@pytest.mark.parametrize("d,kv,heads,page,tokens", [(64, 2, 2, 64, 5), (128, 1, 4, 32, 33), (32, 2, 8, 16, 130),
+                                                    (128, 2, 4, 128, 70), (64, 1, 3, 64, 17)])
+def test_attention_chunks(cuda_device, d, kv, heads, page, tokens):
+    """Several new tokens, causal among themselves, with padding rows, none at all, and no context."""
+    lengths, counts = [0, 40, 200, 77], [tokens, 1, 0, tokens - 2]
+    book = Book([a + b for a, b in zip(lengths, counts)], kv, d, page, seed=tokens)
+    _check_attention(book, lengths, counts, tokens, heads, view=tokens == 33)
+
+
+def _tree(n, seed, deep=False):
+    rs = np.random.RandomState(seed)
+    return [-1] + [j - 1 if deep else int(rs.randint(0, j)) for j in range(1, n)]
+
+
+@pytest.mark.parametrize("d,kv,heads,page,nodes", [(64, 4, 4, 64, 6), (128, 2, 8, 64, 24), (128, 1, 8, 32, 64),
+                                                   (32, 2, 2, 16, 256), (64, 2, 6, 128, 100)])
+def test_attention_trees(cuda_device, d, kv, heads, page, nodes):
+    """A random tree a sequence, one of them a chain, one a star, one of roots only."""
+    lengths, counts = [100, 0, 64, 37], [nodes, nodes - 1, nodes, nodes]
+    parents = [_tree(nodes, 1), _tree(nodes, 2, deep=True), [-1] + [0] * (nodes - 1), [-1] * nodes]
+    book = Book([a + b for a, b in zip(lengths, counts)], kv, d, page, seed=nodes)
+    _check_attention(book, lengths, counts, nodes, heads, parents)
+
+
+def test_attention_one_tree_for_all_and_odd_parents(cuda_device):
+    """parents [nodes] serves every sequence; a parent that is not before its child is none."""
+    book = Book([60, 61], 2, 64, 16)
+    _check_attention(book, [50, 51], None, 10, 4, _tree(10, 3))
+    _check_attention(book, [50, 51], None, 10, 4, [[-1, 0, 5, 2, 99, 4, -7, 7, 7, 3], _tree(10, 4)])
+
+
+def test_attention_chain_is_causal(cuda_device):
+    """A tree that is a chain gives what no tree gives, bit for bit."""
+    book = Book([90, 133], 2, 64, 32)
+    a = _check_attention(book, [57, 100], None, 33, 4, _tree(33, 0, deep=True))
+    b = _check_attention(book, [57, 100], None, 33, 4)
+    assert a.tobytes() == b.tobytes()
+
+
+@pytest.mark.parametrize("tokens", [1, 12])
+@pytest.mark.parametrize("spread,strong", [(12.0, 1e-4), (0.5, 12.0), (30.0, 1e-12), (1.0, 0.0), (1.0, 1e-30)])
+def test_attention_extreme_scales(cuda_device, tokens, spread, strong):
+    """Scales over many orders of magnitude, nearly one-hot softmaxes, q of zeros and of tiny values."""
+    book = Book([401, 200], 2, 64, 64)
+    _check_attention(book, [401 - tokens, 200 - tokens], None, tokens, 4, spread=spread, strong=strong)
+
+
+def test_attention_scale_argument(cuda_device):
+    book = Book([300], 1, 32, 16)
+    _check_attention(book, [299], None, 1, 2, scale=0.03)
+    _check_attention(book, [299], None, 1, 2, scale=0.9)
+
+
+@pytest.mark.parametrize("lengths,tokens,heads,kv", [([20000], 1, 8, 1), ([9000, 3, 5000], 1, 2, 2), ([7000], 40, 4, 1)])
+def test_attention_long(cuda_device, lengths, tokens, heads, kv):
+    """Contexts that are split over many blocks and joined."""
+    book = Book([n + tokens for n in lengths], kv, 128, 64)
+    _check_attention(book, lengths, None, tokens, heads)
+
+
+def test_attention_is_repeatable_and_independent_of_the_batch(cuda_device):
+    """The same call gives the same bits."""
+    book = Book([3000, 700], 2, 128, 64)
+    lengths = [2999, 699]
+    a = _check_attention(book, lengths, None, 1, 8)
+    for _ in range(3):
+        assert _check_attention(book, lengths, None, 1, 8).tobytes() == a.tobytes()
+
+
+def test_attention_nan_in_a_visible_row_only(cuda_device):
+    """A NaN scale in a token's row reaches the rows that see it and no others."""
+    book = Book([70], 2, 64, 32)
+    book.fill([70])
+    q = torch.randn(1, 6, 4 * 64, device="cuda")
+    # node 65's V row of head 1: seen by itself and its descendants (nodes 1 and 3 of the tree)
+    book.cache.v_scale[book.table_h[0, 65 // 32], 1, 65 % 32] = math.nan
+    y = book.cache.attention(q, 4, book.table, _i32([64]), None, _i32([-1, 0, 0, 1, 2, 0])).data.view(6, 4, 64)
+    bad = torch.isnan(y).all(-1).cpu()
+    want = torch.zeros(6, 4, dtype=torch.bool)
+    want[1, 2:] = want[3, 2:] = True
+    assert torch.equal(bad, want) and torch.equal(torch.isnan(y).any(-1).cpu(), want)
+
+
+def test_bad_pages_are_left_out_and_reported(cuda_device):
+    """A page number outside the pool, or a position past the table, reads and writes nothing."""
+    from kansaiml_b200 import _lib
+    for wrong in (10 ** 6, -2):
+        book = Book([40], 1, 64, 16)
+        kvals, vvals = book.fill([40])
+        table = book.table.clone()
+        table[0, 1] = wrong
+        q = torch.randn(1, 1, 64, device="cuda")
+        y = book.cache.attention(q, 1, table, _i32([39])).numpy()[0, 0]
+        assert _status() == _lib.KZ_ERR_INVALID_ARGUMENT
+        seen = np.r_[0:16, 32:40]
+        want, bound = _attention_64(q.cpu().numpy()[0], kvals[0][seen], vvals[0][seen], len(seen) - 1, 1, 1, None, 1 / 8)
+        assert np.all(np.abs(y - want[0]) <= bound[0])
+        k, v = book.cache.read(table, _i32([40]), 40)
+        assert _status() == _lib.KZ_ERR_INVALID_ARGUMENT
+        assert not k.data[0, 16:32].any() and not v.data[0, 16:32].any()
+        np.testing.assert_array_equal(k.numpy()[0, seen], kvals[0][seen, 0].astype(np.float32))
+        before = book.held()
+        book.cache.write(torch.randn(1, 3, 64, device="cuda"), torch.randn(1, 3, 64, device="cuda"), table, _i32([20]))
+        assert _status() == _lib.KZ_ERR_INVALID_ARGUMENT
+        book.cache.keep(table, _i32([20]), _i32([[1, 2]]), _i32([2]))
+        assert _status() == _lib.KZ_ERR_INVALID_ARGUMENT
+        for a, b in zip(book.held(), before):
+            assert a.tobytes() == b.tobytes()
+    # lengths past the table, and below 0
+    for length in (10 ** 9, -5):
+        book.cache.attention(torch.randn(1, 2, 64, device="cuda"), 1, book.table, _i32([length]))
+        book.cache.write(torch.randn(1, 3, 64, device="cuda"), torch.randn(1, 3, 64, device="cuda"), book.table,
+                         _i32([length]))
+        assert _status() == _lib.KZ_ERR_INVALID_ARGUMENT
+    for a, b in zip(book.held(), before):
+        assert a.tobytes() == b.tobytes()
+
+
+def test_empty_calls(cuda_device):
+    book = Book([4], 2, 32, 16)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    z = torch.empty(0, 3, 64, device="cuda")
+    assert book.cache.attention(z, 2, book.table[:0], none).shape == [0, 3, 64]
+    book.cache.write(z, z, book.table[:0], none)
+    assert book.cache.attention(torch.empty(1, 0, 64, device="cuda"), 2, book.table, _i32([4])).shape == [1, 0, 64]
+    assert book.cache.read(book.table[:0], none, 5)[0].shape == [0, 5, 64]
+    assert _status() == 0
+
+
+# ------------------------------------------------------------- verification
+
+def _verify_64(tokens, parents, target, draft, au, su):
+    """One sequence, in float64, straight from the definition."""
+    n, vocab = target.shape
+    node, r, path = 0, target[0].astype(np.float64), [0]
+    for j in range(1, n):
+        if parents[j] != node or not 0 <= parents[j] < j or not 0 <= tokens[j] < vocab:
+            continue
+        q = draft[node].astype(np.float64) if draft is not None else np.eye(vocab)[tokens[j]]
+        if float(au[j]) * q[tokens[j]] < r[tokens[j]]:
+            node, r = j, target[j].astype(np.float64)
+            path.append(j)
+        else:
+            rest = np.maximum(r - q, 0)
+            if rest.sum() > 0:
+                r = rest / rest.sum()
+    below = np.cumsum(r)
+    return path, min(int(np.searchsorted(below, float(su) * below[-1], side="right")), vocab - 1)
+
+
+def _softmax(rs, shape, strength):
+    x = rs.standard_normal(shape) * strength
+    e = np.exp(x - x.max(-1, keepdims=True))
+    return (e / e.sum(-1, keepdims=True)).astype(np.float32)
+
+
+@pytest.mark.parametrize("batch,nodes,vocab,draft", [
+    (40, 8, 65, True), (40, 8, 65, False), (5, 1, 1, False), (9, 1, 50000, False), (7, 24, 2049, True), (3, 40, 100003, True),
+    (3, 40, 32768, False), (2, 300, 33, True), (16, 5, 2, True),
+])
+@pytest.mark.parametrize("shared", [False, True])
+def test_verify_tree(cuda_device, batch, nodes, vocab, draft, shared):
+    from kansaiml_b200.cache import verify_tree
+    rs = np.random.RandomState(batch * nodes + vocab)
+    target = _softmax(rs, (batch, nodes, vocab), 2.0)
+    q = (0.6 * target + 0.4 * _softmax(rs, (batch, nodes, vocab), 2.0)).astype(np.float32)
+    parents = np.array([_tree(nodes, 7 if shared else 100 + b) for b in range(batch)], np.int32)
+    tokens = np.zeros((batch, nodes), np.int64)
+    for b in range(batch):
+        for j in range(1, nodes):
+            p = q[b, parents[b, j]].astype(np.float64)
+            tokens[b, j] = rs.choice(vocab, p=p / p.sum())
+    au, su = rs.uniform(size=(batch, nodes)).astype(np.float32), rs.uniform(size=batch).astype(np.float32)
+    path, count, token = verify_tree(_dev(tokens), _dev(parents[0] if shared else parents), _dev(target),
+                                     _dev(q) if draft else None, _dev(au), _dev(su))
+    path, count, token = path.cpu().numpy(), count.cpu().numpy(), token.cpu().numpy()
+    for b in range(batch):
+        want, nxt = _verify_64(tokens[b], parents[b], target[b], q[b] if draft else None, au[b], su[b])
+        assert path[b].tolist() == want + [-1] * (nodes - len(want)), b
+        assert count[b] == len(want) and token[b] == nxt, b
+    assert _status() == 0
+
+
+def test_verify_edges(cuda_device):
+    """u = 0 and the largest u below 1, zeros around the mass, a draft that equals
+    the target, the same token twice, and rows that are no distribution."""
+    from kansaiml_b200.cache import verify_tree
+    top = np.nextafter(np.float32(1), np.float32(0))
+    v = 3000
+    p = np.zeros((6, 3, v), np.float32)
+    p[:, :, 1000] = 0.25
+    p[:, :, 2500] = 0.75
+    q = p.copy()
+    q[3:, 0] = 0
+    q[3:, 0, 7] = 1                                          # token 7 has no mass in the target
+    tokens = np.array([[0, 1000, 2500]] * 3 + [[0, 7, 7]] * 3, np.int64)
+    parents = np.array([[-1, 0, 0]] * 6, np.int32)
+    au = np.array([[0, 0, 0], [0, top, top], [0, top, 0], [0, 0, 0], [0, top, top], [0, 0.5, 0.5]], np.float32)
+    su = np.array([0, top, 0.25, 0, top, 0.2499999], np.float32)
+    for draft in (q, None):
+        path, count, token = verify_tree(_dev(tokens), _dev(parents), _dev(p), None if draft is None else _dev(draft),
+                                         _dev(au), _dev(su))
+        for b in range(6):
+            want, nxt = _verify_64(tokens[b], parents[b], p[b], None if draft is None else draft[b], au[b], su[b])
+            assert path[b].tolist() == want + [-1] * (3 - len(want)) and count[b] == len(want) and token[b] == nxt, b
+    # no mass at all, and tokens and parents that are none: an answer inside the vocabulary, nothing read outside
+    path, count, token = verify_tree(_dev(np.array([[0, -1, v]])), _i32([[5, 0, 0]]), torch.zeros(1, 3, v, device="cuda"),
+                                     None, torch.rand(1, 3, device="cuda"), torch.rand(1, device="cuda"))
+    from kansaiml_b200 import _lib
+    assert _status() == _lib.KZ_ERR_INVALID_ARGUMENT
+    assert count.tolist() == [1] and path.tolist() == [[0, -1, -1]] and token.tolist() == [v - 1]
+
+
+@pytest.mark.parametrize("draft", [True, False])
+def test_verified_tokens_follow_the_target(cuda_device, draft):
+    """Whatever is drafted, the token after the root is distributed as the
+    target's row: 20000 trees of four drafts from a wrong distribution.  Each
+    frequency is within 5 standard deviations (a chance of 6e-7 each) of p."""
+    from kansaiml_b200.cache import verify_tree
+    n, v = 20000, 6
+    rs = np.random.RandomState(11)
+    p = np.array([0.4, 0.05, 0.25, 0.0, 0.2, 0.1], np.float32)
+    q = np.array([0.1, 0.3, 0.2, 0.2, 0.1, 0.1], np.float32)
+    target = np.broadcast_to(p, (n, 5, v))
+    tokens = np.concatenate([np.zeros((n, 1)), rs.choice(v, (n, 4), p=q.astype(np.float64) / q.astype(np.float64).sum())],
+                            1).astype(np.int64)
+    path, count, token = verify_tree(_dev(tokens), _i32([-1, 0, 0, 0, 0]), _dev(target),
+                                     _dev(np.broadcast_to(q, (n, 5, v))) if draft else None,
+                                     _dev(rs.uniform(size=(n, 5)).astype(np.float32)),
+                                     _dev(rs.uniform(size=n).astype(np.float32)))
+    path, count, token = path.cpu().numpy(), count.cpu().numpy(), token.cpu().numpy()
+    first = np.where(count > 1, tokens[np.arange(n), np.maximum(path[:, 1], 0)], token)
+    seen = np.bincount(first, minlength=v) / n
+    assert np.all(np.abs(seen - p) <= 5 * np.sqrt(p * (1 - p) / n) + 1e-12), seen
