@@ -358,11 +358,15 @@ int kz_cache_keep(const kz_cache* cache, const int32_t* table, int64_t table_col
  * itself in the tree (parents[b * parents_batch_stride + t], -1 or anything
  * that is not below t: none; tokens <= KZ_TREE_MAX_NODES) or, parents NULL,
  * every one up to itself.  out [batch, tokens, heads * head_dim] contiguous;
- * rows past counts[b], and rows that see no key, are 0. */
+ * rows past counts[b], and rows that see no key, are 0.  batch < 65536.
+ * `workspace` (16-byte aligned device memory, scratch of this call alone) must
+ * hold kz_cache_attention_workspace_bytes(...) bytes, 0 for short tables. */
+size_t kz_cache_attention_workspace_bytes(const kz_cache* cache, int64_t tokens, int64_t heads, int64_t table_cols);
 int kz_cache_attention_f32(const kz_cache* cache, const float* q, int64_t batch, int64_t tokens, int64_t heads,
                            int64_t q_batch_stride, int64_t q_row_stride, const int32_t* table, int64_t table_cols,
                            const int32_t* lengths, const int32_t* counts, const int32_t* parents,
-                           int64_t parents_batch_stride, float scale, float* out, kz_stream_t stream);
+                           int64_t parents_batch_stride, float scale, float* out, void* workspace,
+                           size_t workspace_bytes, kz_stream_t stream);
 
 /* Verifies a tree of drafted tokens (node 0 the root, parents[n] < n; other
  * values make no child) against the target's probabilities target[batch, nodes,

@@ -69,7 +69,8 @@ SIGNATURES = {
     "kz_cache_read_f32": (_I, [ctypes.POINTER(KzCache), _P, _I64, _P, _I64, _I64, _P, _P, _P]),
     "kz_cache_keep": (_I, [ctypes.POINTER(KzCache), _P, _I64, _P, _P, _P, _I64, _I64, _P]),
     "kz_cache_attention_f32": (_I, [ctypes.POINTER(KzCache), _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _P,
-                                    _I64, _F, _P, _P]),
+                                    _I64, _F, _P, _P, _SZ, _P]),
+    "kz_cache_attention_workspace_bytes": (_SZ, [ctypes.POINTER(KzCache), _I64, _I64, _I64]),
     "kz_verify_tree_f32": (_I, [_P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P]),
     "kz_peer_alloc": (_I, [_SZ, ctypes.POINTER(_P), _P]),
     "kz_peer_open": (_I, [_P, ctypes.POINTER(_P)]),

@@ -198,9 +198,11 @@ class QCache:
                 raise ValueError(f"attention: a tree has at most {_lib.KZ_TREE_MAX_NODES} nodes (got {tokens})")
             parents, pb = _parents(parents, batch, tokens, self.device)
         out = torch.empty((batch, tokens, heads * self.head_dim), dtype=torch.float32, device=self.device)
+        need = _lib.load().kz_cache_attention_workspace_bytes(self._ref, tokens, heads, cols)
+        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         _on(self.device, "kz_cache_attention_f32", self._ref, ptr(q), batch, tokens, heads, qb, qr, ptr(table), cols,
             ptr(lengths), ptr(counts), ptr(parents), pb, 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
-            ptr(out))
+            ptr(out), ptr(work), need)
         return Tensor(out)
 
     def keep(self, table, lengths, path, count):

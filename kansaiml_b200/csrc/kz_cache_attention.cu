@@ -1,23 +1,53 @@
 // Attention over the paged int8 K/V cache: single tokens, chunks of a prompt,
 // trees of drafted tokens.
 //
-//   s_l = (q . c_l) * ks_l / sqrt(d)      c_l, ks_l: key l's codes and scale
+//   s_l = (q . c_l) * ks_l * scale        c_l, ks_l: key l's codes and scale
 //   o   = sum_l w_l * (vs_l * cv_l),  w = softmax(s) over the visible keys
 //
 // The new tokens' own K/V are in the cache already (positions length ..
 // length + count - 1).  New token t sees every token before the new ones, and
 // of the new ones its ancestors and itself in the tree (parents) or, without
 // a tree, every one up to itself.  Rows past a sequence's count are 0.
+//
+// Arithmetic.  An int8 code is exact in fp16, so both products run on the
+// tensor cores with the codes as they are, and the fp32 operand (q, and the
+// weights times vs) as the sum of two fp16 values, which keeps 22 bits of it:
+// q is scaled by a power of two per row so that its largest value lies in
+// [2^13, 2^14), w * vs by one per warp, so that no half is lost to fp16's
+// range.  Sums are 32-bit; the tensor core's sum of a step of keys is added to
+// the row's sum by an fp32 multiply-add that also carries the softmax's
+// rescaling, so that long contexts do not add up its truncation.
+//
+// Work.  The rows of one key head (its `group` query heads times the new
+// tokens) form tiles of RT rows.  S^T = K Q^T and O^T = V^T P^T put the keys
+// (the head's width) on the 16-row side of the mma and the query rows on its
+// 8-column side, so that 8 rows, not 16, are the smallest tile and each code
+// is converted once for all of a warp's rows.  The four warps of a CTA split
+// the keys of a tile (KG ways) and the rows (RG ways); each keeps its own
+// running maximum and sum, joined at the end.  A fifth warp streams the pages
+// by TMA (swizzled over the row, so ldmatrix reads without conflicts) into a
+// ring of tiles of 128 keys.
+//
+// The keys of all sequences are cut into equal ranges, one per CTA, two CTAs
+// a SM, so that ragged batches and long single sequences fill the GPU alike; a
+// (sequence, head, row tile) that spans several ranges leaves its parts in the
+// workspace, and a second kernel joins them.
+#include <cuda_fp16.h>
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "kz_cache.cuh"
 
 namespace kz {
 namespace {
 
-constexpr int kCaThreads = 128;
+constexpr int kKT = 128;                    // keys a tile
+constexpr int kConsumers = 128;             // four warps compute, a fifth loads
+constexpr int kCaThreads = kConsumers + 32;
+constexpr int kMinTiles = 4;                // tiles a CTA's range has at least
+constexpr int kTreeWords = KZ_TREE_MAX_NODES / 32;
 
 struct CacheAttArgs {
     CacheView c;
@@ -28,66 +58,702 @@ struct CacheAttArgs {
     const int32_t* parents;
     int64_t parents_bs;
     float* out;
+    float* parts;          // two slots a CTA: sums [RT][D], maxima [RT], weights [RT]; NULL: every range is whole
     int batch, tokens, heads, group;
     float scale;
     int* status;
 };
 
-// A warp a (sequence, new token, head): one pass over the keys with the
-// running maximum and sum.
-template <int D>
-__global__ void __launch_bounds__(kCaThreads) cache_attention_kernel(CacheAttArgs a) {
-    constexpr int E = D / 32;
-    griddep_launch_dependents();
-    griddep_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t item = (int64_t)blockIdx.x * (kCaThreads / 32) + (threadIdx.x >> 5);
-    if (item >= (int64_t)a.batch * a.tokens * a.heads) return;
-    const int h = (int)(item % a.heads);
-    const int64_t bt = item / a.heads;
-    const int t = (int)(bt % a.tokens);
-    const int64_t b = bt / a.tokens;
-    const int count = a.counts ? min(a.counts[b], a.tokens) : a.tokens;
-    const int64_t len = min((int64_t)max(0, a.s.lengths[b]), (int64_t)a.s.cols * a.c.page);
-    const int32_t* parents = a.parents ? a.parents + b * a.parents_bs : nullptr;
-    const int kvh = h / a.group;
-    float q[E], o[E], m = -INFINITY, sum = 0.0f;
+template <int D, int NT_, int RG_>
+struct Shape {
+    static constexpr int NT = NT_, RG = RG_, KG = 4 / RG_;
+    static constexpr int RT = 8 * NT * RG;                  // rows a tile
+    static constexpr int STEPS = kKT / (32 * KG);           // steps of 32 keys a warp takes in a tile
+    static constexpr int STAGES = RT <= 16 ? 3 : 2;
+    static constexpr int CODES = kKT * D, STAGE = 2 * CODES + 2 * kKT * 4;
+    static constexpr int PITCH = D + 4;                     // joined rows: float2 stores without conflicts
+    static constexpr int QBYTES = RT * D * 4;               // both halves of q, as mma operands
+    static constexpr int UBYTES = KG > 1 && RT * PITCH * 4 > QBYTES ? RT * PITCH * 4 : QBYTES;
+    static constexpr int SMEM = STAGES * STAGE + UBYTES + 1024;
+    static constexpr int SLOT = RT * (D + 2);               // floats of a part
+};
+
+// ------------------------------------------------------------- the schedule
+
+// A sequence's share of the work.
+struct Seq {
+    int len, count, tiles, row_tiles;
+};
+template <int RT>
+__device__ __forceinline__ Seq sequence(const CacheAttArgs& a, int b) {
+    Seq s;
+    const int64_t most = (int64_t)a.s.cols * a.c.page;
+    s.len = (int)min((int64_t)max(0, a.s.lengths[b]), most);
+    s.count = a.counts ? max(0, min(a.counts[b], a.tokens)) : a.tokens;
+    s.tiles = (int)(((int64_t)s.len + s.count + kKT - 1) / kKT);
+    s.row_tiles = (int)(((int64_t)s.count * a.group + RT - 1) / RT);
+    return s;
+}
+__device__ __forceinline__ int64_t units_of(const CacheAttArgs& a, const Seq& s) {
+    return (int64_t)s.row_tiles * a.c.heads * (a.parts ? s.tiles : 1);   // whole ranges: a unit is a row tile
+}
+__device__ __forceinline__ int64_t units_a_cta(const CacheAttArgs& a, int64_t total, int ctas) {
+    const int64_t per = (total + ctas - 1) / ctas;
+    return a.parts ? max(per, (int64_t)kMinTiles) : max(per, (int64_t)1);
+}
+
+// Sum of a value over the 128 threads that share `sum` (named barrier 1).
+__device__ __forceinline__ int64_t sum_128(int64_t v, int64_t* sum) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        q[e] = a.q[b * a.q_bs + t * a.q_rs + (int64_t)h * D + lane * E + e] * a.scale;
-        o[e] = 0.0f;
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) sum[threadIdx.x >> 5] = v;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    return sum[0] + sum[1] + sum[2] + sum[3];
+}
+
+// A part of one (sequence, head, row tile): key tiles [t0, t1).
+struct Segment {
+    int b, h, rt, t0, t1;
+    int len, count;
+    int first_token, last_token;   // of the row tile
+    bool whole;                    // all of its tiles
+};
+
+// Walks the segments of units [at, end): b0, base: the sequence that holds `at` and its first unit.
+template <int RT>
+struct Walk {
+    int64_t at, end, base;
+    int b;
+    Seq s;
+    __device__ __forceinline__ bool next(const CacheAttArgs& a, Segment& g) {
+        if (at >= end) return false;
+        while (at >= base + units_of(a, s)) {
+            if (b + 1 >= a.batch) return false;
+            base += units_of(a, s);
+            s = sequence<RT>(a, ++b);
+        }
+        const int64_t off = at - base;
+        const int per = a.parts ? s.tiles : 1;
+        const int hr = (int)(off / per);
+        g.b = b;
+        g.h = hr / s.row_tiles;
+        g.rt = hr % s.row_tiles;
+        g.t0 = (int)(off % per);
+        const int take = (int)min((int64_t)(per - g.t0), end - at);
+        g.whole = take == per;
+        g.t1 = a.parts ? g.t0 + take : s.tiles;
+        at += take;
+        g.len = s.len;
+        g.count = s.count;
+        g.first_token = g.rt * RT / a.group;
+        g.last_token = min(s.count - 1, (g.rt * RT + RT - 1) / a.group);
+        g.t1 = min(g.t1, (g.len + g.last_token) / kKT + 1);   // later tiles: no row of this tile sees them
+        return true;
     }
-    int anc = t;   // the next visible node at or below the current one, walking up from t
-    if (t < count) {
-        for (int64_t l = len + t; l >= 0; --l) {
-            if (parents && l >= len) {
-                if (l - len != anc) continue;
-                const int up = parents[anc];
-                anc = up < anc ? up : -1;
+};
+
+// ------------------------------------------------------------ mma and codes
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t transposed_8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+// Two of a word's four codes (offset by 128) as fp16: the byte in the mantissa
+// of 1024, less 1152.
+template <int SEL>
+__device__ __forceinline__ uint32_t two_codes(uint32_t w) {
+    const uint32_t m = __byte_perm(w, 0x64646464u, SEL);
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(0x64806480u));
+    return r;
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// x's 11 leading bits; the rest, x less them, is exact
+__device__ __forceinline__ float leading(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFFE000u); }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// exp2(m - top), 0 where m is -inf (no key yet)
+__device__ __forceinline__ float shrink(float m, float top) { return m == -INFINITY ? 0.0f : exp2_approx(m - top); }
+__device__ __forceinline__ float pow2_field(int field) { return __uint_as_float((uint32_t)field << 23); }
+
+template <int D>
+__device__ __forceinline__ uint32_t swizzled(uint32_t off) {   // byte offset in a tile of rows of D bytes
+    return D == 128 ? off ^ ((off >> 3) & 0x70u) : D == 64 ? off ^ ((off >> 3) & 0x30u) : off ^ ((off >> 3) & 0x10u);
+}
+
+// ------------------------------------------------------------- the kernel
+
+template <int D, int NT, int RG>
+__global__ void __launch_bounds__(kCaThreads, 2)
+    cache_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                           const CacheAttArgs a) {
+    using S = Shape<D, NT, RG>;
+    extern __shared__ uint8_t ca_smem[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ca_smem) + 1023) & ~(uintptr_t)1023);
+    uint4* q_ops = reinterpret_cast<uint4*>(ring + S::STAGES * S::STAGE);   // [RT / 8][D / 16][32]: hi, hi, lo, lo
+    float* joined = reinterpret_cast<float*>(q_ops);                        // [RT][PITCH], once q is done with
+    __shared__ __align__(8) uint64_t s_full[S::STAGES], s_empty[S::STAGES];
+    __shared__ uint32_t s_bad[S::STAGES];          // pages of a tile that are not there
+    __shared__ float s_qs[S::RT];                  // a row's score factor
+    __shared__ float s_m[S::KG][S::RT], s_l[S::KG][S::RT];
+    __shared__ uint32_t s_sees[S::RT + 1][kTreeWords];
+    __shared__ int32_t s_parent[KZ_TREE_MAX_NODES];
+    __shared__ int64_t s_sum[4], s_part[kConsumers];
+    __shared__ int64_t s_start[2];                 // this CTA's first sequence and that one's first unit
+    __shared__ int64_t s_units[2];                 // its units
+    __shared__ int s_abort;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < S::STAGES; ++i) {
+            mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&s_empty[i]), 4);
+        }
+        s_abort = 0;
+        fence_mbarrier_init();
+    }
+    griddep_wait();
+    griddep_launch_dependents();
+
+    // ---- this CTA's units, and where they begin
+    if (warp < 4) {
+        const int each = (a.batch + kConsumers - 1) / kConsumers;
+        int64_t mine = 0;
+        for (int b = tid * each; b < min(a.batch, (tid + 1) * each); ++b) mine += units_of(a, sequence<S::RT>(a, b));
+        s_part[tid] = mine;
+        const int64_t total = sum_128(mine, s_sum);
+        if (tid == 0) {
+            const int64_t per = units_a_cta(a, total, gridDim.x);
+            const int64_t u0 = min(total, per * blockIdx.x), u1 = min(total, u0 + per);
+            s_units[0] = u0;
+            s_units[1] = u1;
+            int64_t base = 0;
+            int i = 0, b = 0;
+            if (u0 < u1) {
+                while (i < kConsumers - 1 && base + s_part[i] <= u0) base += s_part[i++];
+                b = i * each;
+                for (; b < a.batch - 1; ++b) {
+                    const int64_t n = units_of(a, sequence<S::RT>(a, b));
+                    if (u0 < base + n) break;
+                    base += n;
+                }
             }
-            const int page = page_of(a.c, a.s, b, l);
-            if (page < 0) {
-                if (lane == 0) record_status(a.status, KZ_ERR_INVALID_ARGUMENT);
-                continue;
-            }
-            const int64_t row = ((int64_t)page * a.c.heads + kvh) * a.c.page + (l & (a.c.page - 1));
-            float s = 0.0f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) s += q[e] * (float)a.c.codes[0][row * D + lane * E + e];
-#pragma unroll
-            for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            s *= a.c.scale[0][row];
-            const float top = fmaxf(m, s);
-            const float keep = expf(m - top), w = expf(s - top), vs = w * a.c.scale[1][row];
-            m = top;
-            sum = sum * keep + w;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = o[e] * keep + vs * (float)a.c.codes[1][row * D + lane * E + e];
+            s_start[0] = b;
+            s_start[1] = base;
         }
     }
+    __syncthreads();
+    Walk<S::RT> walk;
+    walk.at = s_units[0];
+    walk.end = s_units[1];
+    walk.b = (int)s_start[0];
+    walk.base = s_start[1];
+    if (walk.at < walk.end) walk.s = sequence<S::RT>(a, walk.b);
+    Segment g;
+    int it = 0;      // tiles loaded or used so far
+
+    if (warp == 4) {
+        // ---- the loader: a lane a page of the tile
+        const int pages = kKT >> a.c.shift;
+        while (walk.next(a, g)) {
+            const int held = g.len + g.count;                         // keys of the sequence
+            auto page_id = [&](int t) {
+                const int64_t pos = (int64_t)t * kKT + ((int64_t)lane << a.c.shift);
+                return lane < pages && t < g.t1 && pos < held ? page_of(a.c, a.s, g.b, pos) : -2;   // -2: none needed
+            };
+            int id = page_id(g.t0);
+            for (int t = g.t0; t < g.t1; ++t, ++it) {
+                const int stage = it % S::STAGES;
+                const int next = page_id(t + 1);
+                mbar_wait(smem_u32(&s_empty[stage]), ((it / S::STAGES) & 1) ^ 1, a.status, &s_abort);
+                const uint32_t there = __ballot_sync(0xffffffffu, id >= 0), bad = __ballot_sync(0xffffffffu, id == -1);
+                const uint32_t full = smem_u32(&s_full[stage]);
+                if (lane == 0) {
+                    s_bad[stage] = bad;
+                    if (bad) record_status(a.status, KZ_ERR_INVALID_ARGUMENT);
+                    mbar_arrive_expect_tx(full, __popc(there) * a.c.page * (2 * D + 8));
+                }
+                __syncwarp();
+                if (id >= 0) {
+                    const uint32_t at = smem_u32(ring + stage * S::STAGE);
+                    const int row = (id * a.c.heads + g.h) << a.c.shift, k0 = lane << a.c.shift;
+                    tma_load_2d(at + k0 * D, &tm_k, full, 0, row);
+                    tma_load_2d(at + S::CODES + k0 * D, &tm_v, full, 0, row);
+                    bulk_load(at + 2 * S::CODES + k0 * 4, a.c.scale[0] + row, a.c.page * 4, full);
+                    bulk_load(at + 2 * S::CODES + kKT * 4 + k0 * 4, a.c.scale[1] + row, a.c.page * 4, full);
+                }
+                id = next;
+            }
+        }
+    } else {
+        const int kg = warp / RG, rg = warp % RG, gq = lane >> 2, tq = lane & 3;
+        // rows past a sequence's count are 0
+        for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+            const int n = a.counts ? max(0, min(a.counts[b], a.tokens)) : a.tokens;
+            const int64_t row = (int64_t)a.heads * D;
+            float4* o = reinterpret_cast<float4*>(a.out + ((int64_t)b * a.tokens + n) * row);
+            for (int64_t i = tid; i < (a.tokens - n) * (row / 4); i += kConsumers) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        bool first_segment = true;
+        while (walk.next(a, g)) {
+            const int rows = min(S::RT, g.count * a.group - g.rt * S::RT);   // of this tile
+            // ---- q, both halves, as mma operands: lane (gq, tq) of [row / 8][d / 16] holds row gq, d 4 tq .. 4 tq + 3
+            for (int n8 = warp; n8 < S::RT / 8; n8 += 4) {
+                const int r = n8 * 8 + gq, R = g.rt * S::RT + r;
+                float4 x[D / 16];
+                uint32_t m = 0;
+                const float* src = a.q + g.b * a.q_bs + (int64_t)(R / a.group) * a.q_rs +
+                                   ((int64_t)g.h * a.group + R % a.group) * D + 4 * tq;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-        a.out[bt * a.heads * D + (int64_t)h * D + lane * E + e] = sum > 0.0f ? o[e] / sum : 0.0f;
+                for (int i = 0; i < D / 16; ++i) {
+                    x[i] = r < rows ? *reinterpret_cast<const float4*>(src + 16 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    const float e[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t bits = __float_as_uint(e[j]) & 0x7FFFFFFFu;
+                        if (bits < 0x7F800000u) m = max(m, bits);
+                    }
+                }
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const int ex = max((int)(m >> 23), 14);          // the row's largest exponent
+                const float up = pow2_field(267 - ex);           // into [2^13, 2^14)
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const float e[4] = {x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up};
+                    float hi[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) hi[j] = leading(e[j]);
+                    q_ops[(n8 * (D / 16) + i) * 32 + lane] =
+                        make_uint4(half2_bits(hi[0], hi[1]), half2_bits(hi[2], hi[3]),
+                                   half2_bits(e[0] - hi[0], e[1] - hi[1]), half2_bits(e[2] - hi[2], e[3] - hi[3]));
+                }
+                if (tq == 0) s_qs[r] = a.scale * 1.4426950408889634f * pow2_field(ex - 13);   // scores in powers of 2
+            }
+            if (a.parents) {
+                // each token's row of the tree: itself and its ancestors, one bit a node
+                for (int j = tid; j <= g.last_token; j += kConsumers) s_parent[j] = a.parents[g.b * a.parents_bs + j];
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                for (int j = tid; j <= g.last_token - g.first_token; j += kConsumers) {
+#pragma unroll
+                    for (int w = 0; w < kTreeWords; ++w) s_sees[j][w] = 0;
+                    for (int n = g.first_token + j; n >= 0;) {
+                        s_sees[j][n >> 5] |= 1u << (n & 31);
+                        const int up = s_parent[n];
+                        n = up < n ? up : -1;
+                    }
+                }
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+
+            float o[NT][D / 16][4], m[NT][2], l[NT][2], qs[NT][2];
+            int token[NT][2];
+            int ex = 14;                                          // vs is scaled by 2^(140 - ex): the largest below 2^14
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[n][i][j] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int r = (rg * NT + n) * 8 + 2 * tq + j;
+                    m[n][j] = -INFINITY;
+                    l[n][j] = 0.0f;
+                    qs[n][j] = s_qs[r];
+                    token[n][j] = (g.rt * S::RT + r) / a.group;
+                }
+            }
+            const int limit = g.len + g.last_token + 1;           // keys that a row of the tile may see
+
+            for (int t = g.t0; t < g.t1; ++t, ++it) {
+                const int stage = it % S::STAGES;
+                mbar_wait(smem_u32(&s_full[stage]), (it / S::STAGES) & 1, a.status, &s_abort);
+                const uint32_t kt = smem_u32(ring + stage * S::STAGE), vt = kt + S::CODES;
+                const float* ks_t = reinterpret_cast<const float*>(ring + stage * S::STAGE + 2 * S::CODES);
+                const float* vs_t = ks_t + kKT;
+                const uint32_t bad = s_bad[stage];
+#pragma unroll 1
+                for (int st = 0; st < S::STEPS; ++st) {
+                    const int kl = (st * S::KG + kg) * 32, k0 = t * kKT + kl;   // first key, in the tile and the sequence
+                    if (k0 >= limit) break;
+                    const bool masked = k0 + 32 > g.len || bad;
+                    // rows of 16 bytes for ldmatrix: keys (lane & 15), 16-byte column (lane >> 4)
+                    const uint32_t row_at = (kl + (lane & 15)) * D + (lane >> 4) * 16;
+
+                    // ---- S^T: 32 keys x 8 NT rows
+                    float s[2][NT][4];
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) s[mt][n][j] = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t ops[2][2][4];
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt) {
+                            uint32_t r[4];
+                            ldsm4(kt + swizzled<D>(row_at + mt * 16 * D + c * 32), r);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) r[j] ^= 0x80808080u;
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                ops[mt][i][0] = two_codes<0x4140>(r[2 * i]);
+                                ops[mt][i][1] = two_codes<0x4140>(r[2 * i + 1]);
+                                ops[mt][i][2] = two_codes<0x4342>(r[2 * i]);
+                                ops[mt][i][3] = two_codes<0x4342>(r[2 * i + 1]);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                const uint4 b = q_ops[((rg * NT + n) * (D / 16) + 2 * c + i) * 32 + lane];
+#pragma unroll
+                                for (int mt = 0; mt < 2; ++mt) mma_16816(s[mt][n], ops[mt][i], b.x, b.y);
+#pragma unroll
+                                for (int mt = 0; mt < 2; ++mt) mma_16816(s[mt][n], ops[mt][i], b.z, b.w);
+                            }
+                    }
+
+                    // ---- scales; the step's largest vs (of keys that are there) sets the power of two
+                    float ks[2][2], vs[2][2];
+                    uint32_t top = __float_as_uint(vs_t[kl + lane]) & 0x7FFFFFFFu;
+                    if (top >= 0x7F800000u || (masked && (k0 + lane >= limit || (bad >> ((kl + lane) >> a.c.shift)) & 1u))) top = 0;
+                    const int ex_new = max(ex, (int)(__reduce_max_sync(0xffffffffu, top) >> 23));
+                    const float vs_up = pow2_field(267 - ex_new);
+                    const float ex_shrink = pow2_field(max(0, 127 + ex - ex_new));
+                    ex = ex_new;
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            ks[mt][j] = ks_t[kl + mt * 16 + j * 8 + gq];
+                            vs[mt][j] = vs_t[kl + mt * 16 + j * 8 + gq] * vs_up;
+                        }
+
+                    // ---- softmax, one pass: new maximum, weights, and the weights times vs as two halves
+                    float corr[NT][2];
+                    uint32_t w_hi[2][NT][2], w_lo[2][NT][2];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        uint32_t seen = 0xFFu;          // bit 4 mt + 2 half + column
+                        if (masked) {
+                            seen = 0;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const int key = kl + (e >> 2) * 16 + ((e >> 1) & 1) * 8 + gq, tok = token[n][e & 1];
+                                const int j = t * kKT + key - g.len;
+                                bool v = !((bad >> (key >> a.c.shift)) & 1u);
+                                if (j >= 0)
+                                    v = v && j < g.count && (a.parents ? tok <= g.last_token && ((s_sees[tok - g.first_token][j >> 5] >> (j & 31)) & 1u)
+                                                                       : j <= tok);
+                                seen |= (uint32_t)v << e;
+                            }
+                        }
+                        float z[2][4];
+                        float mx[2] = {m[n][0], m[n][1]};
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                z[mt][e] = s[mt][n][e] * ks[mt][e >> 1] * qs[n][e & 1];
+                                if (!((seen >> (4 * mt + e)) & 1u)) z[mt][e] = -INFINITY;
+                                mx[e & 1] = fmaxf(mx[e & 1], z[mt][e]);
+                            }
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                            for (int x = 4; x <= 16; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
+                            const float c = shrink(m[n][j], mx[j]);
+                            m[n][j] = mx[j];
+                            l[n][j] *= c;
+                            corr[n][j] = c * ex_shrink;
+                            if (mx[j] == -INFINITY) mx[j] = 0.0f;      // no key yet: every weight is 0
+                        }
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt) {
+                            float hi[4], lo[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float p = exp2_approx(z[mt][e] - mx[e & 1]);
+                                l[n][e & 1] += p;
+                                const float w = (seen >> (4 * mt + e)) & 1u ? p * vs[mt][e >> 1] : 0.0f;
+                                hi[e] = leading(w);
+                                lo[e] = w - hi[e];
+                            }
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {   // keys on the mma's inner side: transposed 8 x 8
+                                w_hi[mt][n][j] = transposed_8x8(half2_bits(hi[2 * j], hi[2 * j + 1]));
+                                w_lo[mt][n][j] = transposed_8x8(half2_bits(lo[2 * j], lo[2 * j + 1]));
+                            }
+                        }
+                    }
+
+                    // ---- O^T: D x 8 NT rows, the step's sum joined to the row's
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t ops[2][2][4];
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt) {
+                            uint32_t r[4];
+                            ldsm4_trans(vt + swizzled<D>(row_at + mt * 16 * D + c * 32), r);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) r[j] ^= 0x80808080u;
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {       // mma row x is d 2x, row x + 8 is d 2x + 1
+                                ops[mt][i][0] = two_codes<0x4240>(r[2 * i]);
+                                ops[mt][i][1] = two_codes<0x4341>(r[2 * i]);
+                                ops[mt][i][2] = two_codes<0x4240>(r[2 * i + 1]);
+                                ops[mt][i][3] = two_codes<0x4341>(r[2 * i + 1]);
+                            }
+                        }
+                        float acc[2][NT][4];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.0f;
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) mma_16816(acc[i][n], ops[mt][i], w_hi[mt][n][0], w_hi[mt][n][1]);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) mma_16816(acc[i][n], ops[mt][i], w_lo[mt][n][0], w_lo[mt][n][1]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    o[n][2 * c + i][j] = fmaf(o[n][2 * c + i][j], corr[n][j & 1], acc[i][n][j]);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s_empty[stage]));
+            }
+
+            // ---- the warps' parts joined
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                    for (int x = 4; x <= 16; x <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
+                    if (gq == 0) {
+                        s_m[kg][(rg * NT + n) * 8 + 2 * tq + j] = m[n][j];
+                        s_l[kg][(rg * NT + n) * 8 + 2 * tq + j] = l[n][j];
+                    }
+                }
+            asm volatile("bar.sync 1, 128;" ::: "memory");     // and q is done with
+            const float unit = pow2_field(ex - 13);            // the warp's power of two taken back
+            const bool direct = g.whole;
+            float* slot = direct ? nullptr : a.parts + (2 * (int64_t)blockIdx.x + (first_segment ? 0 : 1)) * S::SLOT;
+            first_segment = false;
+            float* out = a.out + (int64_t)g.b * a.tokens * a.heads * D + (int64_t)g.h * a.group * D;
+            auto out_row = [&](int r) {                         // row r of the tile in `out`
+                const int R = g.rt * S::RT + r;
+                return out + ((int64_t)(R / a.group) * a.heads + R % a.group) * D;
+            };
+            if constexpr (S::KG == 1) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int r = (rg * NT + n) * 8 + 2 * tq + j;
+                        const float f = direct ? (l[n][j] == 0.0f ? 0.0f : unit / l[n][j]) : unit;
+                        if (r < rows) {
+                            float* dst = direct ? out_row(r) : slot + r * D;
+#pragma unroll
+                            for (int i = 0; i < D / 16; ++i)
+                                *reinterpret_cast<float2*>(dst + 16 * i + 2 * gq) = make_float2(o[n][i][j] * f, o[n][i][j + 2] * f);
+                        }
+                    }
+            } else {
+                for (int turn = 0; turn < S::KG; ++turn) {
+                    if (turn == kg) {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const int r = (rg * NT + n) * 8 + 2 * tq + j;
+                                float M = -INFINITY;
+#pragma unroll
+                                for (int k = 0; k < S::KG; ++k) M = fmaxf(M, s_m[k][r]);
+                                const float f = shrink(m[n][j], M) * unit;
+#pragma unroll
+                                for (int i = 0; i < D / 16; ++i) {
+                                    float2* p = reinterpret_cast<float2*>(joined + r * S::PITCH + 16 * i + 2 * gq);
+                                    const float2 v = turn ? *p : make_float2(0.f, 0.f);
+                                    *p = make_float2(fmaf(o[n][i][j], f, v.x), fmaf(o[n][i][j + 2], f, v.y));
+                                }
+                            }
+                    }
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                }
+                for (int i = tid; i < rows * (D / 4); i += kConsumers) {
+                    const int r = i / (D / 4), c = i % (D / 4);
+                    float4 v = *reinterpret_cast<const float4*>(joined + r * S::PITCH + 4 * c);
+                    if (direct) {
+                        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < S::KG; ++k) M = fmaxf(M, s_m[k][r]);
+#pragma unroll
+                        for (int k = 0; k < S::KG; ++k) L += s_l[k][r] * shrink(s_m[k][r], M);
+                        const float f = L == 0.0f ? 0.0f : 1.0f / L;
+                        v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+                    }
+                    *reinterpret_cast<float4*>((direct ? out_row(r) : slot + r * D) + 4 * c) = v;
+                }
+            }
+            if (!direct && tid < S::RT) {
+                float M = -INFINITY, L = 0.0f;
+                for (int k = 0; k < S::KG; ++k) M = fmaxf(M, s_m[k][tid]);
+                for (int k = 0; k < S::KG; ++k) L += s_l[k][tid] * shrink(s_m[k][tid], M);
+                slot[S::RT * D + tid] = M;
+                slot[S::RT * D + S::RT + tid] = L;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");     // q, maxima and the joined rows are free again
+        }
+    }
+    __syncthreads();
+    // a wait that ran out (recorded): give the copies in flight time to land before the shared memory goes
+    if (s_abort)
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+}
+
+// Joins the parts of one (sequence, head, row tile) that several CTAs left:
+// with M the largest of their maxima, o = sum f_c o_c / sum f_c l_c, f_c =
+// 2^(m_c - M).  A warp a row, a lane D / 32 of its values.
+template <int D, int RT>
+__global__ void __launch_bounds__(kConsumers) cache_attention_join_kernel(const CacheAttArgs a, int ctas) {
+    __shared__ int64_t s_sum[4];
+    constexpr int E = D / 32, SLOT = RT * (D + 2);
+    griddep_launch_dependents();
+    const int b = blockIdx.y, lane = threadIdx.x & 31;
+    // lengths and counts were written before the kernel that left the parts began
+    int64_t before = 0, total = 0;
+    for (int i = threadIdx.x; i < a.batch; i += kConsumers) {
+        const int64_t n = units_of(a, sequence<RT>(a, i));
+        total += n;
+        if (i < b) before += n;
+    }
+    total = sum_128(total, s_sum);
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    before = sum_128(before, s_sum);
+    griddep_wait();
+    const Seq s = sequence<RT>(a, b);
+    const int h = blockIdx.x % a.c.heads, rt = blockIdx.x / a.c.heads;
+    if (rt >= s.row_tiles) return;
+    const int64_t per = units_a_cta(a, total, ctas);
+    const int64_t u0 = before + ((int64_t)h * s.row_tiles + rt) * s.tiles, u1 = u0 + s.tiles;
+    const int c0 = (int)(u0 / per), c1 = (int)((u1 - 1) / per);
+    if (c0 == c1) return;                                       // one CTA had it all
+    const int rows = min(RT, s.count * a.group - rt * RT);
+    auto slot = [&](int c) {                                    // a CTA's first part is in its first slot
+        return a.parts + (2 * (int64_t)c + (c > c0 || c0 * per == u0 ? 0 : 1)) * SLOT;
+    };
+    for (int r = threadIdx.x >> 5; r < rows; r += kConsumers / 32) {
+        float M = -INFINITY, L = 0.0f, o[E];
+        for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, slot(c)[RT * D + r]);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.0f;
+#pragma unroll 4
+        for (int c = c0; c <= c1; ++c) {
+            const float* p = slot(c);
+            const float f = shrink(p[RT * D + r], M);
+            L = fmaf(p[RT * D + RT + r], f, L);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(p[r * D + lane * E + e], f, o[e]);
+        }
+        const float f = L == 0.0f ? 0.0f : 1.0f / L;
+        const int R = rt * RT + r;
+        float* dst = a.out + ((int64_t)b * a.tokens + R / a.group) * a.heads * D + ((int64_t)h * a.group + R % a.group) * D;
+#pragma unroll
+        for (int e = 0; e < E; ++e) dst[lane * E + e] = o[e] * f;
+    }
+}
+
+// ---------------------------------------------------------------- launches
+
+// Rows of a tile: the smallest of 8, 16, 32 and 64 that holds a key head's rows.
+int tile_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+// Whether every (sequence, head, row tile) is one CTA's whole work: the table
+// holds no more tiles than a CTA's range has at least.
+bool whole_ranges(int64_t cols, int64_t page) { return cols * page <= (int64_t)kMinTiles * kKT; }
+
+int64_t parts_floats(int64_t rows, int64_t d) { return 2 * 2 * (int64_t)sm_count() * tile_rows(rows) * (d + 2); }
+
+template <int D, int NT, int RG>
+int launch_cache_attention(const CacheAttArgs& a, int64_t row_tiles, cudaStream_t s) {
+    using S = Shape<D, NT, RG>;
+    static std::atomic<int> attr_set[64];
+    int dev = 0;
+    KZ_CHECK_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+        KZ_CHECK_CUDA(cudaFuncSetAttribute(cache_attention_kernel<D, NT, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           S::SMEM));
+        if (dev >= 0 && dev < 64) attr_set[dev] = 1;
+    }
+    CUtensorMap tm_k, tm_v;
+    const uint64_t rows = (uint64_t)a.c.pages * a.c.heads * a.c.page;
+    int st = tensor_map_rows_i8(&tm_k, a.c.codes[0], D, rows, (uint32_t)a.c.page);
+    if (!st) st = tensor_map_rows_i8(&tm_v, a.c.codes[1], D, rows, (uint32_t)a.c.page);
+    if (st) return st;
+    const int64_t most = (int64_t)a.batch * a.c.heads * row_tiles;
+    const int grid = (int)std::min<int64_t>(2 * (int64_t)sm_count(), a.parts ? 2 * (int64_t)sm_count() : most);
+    KZ_CHECK_CUDA(launch_pdl(cache_attention_kernel<D, NT, RG>, dim3(grid), dim3(kCaThreads), S::SMEM, s, tm_k, tm_v, a));
+    if (a.parts)
+        KZ_CHECK_CUDA(launch_pdl(cache_attention_join_kernel<D, S::RT>,
+                                 dim3((unsigned)(row_tiles * a.c.heads), (unsigned)a.batch), dim3(kConsumers), 0, s, a, grid));
+    return KZ_OK;
+}
+
+template <int D>
+int dispatch_cache_attention(const CacheAttArgs& a, cudaStream_t s) {
+    const int64_t rows = (int64_t)a.tokens * a.group;
+    const int rt = tile_rows(rows);
+    const int64_t row_tiles = (rows + rt - 1) / rt;
+    if (rt == 8) return launch_cache_attention<D, 1, 1>(a, row_tiles, s);
+    if (rt == 16) return launch_cache_attention<D, 2, 1>(a, row_tiles, s);
+    if (rt == 32) return launch_cache_attention<D, 2, 2>(a, row_tiles, s);
+    return launch_cache_attention<D, 2, 4>(a, row_tiles, s);
 }
 
 }  // namespace
@@ -95,19 +761,30 @@ __global__ void __launch_bounds__(kCaThreads) cache_attention_kernel(CacheAttArg
 
 using namespace kz;
 
+extern "C" size_t kz_cache_attention_workspace_bytes(const kz_cache* cache, int64_t tokens, int64_t heads,
+                                                     int64_t table_cols) {
+    if (!cache || cache->kv_heads <= 0 || tokens <= 0 || heads <= 0 || table_cols < 0) return 0;
+    if (whole_ranges(table_cols, cache->page_size)) return 0;
+    return sizeof(float) * (size_t)parts_floats(tokens * (heads / cache->kv_heads), cache->head_dim);
+}
+
 extern "C" int kz_cache_attention_f32(const kz_cache* cache, const float* q, int64_t batch, int64_t tokens,
                                       int64_t heads, int64_t q_batch_stride, int64_t q_row_stride,
                                       const int32_t* table, int64_t table_cols, const int32_t* lengths,
                                       const int32_t* counts, const int32_t* parents, int64_t parents_batch_stride,
-                                      float scale, float* out, kz_stream_t stream) {
+                                      float scale, float* out, void* workspace, size_t workspace_bytes,
+                                      kz_stream_t stream) {
     CacheAttArgs a;
     int st = cache_view(cache, "kz_cache_attention_f32", &a.c);
     if (!st) st = seq_view(table, table_cols, lengths, batch, "kz_cache_attention_f32", &a.s);
     if (st) return st;
-    KZ_REQUIRE(heads > 0 && heads % cache->kv_heads == 0,
+    KZ_REQUIRE(heads > 0 && heads < (1 << 16) && heads % cache->kv_heads == 0,
                "kz_cache_attention_f32: heads must be a multiple of kv_heads");
-    KZ_REQUIRE(tokens >= 0 && tokens < (1 << 24) && batch * tokens * heads < (int64_t)INT32_MAX,
-               "kz_cache_attention_f32: size out of range");
+    KZ_REQUIRE(batch < 65536, "kz_cache_attention_f32: batch must be below 65536");
+    KZ_REQUIRE(tokens >= 0 && tokens < (1 << 24) && tokens * heads < (int64_t)INT32_MAX / 64,
+               "kz_cache_attention_f32: tokens * heads out of range");
+    KZ_REQUIRE(table_cols * cache->page_size < (int64_t)INT32_MAX - (1 << 25),
+               "kz_cache_attention_f32: table_cols * page_size out of range");
     if (batch * tokens == 0) return KZ_OK;
     KZ_REQUIRE(q && out, "kz_cache_attention_f32: q or out is NULL");
     KZ_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0 &&
@@ -118,6 +795,16 @@ extern "C" int kz_cache_attention_f32(const kz_cache* cache, const float* q, int
     KZ_REQUIRE(!parents || tokens <= KZ_TREE_MAX_NODES, "kz_cache_attention_f32: a tree has at most 256 nodes");
     KZ_REQUIRE(parents_batch_stride == 0 || parents_batch_stride >= tokens,
                "kz_cache_attention_f32: parents_batch_stride is shorter than tokens");
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (cache->pages == 0) {   // no key anywhere
+        st = check_device();
+        if (st) return st;
+        KZ_CHECK_CUDA(cudaMemsetAsync(out, 0, sizeof(float) * batch * tokens * heads * cache->head_dim, s));
+        return KZ_OK;
+    }
+    const size_t need = kz_cache_attention_workspace_bytes(cache, tokens, heads, table_cols);
+    KZ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0),
+               "kz_cache_attention_f32: workspace too small or not 16-byte aligned");
     st = check_device();
     if (st) return st;
     a.q = q;
@@ -127,18 +814,14 @@ extern "C" int kz_cache_attention_f32(const kz_cache* cache, const float* q, int
     a.parents = parents;
     a.parents_bs = parents_batch_stride;
     a.out = out;
+    a.parts = need ? static_cast<float*>(workspace) : nullptr;
     a.batch = (int)batch;
     a.tokens = (int)tokens;
     a.heads = (int)heads;
     a.group = (int)(heads / cache->kv_heads);
     a.scale = scale;
     a.status = device_status_ptr();
-    const int64_t warps = batch * tokens * heads;
-    const dim3 grid((unsigned)((warps + kCaThreads / 32 - 1) / (kCaThreads / 32)));
-    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    auto kernel = cache->head_dim == 32   ? cache_attention_kernel<32>
-                  : cache->head_dim == 64 ? cache_attention_kernel<64>
-                                          : cache_attention_kernel<128>;
-    KZ_CHECK_CUDA(launch_pdl(kernel, grid, dim3(kCaThreads), 0, s, a));
-    return KZ_OK;
+    return cache->head_dim == 32   ? dispatch_cache_attention<32>(a, s)
+           : cache->head_dim == 64 ? dispatch_cache_attention<64>(a, s)
+                                   : dispatch_cache_attention<128>(a, s);
 }

@@ -28,6 +28,10 @@ int sm_count();
 // KZ_OK if the current device is an sm_100 part, else an error (recorded).
 int check_device();
 
+// Tensor map of rows of `cols` bytes (32, 64 or 128), a box of box_rows whole
+// rows, swizzled over the row's own width (defined in kz_gemm_i8.cu).
+int tensor_map_rows_i8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint32_t box_rows);
+
 #define KZ_CHECK_CUDA(call)                                   \
     do {                                                      \
         cudaError_t e_ = (call);                              \
