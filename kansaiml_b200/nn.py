@@ -166,15 +166,22 @@ class MultiHeadAttention(Module):
             return self.q_proj[i](x)
         return x.matmul(w)
 
-    def forward(self, query, key, value, mask=None):
+    def forward(self, query, key, value, mask=None, step=None):
+        """With ``step`` (a CacheStep; self-attention only), the inputs are a
+        step's new tokens: their keys and values enter the layer's cache and
+        the attention runs over all it holds (mask unused)."""
+        if step is not None and not (query is key and key is value):
+            raise ValueError("attention over a cache is self-attention: query, key and value must be one input")
         if self.qkv is not None and query is key and key is value:
-            return self._self_attention(query, mask)
+            return self._self_attention(query, mask, step)
         if isinstance(query, QActivation):
             raise ValueError("a pre-quantized input needs the fused self-attention path")
         q_in, k_in, v_in = as_tensor(query), as_tensor(key), as_tensor(value)
         q = self._proj(q_in, 0, self.w_q).data
         k = self._proj(k_in, 1, self.w_k).data
         v = self._proj(v_in, 2, self.w_v).data
+        if step is not None:
+            return self._proj(step.attend(q, k, v, self.num_heads), 3, self.w_o)
         causal = self._causal(mask, q.shape[1], k.shape[1])
         m = as_tensor(mask).data if mask is not None and not causal else None
         att, _ = attention_device(q, k, v, self.num_heads, mask=m, causal=causal)
@@ -190,7 +197,7 @@ class MultiHeadAttention(Module):
                 and tuple(as_tensor(mask).shape[-2:]) == (sq, sk))
 
 
-    def _self_attention(self, x, mask):
+    def _self_attention(self, x, mask, step=None):
         """One int8 GEMM for q, k and v; the fp32 attention kernel reads q, k
         and v straight out of its [b, s, 3d] output and writes the heads-merged
         result with its absmax partials, so the int8 output projection's
@@ -201,6 +208,8 @@ class MultiHeadAttention(Module):
         b, s, _ = x.shape
         d = self.d_model
         qkv = self.qkv(x).data.reshape(b, s, 3 * d)
+        if step is not None:
+            return self.q_proj[3](step.attend(qkv[:, :, :d], qkv[:, :, d:2 * d], qkv[:, :, 2 * d:], self.num_heads))
         causal = self._causal(mask, s, s)
         m = as_tensor(mask).data if mask is not None and not causal else None
         att, partials = attention_device(qkv[:, :, :d], qkv[:, :, d:2 * d], qkv[:, :, 2 * d:], self.num_heads,
@@ -229,13 +238,13 @@ class TransformerBlock(Module):
     def _w8a8(self):
         return isinstance(self.fc1, QLinear) and self.attn.qkv is not None
 
-    def forward(self, x, mask=None):
+    def forward(self, x, mask=None, step=None):
         x = as_tensor(x)
         if self._w8a8():
-            x, pending = self._forward_w8a8(x, mask)
+            x, pending = self._forward_w8a8(x, mask, step=step)
             return x.add(pending)
         normed = self.ln1(x)
-        x = x.add(self.attn(normed, normed, normed, mask=mask))
+        x = x.add(self.attn(normed, normed, normed, mask=mask, step=step))
         h = self.ln2(x)
         if isinstance(self.fc1, QLinear):
             h = self.fc1(h, act="gelu")
@@ -243,7 +252,7 @@ class TransformerBlock(Module):
             h = self.gelu(self.fc1(h))
         return x.add(self.fc2(h))
 
-    def _forward_w8a8(self, x, mask, pending=None):
+    def _forward_w8a8(self, x, mask, pending=None, step=None):
         """The same block with every activation quantized where it is made:
         LayerNorm -> quantize is one LayerNorm kernel (with the absmax) plus
         one quantize pass; fc1's GEMM epilogue (bias + GELU) also emits the
@@ -257,10 +266,27 @@ class TransformerBlock(Module):
             qa = QActivation.layernorm(x, ln1.weight, ln1.bias, ln1.eps)
         else:
             x, qa = QActivation.add_layernorm(x, pending, ln1.weight, ln1.bias, ln1.eps)
-        x, qb = QActivation.add_layernorm(x, self.attn(qa, qa, qa, mask=mask), ln2.weight, ln2.bias, ln2.eps)
+        x, qb = QActivation.add_layernorm(x, self.attn(qa, qa, qa, mask=mask, step=step), ln2.weight, ln2.bias, ln2.eps)
         partials = partials_buffer(x.data.device)
         h = self.fc1(qb, act="gelu", out_partials=partials)
         return x, self.fc2(QActivation.from_partials(h, partials))
+
+
+class CacheStep:
+    """One step of generation as one layer sees it: its QCache, the sequences'
+    pages and lengths before the step, how many of the step's rows are tokens
+    (counts, None: all) and the tree they form (parents, None: one after
+    another).  See kansaiml_b200.cache for the tensors."""
+
+    __slots__ = ("cache", "table", "lengths", "counts", "parents")
+
+    def __init__(self, cache, table, lengths, counts=None, parents=None):
+        self.cache, self.table, self.lengths, self.counts, self.parents = cache, table, lengths, counts, parents
+
+    def attend(self, q, k, v, heads):
+        """The new tokens' k and v into the cache, then q's attention over it."""
+        self.cache.write(k, v, self.table, self.lengths, self.counts)
+        return self.cache.attention(q, heads, self.table, self.lengths, self.counts, self.parents)
 
 
 class CausalMask(Tensor):

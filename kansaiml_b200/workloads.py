@@ -14,6 +14,7 @@ import numpy as np
 import torch
 
 from . import nn
+from .cache import PagePool, QCache, verify_tree
 from .quantize import QActivation, QLinear
 from .tensor import Tensor, from_numpy
 
@@ -22,6 +23,35 @@ def _param(a, device):
     t = from_numpy(a, device)
     t.requires_grad = True
     return t
+
+
+class DecoderCache:
+    """What a Decoder keeps of a batch of sequences: one QCache a layer, their
+    common pages, and how many tokens each sequence has (``lengths``, on the
+    device).  ``most`` bounds them on the host: pages are reserved by it."""
+
+    def __init__(self, layers, batch, kv_heads, head_dim, capacity, page_size, device):
+        columns = -(-capacity // page_size)
+        self.capacity, self.most = capacity, 0
+        self.pool = PagePool(batch * columns, batch, columns, page_size, device)
+        self.layers = [QCache(batch * columns, kv_heads, head_dim, page_size, device) for _ in range(layers)]
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=self.pool.table.device)
+
+    def room(self, tokens):
+        """Pages for `tokens` more tokens of every sequence; raises past the capacity."""
+        if self.most + tokens > self.capacity:
+            raise ValueError(f"DecoderCache: {self.most} + {tokens} tokens, the capacity is {self.capacity}")
+        self.pool.reserve(self.most + tokens)
+
+    def advance(self, counts, most):
+        """The last step's first counts[b] tokens stay (an int, or int32 [batch]); most: no sequence has more."""
+        self.lengths += counts
+        self.most = most
+
+    def keep(self, path, count):
+        """An accepted path's tokens to the front, in every layer."""
+        for layer in self.layers:
+            layer.keep(self.pool.table, self.lengths, path, count)
 
 
 class Decoder(nn.Module):
@@ -71,12 +101,124 @@ class Decoder(nn.Module):
             else:
                 x = blk(x if pending is None else x.add(pending), mask=mask)
                 pending = None
+        return self._logits(x, pending)
+
+    def _logits(self, x, pending):
         ln = self.ln
         if pending is None:
             qa = QActivation.layernorm(x, ln.weight, ln.bias, ln.eps)
         else:
             _, qa = QActivation.add_layernorm(x, pending, ln.weight, ln.bias, ln.eps)
         return self.head(qa)
+
+    # ------------------------------------------------------------ generation
+    def new_cache(self, batch, capacity=None, page_size=64):
+        """An empty cache for `batch` sequences of at most `capacity` (default: the context) tokens."""
+        capacity = self.ctx if capacity is None else capacity
+        if not 0 < capacity <= self.ctx:
+            raise ValueError(f"Decoder: the capacity must be 1 to the context's {self.ctx} (got {capacity})")
+        return DecoderCache(len(self.blocks), batch, self.heads, self.d_model // self.heads, capacity, page_size,
+                            self.tok.weight.device)
+
+    def extend(self, ids, cache, counts=None, parents=None, depths=None):
+        """The logits [B, T, vocab] of new tokens ids int64 [B, T] over what the
+        cache holds; their keys and values enter it behind that (cache.advance
+        then makes them part of it).  counts: rows that are tokens (None: all);
+        parents (with depths int64 [B, T], a node's distance from the root): the
+        tokens form a tree."""
+        cache.room(ids.shape[1])
+        where = torch.arange(ids.shape[1], device=ids.device) if depths is None else depths
+        where = (cache.lengths[:, None] + where).clamp(max=self.ctx - 1)
+        x = Tensor(self.tok.weight.data[ids] + self.pos.weight.data[where])
+        pending = None
+        for blk, layer in zip(self.blocks, cache.layers):
+            step = nn.CacheStep(layer, cache.pool.table, cache.lengths, counts, parents)
+            if blk._w8a8():
+                x, pending = blk._forward_w8a8(x, None, pending, step)
+            else:
+                x = blk(x if pending is None else x.add(pending), step=step)
+                pending = None
+        return self._logits(x, pending)
+
+    def generate(self, prompts, new_tokens, temperature=1.0, drafts=0, seed=0):
+        """`new_tokens` more tokens for each prompt (lists of ids), drawn at
+        `temperature` (0: the likeliest).  With drafts > 0, each step verifies
+        up to that many tokens looked up in the sequence itself -- what followed
+        earlier occurrences of its last token, as a tree -- and keeps those that
+        the model's own probabilities accept: the tokens are distributed as
+        without drafts.  Returns one list of new ids per prompt."""
+        device = self.tok.weight.device
+        seen = [list(p) for p in prompts]
+        batch, longest = len(seen), max(len(p) for p in seen)
+        if min(len(p) for p in seen) < 1 or not all(0 <= t < self.vocab for p in seen for t in p):
+            raise ValueError(f"Decoder.generate: a prompt is one or more ids below {self.vocab}")
+        if new_tokens < 1 or longest + new_tokens > self.ctx:
+            raise ValueError(f"Decoder.generate: {longest} + {new_tokens} tokens, the context is {self.ctx}")
+        cache = self.new_cache(batch)
+        random = torch.Generator(device=device).manual_seed(seed)
+
+        def step(ids, counts, parents=None, depths=None):
+            logits = self.extend(ids, cache, counts, parents, depths).data
+            if temperature > 0:
+                return torch.softmax(logits / temperature, -1)
+            return torch.nn.functional.one_hot(logits.argmax(-1), self.vocab).float()
+
+        def verified(ids, parents, probs):
+            nodes = ids.shape[1]
+            return verify_tree(ids, parents, probs, None, torch.rand(batch, nodes, generator=random, device=device),
+                               torch.rand(batch, generator=random, device=device))
+
+        counts = torch.tensor([len(p) for p in seen], dtype=torch.int32, device=device)
+        ids = torch.tensor([p + [0] * (longest - len(p)) for p in seen], device=device)
+        probs = step(ids, counts)
+        probs = probs[torch.arange(batch, device=device), counts.long() - 1][:, None]
+        root = torch.full((1,), -1, dtype=torch.int32, device=device)
+        _, _, token = verified(ids[:, :1], root, probs)
+        cache.advance(counts, longest)
+        out = [[t] for t in token.tolist()]
+        for s, o in zip(seen, out):
+            s += o
+        while True:
+            live = [len(o) < new_tokens for o in out]
+            if not any(live):
+                break
+            room = min(1 + drafts, cache.capacity - cache.most)
+            trees = [_drafted(s, room) if on else ([], [], []) for s, on in zip(seen, live)]
+            nodes = max(len(t[0]) for t in trees)
+            ids = torch.tensor([t[0] + [0] * (nodes - len(t[0])) for t in trees], device=device)
+            parents = torch.tensor([t[1] + [-1] * (nodes - len(t[1])) for t in trees], dtype=torch.int32, device=device)
+            depths = torch.tensor([t[2] + [0] * (nodes - len(t[2])) for t in trees], device=device)
+            counts = torch.tensor([len(t[0]) for t in trees], dtype=torch.int32, device=device)
+            path, count, token = verified(ids, parents, step(ids, counts, parents, depths))
+            count = torch.minimum(count, counts)             # 0: a sequence that is done
+            cache.keep(path, count)
+            for s, o, t, p, n, x in zip(seen, out, trees, path.tolist(), count.tolist(), token.tolist()):
+                new = [t[0][i] for i in p[1:n]] + [x] if n else []
+                s += new
+                o += new
+            cache.advance(count, max(len(s) - 1 for s, on in zip(seen, live) if on))
+        return [o[:new_tokens] for o in out]
+
+
+def _drafted(seen, nodes):
+    """A tree of at most `nodes` tokens from the sequence itself: the last token
+    as the root, then what followed its earlier occurrences, the latest first.
+    Returns (tokens, parents, depths)."""
+    tokens, parents, depths, below = [seen[-1]], [-1], [0], {}
+    for at in range(len(seen) - 2, -1, -1):
+        if seen[at] != seen[-1]:
+            continue
+        node = 0
+        for x in seen[at + 1:at + 5]:
+            if len(tokens) >= nodes:
+                return tokens, parents, depths
+            if (node, x) not in below:
+                below[node, x] = len(tokens)
+                tokens.append(x)
+                parents.append(node)
+                depths.append(depths[node] + 1)
+            node = below[node, x]
+    return tokens, parents, depths
 
 
 def config3_ids(batch=32, ctx=256, vocab=65, seed=0, device="cuda"):

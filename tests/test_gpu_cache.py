@@ -527,3 +527,234 @@ def test_verified_tokens_follow_the_target(cuda_device, draft):
     first = np.where(count > 1, tokens[np.arange(n), np.maximum(path[:, 1], 0)], token)
     seen = np.bincount(first, minlength=v) / n
     assert np.all(np.abs(seen - p) <= 5 * np.sqrt(p * (1 - p) / n) + 1e-12), seen
+
+
+# ----------------------------------------------------- together, as a model uses them
+
+def test_speculative_steps_together(cuda_device):
+    """Write, attention, verification and keep over several steps of trees, the
+    cache then holding exactly the accepted tokens; every step's attention
+    equals the 64-bit one over what the host's own books say is cached."""
+    from kansaiml_b200.cache import PagePool, QCache, verify_tree
+    rs = np.random.RandomState(21)
+    batch, kv, heads, d, page, nodes, vocab = 3, 2, 6, 64, 16, 7, 11
+    pool = PagePool(40, batch, 8, page, "cuda")
+    cache = QCache(40, kv, d, page, "cuda")
+    lengths = torch.zeros(batch, dtype=torch.int32, device="cuda")
+    books = [[np.zeros((0, kv, d)), np.zeros((0, kv, d))] for _ in range(batch)]
+    for step in range(6):
+        n = 20 if step == 0 else nodes
+        parents = None if step == 0 else np.array([_tree(n, 50 * step + b) for b in range(batch)], np.int32)
+        kvs = rs.standard_normal((2, batch, n, kv * d)).astype(np.float32)
+        q = rs.standard_normal((batch, n, heads * d)).astype(np.float32)
+        pool.reserve(max(len(b[0]) for b in books) + n)
+        cache.write(_dev(kvs[0]), _dev(kvs[1]), pool.table, lengths)
+        y = cache.attention(_dev(q), heads, pool.table, lengths, None, None if parents is None else _dev(parents)).numpy()
+        new = []
+        for b in range(batch):
+            stood = []
+            for part in range(2):
+                codes, scales = _quantized(kvs[part, b].reshape(n, kv, d))
+                stood.append(codes * scales.astype(np.float32).astype(np.float64)[..., None])
+            new.append(stood)
+            have = len(books[b][0])
+            want, bound = _attention_64(q[b], np.concatenate([books[b][0], stood[0]]), np.concatenate([books[b][1], stood[1]]),
+                                        have, n, heads, None if parents is None else parents[b], 1 / 8)
+            assert np.all(np.abs(y[b] - want) <= bound)
+        if parents is None:
+            paths = [list(range(n))] * batch
+            lengths += n
+        else:
+            target = _softmax(rs, (batch, n, vocab), 1.0)
+            tokens = rs.randint(0, vocab, (batch, n)).astype(np.int64)
+            path, count, _ = verify_tree(_dev(tokens), _dev(parents), _dev(target), None,
+                                         _dev(rs.uniform(size=(batch, n)).astype(np.float32) * 0.2),
+                                         _dev(rs.uniform(size=batch).astype(np.float32)))
+            cache.keep(pool.table, lengths, path, count)
+            lengths += count
+            paths = [p[:c] for p, c in zip(path.tolist(), count.tolist())]
+        for b in range(batch):
+            books[b] = [np.concatenate([books[b][i], new[b][i][paths[b]]]) for i in range(2)]
+        k, v = cache.read(pool.table, lengths, max(len(b[0]) for b in books))
+        for b in range(batch):
+            for got, book in zip((k, v), books[b]):
+                np.testing.assert_array_equal(got.numpy()[b, :len(book)], book.reshape(len(book), kv * d).astype(np.float32))
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+def test_module_attention_over_a_cache(cuda_device, quantized):
+    """MultiHeadAttention with a step: the output projection of the attention
+    over the cache of its own projections, for a prompt and a token after it."""
+    from kansaiml_b200 import nn as knn
+    from kansaiml_b200.cache import PagePool, QCache
+    from kansaiml_b200.tensor import Tensor
+    mha = knn.MultiHeadAttention(128, 2, seed=4, device="cuda")
+    if quantized:
+        mha.quantize(per_channel=True)
+    pool, cache = PagePool(8, 2, 4, 16, "cuda"), QCache(8, 2, 64, 16, "cuda")
+    pool.reserve(60)
+    seen = []
+    inner = QCache.attention
+
+    def spy(self, q, *args, **kw):
+        out = inner(self, q, *args, **kw)
+        seen.append((q.cpu().numpy(), out.numpy()))
+        return out
+
+    lengths = _i32([0, 0])
+    QCache.attention = spy
+    try:
+        for n in (33, 1, 4):
+            x = Tensor(torch.randn(2, n, 128, device="cuda"))
+            step = knn.CacheStep(cache, pool.table, lengths)
+            y = mha(x, x, x, step=step)
+            assert y.shape == [2, n, 128]
+            k, v = cache.read(pool.table, lengths + n, int(lengths[0]) + n)
+            for b in range(2):
+                want, bound = _attention_64(seen[-1][0][b], k.numpy()[b].reshape(-1, 2, 64).astype(np.float64),
+                                            v.numpy()[b].reshape(-1, 2, 64).astype(np.float64), int(lengths[0]), n, 2,
+                                            None, 1 / 8)
+                assert np.all(np.abs(seen[-1][1][b] - want) <= bound)
+            lengths += n
+    finally:
+        QCache.attention = inner
+    with pytest.raises(ValueError, match="self-attention"):
+        mha(x, Tensor(x.data.clone()), x, step=step)
+    assert _status() == 0
+
+
+def test_decoder_generates_through_the_cache(cuda_device):
+    """Decoder.generate: ragged prompts, with and without looked-up drafts; the
+    logits of a prompt through the cache are near those of the whole-context
+    forward (its K/V are quantized once more: 8 bits of them, so 5% of the
+    logits' norm is far beyond what the rounding moves)."""
+    from kansaiml_b200 import workloads
+    model = workloads.Decoder(seed=3)
+    ids = workloads.config3_ids(batch=4, ctx=100, seed=4)
+    cache = model.new_cache(4)
+    whole = model(ids).data
+    got = model.extend(ids, cache).data
+    assert (got - whole).norm() <= 0.05 * whole.norm()
+    cache.advance(100, 100)
+    more = model.extend(ids[:, :1], cache).data
+    assert more.shape == (4, 1, 65) and torch.isfinite(more).all()
+    prompts = [ids[i, :n].tolist() for i, n in enumerate((5, 40, 100, 1))]
+    for temperature in (0.0, 1.0):
+        for drafts in (0, 6):
+            a = model.generate(prompts, 30, temperature, drafts, seed=7)
+            assert [len(o) for o in a] == [30] * 4 and all(0 <= t < 65 for o in a for t in o)
+            assert a == model.generate(prompts, 30, temperature, drafts, seed=7)
+    with pytest.raises(ValueError, match="context"):
+        model.generate(prompts, 157)
+    with pytest.raises(ValueError, match="prompt"):
+        model.generate([[1], []], 3)
+    with pytest.raises(ValueError, match="capacity"):
+        cache.room(200)
+    assert _status() == 0
+
+
+# ----------------------------------------------------- capture, streams, devices, refusals
+
+def test_captured_steps_replay_with_new_lengths(cuda_device):
+    """A step captured into a graph reads lengths, pages and inputs anew at
+    each replay; two graphs of the same cache do not share scratch."""
+    book = Book([1500, 700], 2, 128, 64)
+    lengths, q = _i32([0, 0]), torch.zeros(2, 1, 8 * 128, device="cuda")
+    q2, l2 = torch.zeros(2, 20, 8 * 128, device="cuda"), _i32([0, 0])
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        book.cache.attention(q, 8, book.table, lengths)
+        book.cache.attention(q2, 8, book.table, l2)
+    stream.synchronize()
+    one, two = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(one):
+        y1 = book.cache.attention(q, 8, book.table, lengths).data
+    with torch.cuda.graph(two):
+        y2 = book.cache.attention(q2, 8, book.table, l2).data
+    book.fill([1500, 700])
+    for at in ([1499, 699], [3, 500], [800, 0]):
+        lengths.copy_(_i32(at))
+        l2.copy_(_i32([max(0, n - 30) for n in at]))
+        q.copy_(torch.randn_like(q))
+        q2.copy_(torch.randn_like(q2))
+        one.replay()
+        two.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y1, book.cache.attention(q, 8, book.table, lengths).data)
+        assert torch.equal(y2, book.cache.attention(q2, 8, book.table, l2).data)
+    assert _status() == 0
+
+
+def test_two_streams_at_once(cuda_device):
+    book = Book([2000, 2000], 2, 64, 64)
+    book.fill([2000, 2000])
+    q = [torch.randn(2, 1, 8 * 64, device="cuda") for _ in range(2)]
+    lengths = _i32([1999, 1500])
+    want = [book.cache.attention(x, 8, book.table, lengths).data for x in q]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(book.cache.attention(q[i], 8, book.table, lengths).data)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+def test_refusals(cuda_device):
+    from kansaiml_b200.cache import QCache, verify_tree
+    book = Book([40], 2, 64, 16)
+    c, t, n = book.cache, book.table, _i32([3])
+    x = torch.zeros(1, 2, 128, device="cuda")
+    for bad, match in (((48, 2), "head_dim"), ((64, 0), "kv_heads")):
+        with pytest.raises(ValueError, match=match):
+            QCache(4, bad[1], bad[0], 16, "cuda")
+    with pytest.raises(ValueError, match="page_size"):
+        QCache(4, 2, 64, 24, "cuda")
+    with pytest.raises(ValueError, match="contiguous"):
+        QCache.wrap(c.k_codes, c.k_scale, c.v_codes, c.v_scale.double())
+    with pytest.raises(ValueError, match="k must be"):
+        c.write(x[:, :, :64], x, t, n)
+    with pytest.raises(ValueError, match="do not match"):
+        c.write(x, x[:, :1], t, n)
+    with pytest.raises(ValueError, match="lengths must be"):
+        c.write(x, x, t, n.long())
+    with pytest.raises(ValueError, match="lengths must be"):
+        c.write(x, x, t, _i32([3, 4]))
+    with pytest.raises(ValueError, match="counts"):
+        c.write(x, x, t, n, [1])
+    with pytest.raises(ValueError, match="on cpu"):
+        c.write(x, x, t.cpu(), n)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        c.write(x.cpu(), x, t, n)
+    with pytest.raises(ValueError, match="multiple of kv_heads"):
+        c.attention(x, 3, t, n)
+    with pytest.raises(ValueError, match="q must be"):
+        c.attention(x, 4, t, n)
+    with pytest.raises(ValueError, match="parents"):
+        c.attention(x, 2, t, n, parents=_i32([0, 1, 2]))
+    big = torch.zeros(1, 257, 128, device="cuda")
+    with pytest.raises(ValueError, match="256"):
+        c.attention(big, 2, t, n, parents=_i32([0] * 257))
+    with pytest.raises(ValueError, match="most"):
+        c.read(t, n, -1)
+    with pytest.raises(ValueError, match="path"):
+        c.keep(t, n, _i32([0, 1]), n)
+    with pytest.raises(ValueError, match="count"):
+        c.keep(t, n, _i32([[0, 1]]), None)
+    p, u = torch.full((1, 2, 5), 0.2, device="cuda"), torch.zeros(1, 2, device="cuda")
+    tok, par, s = torch.zeros(1, 2, dtype=torch.int64, device="cuda"), _i32([-1, 0]), torch.zeros(1, device="cuda")
+    with pytest.raises(ValueError, match="tokens"):
+        verify_tree(tok.int(), par, p, None, u, s)
+    with pytest.raises(ValueError, match="draft"):
+        verify_tree(tok, par, p, p[:, :1], u, s)
+    with pytest.raises(ValueError, match="accept_u"):
+        verify_tree(tok, par, p, None, s, s)
+    with pytest.raises(ValueError, match="target"):
+        verify_tree(tok, par, p[0], None, u, s)
+    with pytest.raises(ValueError, match="1024"):
+        verify_tree(tok, par, torch.zeros(1, 1025, 2, device="cuda"), None, u, s)
+    assert _status() == 0
