@@ -127,4 +127,6 @@ def check(status, what=""):
 
 def call(name, *args):
     """Calls `name` and raises on a non-zero status."""
-    check(getattr(load(), name)(*args), name)
+    status = getattr(_lib or load(), name)(*args)
+    if status:
+        check(status, name)

@@ -38,17 +38,16 @@ def _raw(t, what):
     x = t.data if isinstance(t, Tensor) else t
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{what} must be a Tensor or a torch tensor, not {type(t).__name__}")
-    require_cuda(x, what)
-    return x if x.dtype == torch.float32 else x.float()
+    if not x.is_cuda:
+        require_cuda(x, what)
+    return x if x.dtype is torch.float32 else x.float()
 
 
 def _rows(x, what, width):
     """(x, batch stride, row stride) of a [batch, tokens, width] tensor whose
     rows a kernel can read in 16-byte pieces; any other is copied first."""
-    if x.dim() != 3 or x.shape[2] != width:
-        raise ValueError(f"{what} must be [batch, tokens, {width}], not {list(x.shape)}")
     bs, rs, fs = x.stride()
-    if (x.data_ptr() & 15) or ((bs | rs) & 3) or fs != 1 or bs < 0 or (x.shape[1] > 1 and rs < width):
+    if (x.data_ptr() & 15) or ((bs | rs) & 3) or fs != 1 or bs < 0 or (rs < width and x.shape[1] > 1):
         x = x.contiguous()
         if x.data_ptr() & 15:
             x = x.clone()
@@ -56,21 +55,22 @@ def _rows(x, what, width):
     return x, bs, rs
 
 
-def _ints(t, what, shape, device, dtype=torch.int32):
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what} must be a {str(dtype)[6:]} tensor {list(shape)}, not "
-                         f"{list(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}"
-                         f"{' ' + str(t.dtype)[6:] if isinstance(t, torch.Tensor) else ''}")
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, not on {device}")
-    return t if t.is_contiguous() else t.contiguous()
+def _ints(t, what, shape, index, dtype=torch.int32):
+    """t, contiguous, checked to be integers of that shape on GPU `index`."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == index:
+        return t if t.is_contiguous() else t.contiguous()
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{what} must be a {str(dtype)[6:]} tensor {list(shape)}, not {type(t).__name__}")
+    if t.dtype is not dtype or t.shape != shape:
+        raise ValueError(f"{what} must be a {str(dtype)[6:]} tensor {list(shape)}, not {list(t.shape)} {str(t.dtype)[6:]}")
+    raise ValueError(f"{what} is on {t.device}, not on cuda:{index}")
 
 
-def _parents(parents, batch, nodes, device):
+def _parents(parents, batch, nodes, index):
     """(parents, batch stride): one tree for every sequence, or one each."""
     if isinstance(parents, torch.Tensor) and parents.dim() == 1:
-        return _ints(parents, "parents", (nodes,), device), 0
-    return _ints(parents, "parents", (batch, nodes), device), nodes
+        return _ints(parents, "parents", (nodes,), index), 0
+    return _ints(parents, "parents", (batch, nodes), index), nodes
 
 
 def _on(device, name, *args):
@@ -86,7 +86,8 @@ class QCache:
     """One attention layer's int8 K/V pages: codes [pages, kv_heads, page_size,
     head_dim] and fp32 scales [pages, kv_heads, page_size], for K and for V."""
 
-    __slots__ = ("k_codes", "k_scale", "v_codes", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "_c", "_ref")
+    __slots__ = ("k_codes", "k_scale", "v_codes", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "device", "_at", "_c", "_ref",
+                 "_scratch")
 
     def __init__(self, pages, kv_heads, head_dim, page_size=64, device=None):
         dev = _as_device(device)
@@ -122,10 +123,8 @@ class QCache:
         self.k_codes, self.k_scale, self.v_codes, self.v_scale = k_codes, k_scale, v_codes, v_scale
         self._c = _lib.KzCache(ptr(k_codes), ptr(k_scale), ptr(v_codes), ptr(v_scale), *k_codes.shape)
         self._ref = ctypes.byref(self._c)
-
-    @property
-    def device(self):
-        return self.k_codes.device
+        self.device, self._at = k_codes.device, k_codes.get_device()
+        self._scratch = {}                      # (tokens, heads, columns) -> bytes of attention's workspace
 
     def nbytes(self):
         """Bytes held: one per code and four per scale."""
@@ -136,21 +135,23 @@ class QCache:
                 f"page_size={self.page_size}, device={self.device})")
 
     def _sequences(self, table, lengths, counts=None):
-        dev = self.device
-        require_cuda(self.k_codes, "QCache")
+        if self._at < 0:
+            require_cuda(self.k_codes, "QCache")
         if not isinstance(table, torch.Tensor) or table.dim() != 2:
             raise ValueError("table must be an int32 tensor [batch, columns]")
         batch, cols = table.shape
-        return (batch, cols, _ints(table, "table", (batch, cols), dev), _ints(lengths, "lengths", (batch,), dev),
-                None if counts is None else _ints(counts, "counts", (batch,), dev))
+        return (batch, cols, _ints(table, "table", table.shape, self._at),
+                _ints(lengths, "lengths", (batch,), self._at),
+                None if counts is None else _ints(counts, "counts", (batch,), self._at))
 
     def _input(self, t, what, heads, batch):
         x = _raw(t, what)
-        if x.device != self.device:
+        width = heads * self.head_dim
+        if x.dim() != 3 or x.shape[0] != batch or x.shape[2] != width:
+            raise ValueError(f"{what} must be [{batch}, tokens, {width}], not {list(x.shape)}")
+        if x.get_device() != self._at:
             raise ValueError(f"{what} is on {x.device}, the cache on {self.device}")
-        if x.dim() != 3 or x.shape[0] != batch:
-            raise ValueError(f"{what} must be [{batch}, tokens, {heads * self.head_dim}], not {list(x.shape)}")
-        return _rows(x, what, heads * self.head_dim)
+        return _rows(x, what, width)
 
     def write(self, k, v, table, lengths, counts=None, values=False):
         """Quantizes new tokens' k and v [batch, tokens, kv_heads * head_dim]
@@ -196,9 +197,13 @@ class QCache:
         if parents is not None:
             if tokens > _lib.KZ_TREE_MAX_NODES:
                 raise ValueError(f"attention: a tree has at most {_lib.KZ_TREE_MAX_NODES} nodes (got {tokens})")
-            parents, pb = _parents(parents, batch, tokens, self.device)
+            parents, pb = _parents(parents, batch, tokens, self._at)
         out = torch.empty((batch, tokens, heads * self.head_dim), dtype=torch.float32, device=self.device)
-        need = _lib.load().kz_cache_attention_workspace_bytes(self._ref, tokens, heads, cols)
+        need = self._scratch.get((tokens, heads, cols))
+        if need is None:
+            with torch.cuda.device(self.device):
+                need = _lib.load().kz_cache_attention_workspace_bytes(self._ref, tokens, heads, cols)
+            self._scratch[tokens, heads, cols] = need
         work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         _on(self.device, "kz_cache_attention_f32", self._ref, ptr(q), batch, tokens, heads, qb, qr, ptr(table), cols,
             ptr(lengths), ptr(counts), ptr(parents), pb, 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
@@ -212,7 +217,7 @@ class QCache:
         batch, cols, table, lengths, count = self._sequences(table, lengths, count)
         if not isinstance(path, torch.Tensor) or path.dim() != 2:
             raise ValueError("path must be an int32 tensor [batch, nodes]")
-        path = _ints(path, "path", (batch, path.shape[1]), self.device)
+        path = _ints(path, "path", (batch, path.shape[1]), self._at)
         if count is None:
             raise ValueError("count must be an int32 tensor [batch]")
         _on(self.device, "kz_cache_keep", self._ref, ptr(table), cols, ptr(lengths), ptr(path), ptr(count), batch,
@@ -278,19 +283,19 @@ def verify_tree(tokens, parents, target, draft, accept_u, sample_u):
     batch, nodes, vocab = target.shape
     if nodes > 1024:
         raise ValueError(f"verify_tree: at most 1024 nodes (got {nodes})")
-    dev = target.device
+    dev, at = target.device, target.get_device()
 
     def floats(t, what, shape):
         x = _raw(t, what)
-        if tuple(x.shape) != tuple(shape) or x.device != dev:
+        if x.shape != shape or x.get_device() != at:
             raise ValueError(f"{what} must be {list(shape)} on {dev}, not {list(x.shape)} on {x.device}")
         return x.contiguous()
 
     target = target.contiguous()
     draft = None if draft is None else floats(draft, "draft", target.shape)
     accept_u, sample_u = floats(accept_u, "accept_u", (batch, nodes)), floats(sample_u, "sample_u", (batch,))
-    tokens = _ints(tokens, "tokens", (batch, nodes), dev, torch.int64)
-    parents, pb = _parents(parents, batch, nodes, dev)
+    tokens = _ints(tokens, "tokens", (batch, nodes), at, torch.int64)
+    parents, pb = _parents(parents, batch, nodes, at)
     path = torch.empty((batch, nodes), dtype=torch.int32, device=dev)
     count = torch.empty(batch, dtype=torch.int32, device=dev)
     token = torch.empty(batch, dtype=torch.int64, device=dev)

@@ -13,8 +13,9 @@
 // tensor cores with the codes as they are, and the fp32 operand (q, and the
 // weights times vs) as the sum of two fp16 values, which keeps 22 bits of it:
 // q is scaled by a power of two per row so that its largest value lies in
-// [2^13, 2^14), w * vs by one per warp, so that no half is lost to fp16's
-// range.  Sums are 32-bit; the tensor core's sum of a step of keys is added to
+// [2^13, 2^14), and the softmax's exponent is measured from the row's running
+// maximum of s + log2(vs), which puts its largest w * vs there too, so that no
+// half is lost to fp16's range.  Sums are 32-bit; the tensor core's sum of a step of keys is added to
 // the row's sum by an fp32 multiply-add that also carries the softmax's
 // rescaling, so that long contexts do not add up its truncation.
 //
@@ -32,37 +33,16 @@
 // a SM, so that ragged batches and long single sequences fill the GPU alike; a
 // (sequence, head, row tile) that spans several ranges leaves its parts in the
 // workspace, and a second kernel joins them.
-#include <cuda_fp16.h>
-#include <math.h>
-
 #include <algorithm>
 #include <atomic>
 
-#include "kz_cache.cuh"
+#include "kz_cache_attention.cuh"
 
 namespace kz {
 namespace {
 
-constexpr int kKT = 128;                    // keys a tile
 constexpr int kConsumers = 128;             // four warps compute, a fifth loads
 constexpr int kCaThreads = kConsumers + 32;
-constexpr int kMinTiles = 4;                // tiles a CTA's range has at least
-constexpr int kTreeWords = KZ_TREE_MAX_NODES / 32;
-
-struct CacheAttArgs {
-    CacheView c;
-    SeqView s;
-    const float* q;
-    int64_t q_bs, q_rs;
-    const int32_t* counts;
-    const int32_t* parents;
-    int64_t parents_bs;
-    float* out;
-    float* parts;          // two slots a CTA: sums [RT][D], maxima [RT], weights [RT]; NULL: every range is whole
-    int batch, tokens, heads, group;
-    float scale;
-    int* status;
-};
 
 template <int D, int NT_, int RG_>
 struct Shape {
@@ -76,80 +56,6 @@ struct Shape {
     static constexpr int UBYTES = KG > 1 && RT * PITCH * 4 > QBYTES ? RT * PITCH * 4 : QBYTES;
     static constexpr int SMEM = STAGES * STAGE + UBYTES + 1024;
     static constexpr int SLOT = RT * (D + 2);               // floats of a part
-};
-
-// ------------------------------------------------------------- the schedule
-
-// A sequence's share of the work.
-struct Seq {
-    int len, count, tiles, row_tiles;
-};
-template <int RT>
-__device__ __forceinline__ Seq sequence(const CacheAttArgs& a, int b) {
-    Seq s;
-    const int64_t most = (int64_t)a.s.cols * a.c.page;
-    s.len = (int)min((int64_t)max(0, a.s.lengths[b]), most);
-    s.count = a.counts ? max(0, min(a.counts[b], a.tokens)) : a.tokens;
-    s.tiles = (int)(((int64_t)s.len + s.count + kKT - 1) / kKT);
-    s.row_tiles = (int)(((int64_t)s.count * a.group + RT - 1) / RT);
-    return s;
-}
-__device__ __forceinline__ int64_t units_of(const CacheAttArgs& a, const Seq& s) {
-    return (int64_t)s.row_tiles * a.c.heads * (a.parts ? s.tiles : 1);   // whole ranges: a unit is a row tile
-}
-__device__ __forceinline__ int64_t units_a_cta(const CacheAttArgs& a, int64_t total, int ctas) {
-    const int64_t per = (total + ctas - 1) / ctas;
-    return a.parts ? max(per, (int64_t)kMinTiles) : max(per, (int64_t)1);
-}
-
-// Sum of a value over the 128 threads that share `sum` (named barrier 1).
-__device__ __forceinline__ int64_t sum_128(int64_t v, int64_t* sum) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if ((threadIdx.x & 31) == 0) sum[threadIdx.x >> 5] = v;
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    return sum[0] + sum[1] + sum[2] + sum[3];
-}
-
-// A part of one (sequence, head, row tile): key tiles [t0, t1).
-struct Segment {
-    int b, h, rt, t0, t1;
-    int len, count;
-    int first_token, last_token;   // of the row tile
-    bool whole;                    // all of its tiles
-};
-
-// Walks the segments of units [at, end): b0, base: the sequence that holds `at` and its first unit.
-template <int RT>
-struct Walk {
-    int64_t at, end, base;
-    int b;
-    Seq s;
-    __device__ __forceinline__ bool next(const CacheAttArgs& a, Segment& g) {
-        if (at >= end) return false;
-        while (at >= base + units_of(a, s)) {
-            if (b + 1 >= a.batch) return false;
-            base += units_of(a, s);
-            s = sequence<RT>(a, ++b);
-        }
-        const int64_t off = at - base;
-        const int per = a.parts ? s.tiles : 1;
-        const int hr = (int)(off / per);
-        g.b = b;
-        g.h = hr / s.row_tiles;
-        g.rt = hr % s.row_tiles;
-        g.t0 = (int)(off % per);
-        const int take = (int)min((int64_t)(per - g.t0), end - at);
-        g.whole = take == per;
-        g.t1 = a.parts ? g.t0 + take : s.tiles;
-        at += take;
-        g.len = s.len;
-        g.count = s.count;
-        g.first_token = g.rt * RT / a.group;
-        g.last_token = min(s.count - 1, (g.rt * RT + RT - 1) / a.group);
-        g.t1 = min(g.t1, (g.len + g.last_token) / kKT + 1);   // later tiles: no row of this tile sees them
-        return true;
-    }
 };
 
 // ------------------------------------------------------------ mma and codes
@@ -176,31 +82,6 @@ __device__ __forceinline__ uint32_t transposed_8x8(uint32_t v) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-// Two of a word's four codes (offset by 128) as fp16: the byte in the mantissa
-// of 1024, less 1152.
-template <int SEL>
-__device__ __forceinline__ uint32_t two_codes(uint32_t w) {
-    const uint32_t m = __byte_perm(w, 0x64646464u, SEL);
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(0x64806480u));
-    return r;
-}
-__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-// x's 11 leading bits; the rest, x less them, is exact
-__device__ __forceinline__ float leading(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFFE000u); }
-__device__ __forceinline__ float exp2_approx(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-// exp2(m - top), 0 where m is -inf (no key yet)
-__device__ __forceinline__ float shrink(float m, float top) { return m == -INFINITY ? 0.0f : exp2_approx(m - top); }
-__device__ __forceinline__ float pow2_field(int field) { return __uint_as_float((uint32_t)field << 23); }
-
 template <int D>
 __device__ __forceinline__ uint32_t swizzled(uint32_t off) {   // byte offset in a tile of rows of D bytes
     return D == 128 ? off ^ ((off >> 3) & 0x70u) : D == 64 ? off ^ ((off >> 3) & 0x30u) : off ^ ((off >> 3) & 0x10u);
@@ -214,7 +95,7 @@ __global__ void __launch_bounds__(kCaThreads, 2)
                            const CacheAttArgs a) {
     using S = Shape<D, NT, RG>;
     extern __shared__ uint8_t ca_smem[];
-    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ca_smem) + 1023) & ~(uintptr_t)1023);
+    uint8_t* ring = ca_smem + (-smem_u32(ca_smem) & 1023u);      // an offset, so that accesses stay shared-memory ones
     uint4* q_ops = reinterpret_cast<uint4*>(ring + S::STAGES * S::STAGE);   // [RT / 8][D / 16][32]: hi, hi, lo, lo
     float* joined = reinterpret_cast<float*>(q_ops);                        // [RT][PITCH], once q is done with
     __shared__ __align__(8) uint64_t s_full[S::STAGES], s_empty[S::STAGES];
@@ -223,12 +104,12 @@ __global__ void __launch_bounds__(kCaThreads, 2)
     __shared__ float s_m[S::KG][S::RT], s_l[S::KG][S::RT];
     __shared__ uint32_t s_sees[S::RT + 1][kTreeWords];
     __shared__ int32_t s_parent[KZ_TREE_MAX_NODES];
-    __shared__ int64_t s_sum[4], s_part[kConsumers];
-    __shared__ int64_t s_start[2];                 // this CTA's first sequence and that one's first unit
-    __shared__ int64_t s_units[2];                 // its units
+    __shared__ int s_sum[4], s_part[kConsumers];
+    __shared__ int s_start[2];                     // this CTA's first sequence and that one's first unit
+    __shared__ int s_units[2];                     // its units
     __shared__ int s_abort;
 
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // uniform: so are the roles' branches
     if (tid == 0) {
         for (int i = 0; i < S::STAGES; ++i) {
             mbar_init(smem_u32(&s_full[i]), 1);
@@ -243,22 +124,21 @@ __global__ void __launch_bounds__(kCaThreads, 2)
     // ---- this CTA's units, and where they begin
     if (warp < 4) {
         const int each = (a.batch + kConsumers - 1) / kConsumers;
-        int64_t mine = 0;
+        int mine = 0;
         for (int b = tid * each; b < min(a.batch, (tid + 1) * each); ++b) mine += units_of(a, sequence<S::RT>(a, b));
         s_part[tid] = mine;
-        const int64_t total = sum_128(mine, s_sum);
+        const int total = sum_128(mine, s_sum);
         if (tid == 0) {
-            const int64_t per = units_a_cta(a, total, gridDim.x);
-            const int64_t u0 = min(total, per * blockIdx.x), u1 = min(total, u0 + per);
+            const int per = units_a_cta(a, total, gridDim.x);
+            const int u0 = (int)min((int64_t)total, (int64_t)per * blockIdx.x), u1 = (int)min((int64_t)total, (int64_t)u0 + per);
             s_units[0] = u0;
             s_units[1] = u1;
-            int64_t base = 0;
-            int i = 0, b = 0;
+            int base = 0, i = 0, b = 0;
             if (u0 < u1) {
                 while (i < kConsumers - 1 && base + s_part[i] <= u0) base += s_part[i++];
                 b = i * each;
                 for (; b < a.batch - 1; ++b) {
-                    const int64_t n = units_of(a, sequence<S::RT>(a, b));
+                    const int n = units_of(a, sequence<S::RT>(a, b));
                     if (u0 < base + n) break;
                     base += n;
                 }
@@ -271,7 +151,7 @@ __global__ void __launch_bounds__(kCaThreads, 2)
     Walk<S::RT> walk;
     walk.at = s_units[0];
     walk.end = s_units[1];
-    walk.b = (int)s_start[0];
+    walk.b = s_start[0];
     walk.base = s_start[1];
     if (walk.at < walk.end) walk.s = sequence<S::RT>(a, walk.b);
     Segment g;
@@ -373,7 +253,6 @@ __global__ void __launch_bounds__(kCaThreads, 2)
 
             float o[NT][D / 16][4], m[NT][2], l[NT][2], qs[NT][2];
             int token[NT][2];
-            int ex = 14;                                          // vs is scaled by 2^(140 - ex): the largest below 2^14
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -443,20 +322,15 @@ __global__ void __launch_bounds__(kCaThreads, 2)
                             }
                     }
 
-                    // ---- scales; the step's largest vs (of keys that are there) sets the power of two
-                    float ks[2][2], vs[2][2];
-                    uint32_t top = __float_as_uint(vs_t[kl + lane]) & 0x7FFFFFFFu;
-                    if (top >= 0x7F800000u || (masked && (k0 + lane >= limit || (bad >> ((kl + lane) >> a.c.shift)) & 1u))) top = 0;
-                    const int ex_new = max(ex, (int)(__reduce_max_sync(0xffffffffu, top) >> 23));
-                    const float vs_up = pow2_field(267 - ex_new);
-                    const float ex_shrink = pow2_field(max(0, 127 + ex - ex_new));
-                    ex = ex_new;
+                    // ---- scales
+                    float ks[2][2], vs[2][2], lv[2][2];
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             ks[mt][j] = ks_t[kl + mt * 16 + j * 8 + gq];
-                            vs[mt][j] = vs_t[kl + mt * 16 + j * 8 + gq] * vs_up;
+                            vs[mt][j] = vs_t[kl + mt * 16 + j * 8 + gq];
+                            lv[mt][j] = log2_vs(vs[mt][j]);
                         }
 
                     // ---- softmax, one pass: new maximum, weights, and the weights times vs as two halves
@@ -485,25 +359,25 @@ __global__ void __launch_bounds__(kCaThreads, 2)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 z[mt][e] = s[mt][n][e] * ks[mt][e >> 1] * qs[n][e & 1];
-                                if (!((seen >> (4 * mt + e)) & 1u)) z[mt][e] = -INFINITY;
-                                mx[e & 1] = fmaxf(mx[e & 1], z[mt][e]);
+                                float x = z[mt][e] + lv[mt][e >> 1];
+                                if (!((seen >> (4 * mt + e)) & 1u)) z[mt][e] = x = -INFINITY;
+                                mx[e & 1] = fmaxf(mx[e & 1], x);
                             }
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
 #pragma unroll
                             for (int x = 4; x <= 16; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
-                            const float c = shrink(m[n][j], mx[j]);
+                            corr[n][j] = shrink(m[n][j], mx[j]);
                             m[n][j] = mx[j];
-                            l[n][j] *= c;
-                            corr[n][j] = c * ex_shrink;
-                            if (mx[j] == -INFINITY) mx[j] = 0.0f;      // no key yet: every weight is 0
+                            l[n][j] *= corr[n][j];
+                            mx[j] = mx[j] == -INFINITY ? 0.0f : kLift - mx[j];      // -inf: no key yet, every weight is 0
                         }
 #pragma unroll
                         for (int mt = 0; mt < 2; ++mt) {
                             float hi[4], lo[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const float p = exp2_approx(z[mt][e] - mx[e & 1]);
+                                const float p = exp2_approx(z[mt][e] + mx[e & 1]);
                                 l[n][e & 1] += p;
                                 const float w = (seen >> (4 * mt + e)) & 1u ? p * vs[mt][e >> 1] : 0.0f;
                                 hi[e] = leading(w);
@@ -579,7 +453,6 @@ __global__ void __launch_bounds__(kCaThreads, 2)
                     }
                 }
             asm volatile("bar.sync 1, 128;" ::: "memory");     // and q is done with
-            const float unit = pow2_field(ex - 13);            // the warp's power of two taken back
             const bool direct = g.whole;
             float* slot = direct ? nullptr : a.parts + (2 * (int64_t)blockIdx.x + (first_segment ? 0 : 1)) * S::SLOT;
             first_segment = false;
@@ -594,7 +467,7 @@ __global__ void __launch_bounds__(kCaThreads, 2)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const int r = (rg * NT + n) * 8 + 2 * tq + j;
-                        const float f = direct ? (l[n][j] == 0.0f ? 0.0f : unit / l[n][j]) : unit;
+                        const float f = direct ? (l[n][j] == 0.0f ? 0.0f : 1.0f / l[n][j]) : 1.0f;
                         if (r < rows) {
                             float* dst = direct ? out_row(r) : slot + r * D;
 #pragma unroll
@@ -613,7 +486,7 @@ __global__ void __launch_bounds__(kCaThreads, 2)
                                 float M = -INFINITY;
 #pragma unroll
                                 for (int k = 0; k < S::KG; ++k) M = fmaxf(M, s_m[k][r]);
-                                const float f = shrink(m[n][j], M) * unit;
+                                const float f = shrink(m[n][j], M);
 #pragma unroll
                                 for (int i = 0; i < D / 16; ++i) {
                                     float2* p = reinterpret_cast<float2*>(joined + r * S::PITCH + 16 * i + 2 * gq);
@@ -655,19 +528,24 @@ __global__ void __launch_bounds__(kCaThreads, 2)
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
 }
 
-// Joins the parts of one (sequence, head, row tile) that several CTAs left:
-// with M the largest of their maxima, o = sum f_c o_c / sum f_c l_c, f_c =
-// 2^(m_c - M).  A warp a row, a lane D / 32 of its values.
+// Joins the parts of a (sequence, head, row tile) that several CTAs left: with
+// M the largest of their maxima, o = sum f_c o_c / sum f_c l_c, f_c =
+// 2^(m_c - M).  Latency bounds it (a row's parts are few and far apart), so a
+// block has four rows only, a lane D / 32 of a row's values; up to four parts
+// are a warp's work, more are dealt out to the four warps, each with a maximum
+// of its own, and joined once more.
+constexpr int kJoinRows = 4;
 template <int D, int RT>
 __global__ void __launch_bounds__(kConsumers) cache_attention_join_kernel(const CacheAttArgs a, int ctas) {
-    __shared__ int64_t s_sum[4];
-    constexpr int E = D / 32, SLOT = RT * (D + 2);
+    constexpr int E = D / 32, SLOT = RT * (D + 2), BLOCKS = RT / kJoinRows;
+    __shared__ int s_sum[4];
+    __shared__ float s_part[4][kJoinRows][D], s_m[4][kJoinRows], s_l[4][kJoinRows];
     griddep_launch_dependents();
-    const int b = blockIdx.y, lane = threadIdx.x & 31;
+    const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // lengths and counts were written before the kernel that left the parts began
-    int64_t before = 0, total = 0;
+    int before = 0, total = 0;
     for (int i = threadIdx.x; i < a.batch; i += kConsumers) {
-        const int64_t n = units_of(a, sequence<RT>(a, i));
+        const int n = units_of(a, sequence<RT>(a, i));
         total += n;
         if (i < b) before += n;
     }
@@ -676,36 +554,71 @@ __global__ void __launch_bounds__(kConsumers) cache_attention_join_kernel(const 
     before = sum_128(before, s_sum);
     griddep_wait();
     const Seq s = sequence<RT>(a, b);
-    const int h = blockIdx.x % a.c.heads, rt = blockIdx.x / a.c.heads;
-    if (rt >= s.row_tiles) return;
-    const int64_t per = units_a_cta(a, total, ctas);
-    const int64_t u0 = before + ((int64_t)h * s.row_tiles + rt) * s.tiles, u1 = u0 + s.tiles;
-    const int c0 = (int)(u0 / per), c1 = (int)((u1 - 1) / per);
+    const int tile = blockIdx.x / BLOCKS, h = tile % a.c.heads, rt = tile / a.c.heads;
+    const int r0 = (blockIdx.x % BLOCKS) * kJoinRows, rows = min(RT, s.count * a.group - rt * RT) - r0;   // of this block
+    if (rt >= s.row_tiles || rows <= 0) return;
+    const int per = units_a_cta(a, total, ctas);
+    const int u0 = before + (h * s.row_tiles + rt) * s.tiles, c0 = u0 / per, c1 = (u0 + s.tiles - 1) / per;
     if (c0 == c1) return;                                       // one CTA had it all
-    const int rows = min(RT, s.count * a.group - rt * RT);
     auto slot = [&](int c) {                                    // a CTA's first part is in its first slot
         return a.parts + (2 * (int64_t)c + (c > c0 || c0 * per == u0 ? 0 : 1)) * SLOT;
     };
-    for (int r = threadIdx.x >> 5; r < rows; r += kConsumers / 32) {
-        float M = -INFINITY, L = 0.0f, o[E];
-        for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, slot(c)[RT * D + r]);
+    // the sums of row r over the parts first, first + step, ...
+    auto gather = [&](int r, int first, int step, float& M, float& L, float (&o)[E]) {
+        M = -INFINITY;
+        L = 0.0f;
+        for (int c = first + step * lane; c <= c1; c += 32 * step) M = fmaxf(M, slot(c)[RT * D + r]);
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = 0.0f;
 #pragma unroll 4
-        for (int c = c0; c <= c1; ++c) {
+        for (int c = first; c <= c1; c += step) {
             const float* p = slot(c);
             const float f = shrink(p[RT * D + r], M);
             L = fmaf(p[RT * D + RT + r], f, L);
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(p[r * D + lane * E + e], f, o[e]);
+            for (int e = 0; e < E; ++e) o[e] = fmaf(p[r * D + lane + 32 * e], f, o[e]);
         }
+    };
+    auto finish = [&](int r, float L, const float (&o)[E]) {
         const float f = L == 0.0f ? 0.0f : 1.0f / L;
         const int R = rt * RT + r;
         float* dst = a.out + ((int64_t)b * a.tokens + R / a.group) * a.heads * D + ((int64_t)h * a.group + R % a.group) * D;
 #pragma unroll
-        for (int e = 0; e < E; ++e) dst[lane * E + e] = o[e] * f;
+        for (int e = 0; e < E; ++e) dst[lane + 32 * e] = o[e] * f;
+    };
+    float M, L, o[E];
+    if (c1 - c0 < 4) {
+        if (warp < rows) {
+            gather(r0 + warp, c0, 1, M, L, o);
+            finish(r0 + warp, L, o);
+        }
+        return;
+    }
+    for (int i = 0; i < min(rows, kJoinRows); ++i) {
+        gather(r0 + i, c0 + warp, 4, M, L, o);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s_part[warp][i][lane + 32 * e] = o[e];
+        if (lane == 0) {
+            s_m[warp][i] = M;
+            s_l[warp][i] = L;
+        }
+    }
+    __syncthreads();
+    if (warp < rows) {
+        M = fmaxf(fmaxf(s_m[0][warp], s_m[1][warp]), fmaxf(s_m[2][warp], s_m[3][warp]));
+        L = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = shrink(s_m[w][warp], M);
+            L = fmaf(s_l[w][warp], f, L);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(s_part[w][warp][lane + 32 * e], f, o[e]);
+        }
+        finish(r0 + warp, L, o);
     }
 }
 
@@ -718,7 +631,13 @@ int tile_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 3
 // holds no more tiles than a CTA's range has at least.
 bool whole_ranges(int64_t cols, int64_t page) { return cols * page <= (int64_t)kMinTiles * kKT; }
 
-int64_t parts_floats(int64_t rows, int64_t d) { return 2 * 2 * (int64_t)sm_count() * tile_rows(rows) * (d + 2); }
+// Whether the rows of a key head are many enough for the tcgen05 kernel.
+bool many_rows(int64_t rows) { return rows > 16; }
+
+int64_t parts_floats(int64_t rows, int64_t d) {
+    const int64_t ctas = (many_rows(rows) ? 1 : 2) * (int64_t)sm_count();
+    return 2 * ctas * (many_rows(rows) ? kTcRows : tile_rows(rows)) * (d + 2);
+}
 
 template <int D, int NT, int RG>
 int launch_cache_attention(const CacheAttArgs& a, int64_t row_tiles, cudaStream_t s) {
@@ -741,13 +660,22 @@ int launch_cache_attention(const CacheAttArgs& a, int64_t row_tiles, cudaStream_
     KZ_CHECK_CUDA(launch_pdl(cache_attention_kernel<D, NT, RG>, dim3(grid), dim3(kCaThreads), S::SMEM, s, tm_k, tm_v, a));
     if (a.parts)
         KZ_CHECK_CUDA(launch_pdl(cache_attention_join_kernel<D, S::RT>,
-                                 dim3((unsigned)(row_tiles * a.c.heads), (unsigned)a.batch), dim3(kConsumers), 0, s, a, grid));
+                                 dim3((unsigned)(row_tiles * a.c.heads * (S::RT / kJoinRows)), (unsigned)a.batch), dim3(kConsumers), 0, s, a, grid));
     return KZ_OK;
 }
 
 template <int D>
 int dispatch_cache_attention(const CacheAttArgs& a, cudaStream_t s) {
     const int64_t rows = (int64_t)a.tokens * a.group;
+    if (many_rows(rows)) {
+        const int64_t tiles = (rows + kTcRows - 1) / kTcRows;
+        const int grid = (int)std::min<int64_t>(sm_count(), a.parts ? sm_count() : a.batch * a.c.heads * tiles);
+        const int st = launch_cache_attention_tc(a, D, grid, s);
+        if (!st && a.parts)
+            KZ_CHECK_CUDA(launch_pdl(cache_attention_join_kernel<D, kTcRows>,
+                                     dim3((unsigned)(tiles * a.c.heads * (kTcRows / kJoinRows)), (unsigned)a.batch), dim3(kConsumers), 0, s, a, grid));
+        return st;
+    }
     const int rt = tile_rows(rows);
     const int64_t row_tiles = (rows + rt - 1) / rt;
     if (rt == 8) return launch_cache_attention<D, 1, 1>(a, row_tiles, s);
@@ -785,6 +713,9 @@ extern "C" int kz_cache_attention_f32(const kz_cache* cache, const float* q, int
                "kz_cache_attention_f32: tokens * heads out of range");
     KZ_REQUIRE(table_cols * cache->page_size < (int64_t)INT32_MAX - (1 << 25),
                "kz_cache_attention_f32: table_cols * page_size out of range");
+    const int64_t most_tiles = (table_cols * cache->page_size + tokens) / kKT + 1;
+    KZ_REQUIRE(batch * cache->kv_heads * (tokens * (heads / cache->kv_heads) / 8 + 1) < (int64_t)INT32_MAX / most_tiles,
+               "kz_cache_attention_f32: the call's work is out of range");
     if (batch * tokens == 0) return KZ_OK;
     KZ_REQUIRE(q && out, "kz_cache_attention_f32: q or out is NULL");
     KZ_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0 &&

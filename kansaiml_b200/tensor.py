@@ -41,7 +41,8 @@ def _as_device(device):
 
 def stream_handle(device):
     """The raw cudaStream_t of torch's current stream on `device`."""
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def require_cuda(t, what):
