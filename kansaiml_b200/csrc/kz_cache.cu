@@ -40,8 +40,8 @@ struct WriteArgs {
     int64_t bs[2], rs[2];              // batch and row strides (floats)
     float* values[2];                  // what the codes stand for, [batch, tokens, heads * d], or NULL
     const int32_t* counts;
-    uint32_t tokens, rows;             // rows = batch * tokens * heads
-    FastDiv by_heads, by_tokens;
+    uint32_t tokens, items;            // items = batch * tokens * groups of heads
+    FastDiv by_groups, by_tokens;
     int* status;
 };
 
@@ -57,42 +57,44 @@ __device__ __forceinline__ float4 codes_times(uint32_t w, float s) {
     return v;
 }
 
-// One group of D / 4 lanes holds a row (16 bytes a lane); a warp works on
-// kU x 2 such row sets at a time (K and V of kU consecutive rows a group), so
-// 2 kU 16-byte loads are in flight a lane.  The rows' scales need two double
-// divisions each: they are handed to one lane a row and back by shuffles, so a
-// warp divides once for all its rows instead of once a row set.
+// A warp takes a token's next kU * G heads: G groups of D / 4 lanes (16 bytes a
+// lane) hold a row each, K and V of kU such row sets are in flight.  What
+// depends on the token alone (its page, its slot) is found once a warp.  The
+// rows' scales need two double divisions each: they are handed to one lane a
+// row and back by shuffles, so a warp divides once for all its rows.
 template <int D, int kU>
-__global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(WriteArgs a) {
+__global__ void __launch_bounds__(kCacheThreads, 4) cache_write_kernel(WriteArgs a) {
     constexpr int L = D / 4, G = 32 / L, N = 2 * kU * G;   // lanes a row, groups a warp, rows a warp
     static_assert(N <= 32, "a lane for each row's scale");
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const int lane = threadIdx.x & 31, sub = lane / L, col = 4 * (lane % L);
-    const uint32_t first = (blockIdx.x * (kCacheThreads / 32) + (threadIdx.x >> 5)) * (uint32_t)(kU * G);
-    if (first >= a.rows) return;
+    const uint32_t item = blockIdx.x * (kCacheThreads / 32) + __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    if (item >= a.items) return;
+    const uint32_t bt = div_by(item, a.by_groups), h0 = (item - bt * a.by_groups.d) * (kU * G) + sub;   // u adds u * G
+    const uint32_t b = div_by(bt, a.by_tokens), t = bt - b * a.by_tokens.d;
+    const int64_t out_at = ((int64_t)bt * a.c.heads + h0) * D + col;
+    if (a.counts && (int)t >= a.counts[b]) {               // padding: its values are 0
+#pragma unroll
+        for (int i = 0; i < 2 * kU; ++i)
+            if (h0 + (i >> 1) * G < (uint32_t)a.c.heads && a.values[i & 1])
+                __stcs(reinterpret_cast<float4*>(a.values[i & 1] + out_at + (i >> 1) * G * D), make_float4(0.f, 0.f, 0.f, 0.f));
+        return;
+    }
     float4 x[2 * kU];
-    int64_t row_at[kU];      // the row's place in the cache, -1: none
-    int64_t out_at[kU];      // and in the returned values, -1: past the last row
     uint32_t bits[2 * kU];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-        const uint32_t r = first + u * G + sub;
-        const uint32_t bt = div_by(r, a.by_heads), h = r - bt * a.by_heads.d;
-        const uint32_t b = div_by(bt, a.by_tokens), t = bt - b * a.by_tokens.d;
-        row_at[u] = -1;
-        out_at[u] = r < a.rows ? (int64_t)r * D + col : -1;
-        x[2 * u] = x[2 * u + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < a.rows && (!a.counts || (int)t < a.counts[b])) {
-            x[2 * u] = __ldcs(reinterpret_cast<const float4*>(a.x[0] + b * a.bs[0] + t * a.rs[0] + h * D + col));
-            x[2 * u + 1] = __ldcs(reinterpret_cast<const float4*>(a.x[1] + b * a.bs[1] + t * a.rs[1] + h * D + col));
-            const int page = page_of(a.c, a.s, b, (int64_t)a.s.lengths[b] + t);
-            if (page >= 0)
-                row_at[u] = ((int64_t)page * a.c.heads + h) * a.c.page + ((a.s.lengths[b] + (int)t) & (a.c.page - 1));
-            else if (lane % L == 0)
-                record_status(a.status, KZ_ERR_INVALID_ARGUMENT);
-        }
+    for (int i = 0; i < 2 * kU; ++i) {
+        const int kv = i & 1;
+        const uint32_t h = h0 + (i >> 1) * G;
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (h < (uint32_t)a.c.heads)
+            x[i] = __ldcs(reinterpret_cast<const float4*>(a.x[kv] + b * a.bs[kv] + t * a.rs[kv] + h * D + col));
     }
+    const int64_t pos = (int64_t)a.s.lengths[b] + t;
+    const int page = page_of(a.c, a.s, b, pos);
+    if (page < 0 && lane == 0) record_status(a.status, KZ_ERR_INVALID_ARGUMENT);
+    const int64_t row_at = ((int64_t)page * a.c.heads + h0) * a.c.page + (pos & (a.c.page - 1));
 #pragma unroll
     for (int i = 0; i < 2 * kU; ++i) {
         uint32_t m = max(max(abs_bits(x[i].x), abs_bits(x[i].y)), max(abs_bits(x[i].z), abs_bits(x[i].w)));
@@ -104,7 +106,7 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(WriteArgs a)
     uint32_t mine = 0;
 #pragma unroll
     for (int i = 0; i < 2 * kU; ++i) {
-        const uint32_t m = __shfl_sync(0xffffffffu, bits[i], (lane % G) * L);
+        const uint32_t m = G == 1 ? bits[i] : __shfl_sync(0xffffffffu, bits[i], (lane % G) * L);
         if (lane / G == i) mine = m;
     }
     const ScaleInfo si = scale_from_absmax_bits(mine);
@@ -114,23 +116,24 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(WriteArgs a)
         const int u = i >> 1, kv = i & 1;
         const float s = __shfl_sync(0xffffffffu, s32, i * G + sub);
         const float rcp = __shfl_sync(0xffffffffu, si.rcp, i * G + sub);
-        if (out_at[u] < 0) continue;
+        if (h0 + u * G >= (uint32_t)a.c.heads) continue;
         uint32_t w = 0;
-        if (bits[i] < kInfBits) {
+        if (bits[i] - 1 < kInfBits - 1) {            // neither zeros nor NaN/Inf, whose codes are 0
             const bool fast = bits[i] >= __float_as_uint(7.8886090522101181e-31f);   // as scale_from_absmax_bits has it
             float near;
             w = pack4_fast(x[i], rcp, near);
             if (!fast || near > kTieGuardFma)
                 w = pack4_repair(x[i], w, scale_from_absmax_bits(bits[i]).scale, rcp, fast);
         }
-        if (row_at[u] >= 0) {
-            *reinterpret_cast<uint32_t*>(a.c.codes[kv] + row_at[u] * D + col) = w;
+        if (page >= 0) {
+            const int64_t row = row_at + (int64_t)u * G * a.c.page;
+            *reinterpret_cast<uint32_t*>(a.c.codes[kv] + row * D + col) = w;
             if (col == 0) {
-                a.c.scale[kv][row_at[u]] = s;
+                a.c.scale[kv][row] = s;
                 if (bits[i] >= kInfBits) record_status(a.status, KZ_ERR_NONFINITE);
             }
         }
-        if (a.values[kv]) __stcs(reinterpret_cast<float4*>(a.values[kv] + out_at[u]), codes_times(w, s));
+        if (a.values[kv]) __stcs(reinterpret_cast<float4*>(a.values[kv] + out_at + u * G * D), codes_times(w, s));
     }
 }
 
@@ -149,8 +152,8 @@ struct ReadArgs {
 template <int D>
 __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(ReadArgs a) {
     constexpr int L = D / 4, G = 32 / L;
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const int lane = threadIdx.x & 31, sub = lane / L, col = 4 * (lane % L);
     const uint32_t item = blockIdx.x * (kCacheThreads / 32) + (threadIdx.x >> 5);
     if (item >= a.items) return;
@@ -212,8 +215,8 @@ struct KeepArgs {
 template <int D>
 __global__ void __launch_bounds__(kCacheThreads) cache_keep_kernel(KeepArgs a) {
     constexpr int L = D / 16, G = 32 / L;    // 16 codes a lane
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const int lane = threadIdx.x & 31, sub = lane / L, col = 16 * (lane % L);
     const int64_t item = (int64_t)blockIdx.x * (kCacheThreads / 32) + (threadIdx.x >> 5);
     if (item >= (int64_t)a.batch * a.c.heads) return;
@@ -258,12 +261,17 @@ __global__ void __launch_bounds__(kCacheThreads) cache_keep_kernel(KeepArgs a) {
     }
 }
 
+// Row sets a warp holds: as many as the heads fill, four at most.
 template <int D>
-int launch_write(const WriteArgs& a, cudaStream_t s) {
-    constexpr int kU = 4;
-    const uint32_t per_block = (kCacheThreads / 32) * kU * (128 / D);
-    KZ_CHECK_CUDA(launch_pdl(cache_write_kernel<D, kU>, dim3((a.rows + per_block - 1) / per_block),
-                             dim3(kCacheThreads), 0, s, a));
+int launch_write(WriteArgs a, int64_t batch, cudaStream_t s) {
+    constexpr int G = 128 / D;
+    const int sets = a.c.heads <= G ? 1 : a.c.heads <= 2 * G ? 2 : 4;
+    const uint32_t groups = (uint32_t)((a.c.heads + sets * G - 1) / (sets * G));
+    a.items = (uint32_t)(batch * a.tokens * groups);
+    a.by_groups = fast_div(groups);
+    const dim3 grid((a.items + kCacheThreads / 32 - 1) / (kCacheThreads / 32));
+    auto kernel = sets == 1 ? cache_write_kernel<D, 1> : sets == 2 ? cache_write_kernel<D, 2> : cache_write_kernel<D, 4>;
+    KZ_CHECK_CUDA(launch_pdl(kernel, grid, dim3(kCacheThreads), 0, s, a));
     return KZ_OK;
 }
 
@@ -338,13 +346,12 @@ extern "C" int kz_cache_write_f32(const kz_cache* cache, const float* k, const f
     a.values[1] = v_values;
     a.counts = counts;
     a.tokens = (uint32_t)tokens;
-    a.rows = (uint32_t)(batch * tokens * cache->kv_heads);
-    a.by_heads = fast_div((uint32_t)cache->kv_heads);
     a.by_tokens = fast_div((uint32_t)tokens);
     a.status = device_status_ptr();
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    return cache->head_dim == 32 ? launch_write<32>(a, s) : cache->head_dim == 64 ? launch_write<64>(a, s)
-                                                                                  : launch_write<128>(a, s);
+    return cache->head_dim == 32   ? launch_write<32>(a, batch, s)
+           : cache->head_dim == 64 ? launch_write<64>(a, batch, s)
+                                   : launch_write<128>(a, batch, s);
 }
 
 extern "C" int kz_cache_read_f32(const kz_cache* cache, const int32_t* table, int64_t table_cols,

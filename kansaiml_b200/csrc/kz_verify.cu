@@ -9,15 +9,24 @@
 //     u[j] * q(x[j]) < r(x[j])   accept: j becomes the current node, r = p[j]
 //     otherwise                  reject: r = (r - q)+ / sum (r - q)+  (unchanged where that sum is 0)
 // and the next token is the smallest i with r(0) + .. + r(i) > u * sum r.
-// Everything is computed in double from the fp32 rows, so that the decisions
-// do not depend on how the work is split.
+// Everything is computed in double from the fp32 rows (or in two fp32 parts
+// that keep as much), so that the decisions do not depend on how the work is
+// split.
+//
+// After k rejections at a node r is (p - c_k q)+ / t_k with c_0 = 0, t_0 = 1,
+// c_(k+1) = c_k + t_k and t_(k+1) = sum (p - c_(k+1) q)+: dividing the rule's
+// r_k = (p - c_k q)+ / t_k through, (r_k - q)+ is (p - (c_k + t_k) q)+ / t_k.
 //
 // Each sequence is walked by one cluster: every CTA takes a slice of the
 // vocabulary and repeats the walk itself (the accept tests need single values
 // only, gathered up front), so that the cluster meets once a rejection and
 // once at the end, to exchange the slices' sums through distributed shared
-// memory.  A rejection reads two rows (one without a draft), the last token
-// the same rows once more; nothing else of the probabilities is touched.
+// memory.  With a draft each rejection is a pass over two rows; if the walk
+// ends with it, its sums are those that the last token is drawn by.  Without
+// one r is p with the rejected tokens taken out, over what is left: one pass
+// over a node's row gives its sum, from which each rejected token's p is
+// subtracted.  Nothing else of the probabilities is touched.  What bounds it is latency, so a warp loads all of
+// its part of a slice (8 chunks, 128 values of each at a time) before it adds anything up.
 #include <math.h>
 
 #include <algorithm>
@@ -27,7 +36,7 @@
 namespace kz {
 namespace {
 
-constexpr int kVThreads = 512, kVWarps = kVThreads / 32;
+constexpr int kVThreads = 256, kVWarps = kVThreads / 32, kVChunks = 8;
 constexpr int kVMaxNodes = 1024;
 constexpr int kVMaxCluster = 8;
 
@@ -42,18 +51,23 @@ struct VerifyArgs {
     int32_t* path;             // [B, N]
     int32_t* count;            // [B]
     int64_t* next;             // [B]
-    int nodes, vocab, per;     // per: values a CTA's slice holds (a multiple of 128 * warps)
+    int nodes, vocab, chunk;   // chunk: a multiple of 128 values; a warp has kVChunks, a slice all its warps' chunks
+    int wide;                  // rows start on 16 bytes
     int* status;
 };
 
 struct VerifyShared {
     double sum[2][kVMaxCluster];       // the slices' sums, a buffer for each of two successive meetings
-    double warp_sum[kVWarps];
-    double scale[kVMaxNodes];          // 1 / sum of each rejection at the current node
+    double chunk_sum[kVWarps][kVChunks];
+    // the rejections at the current node
+    double c, t;                       // see above; without a draft t is the sum of what is left
+    double gone_p[kVMaxNodes];         // without a draft: the rejected tokens and their p
+    int gone[kVMaxNodes];
     float p_at[kVMaxNodes], q_at[kVMaxNodes], u[kVMaxNodes];
     int parent[kVMaxNodes], token[kVMaxNodes];
-    int gone[kVMaxNodes];              // no draft: the tokens rejected at the current node
     int rejections, node, child, found;
+    int summed;                        // the node whose sums are in `sum` and `chunk_sum`: of p without a draft, with
+                                       // one of (p - c q)+
 };
 
 __device__ __forceinline__ double warp_sum_f64(double v) {
@@ -62,31 +76,110 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
     return v;
 }
 
-// r at token i, from the target's and the draft's value there
-__device__ __forceinline__ double rest_at(const VerifyShared& s, bool has_draft, int i, float p, float q) {
-    double r = p;
-    for (int k = 0; k < s.rejections; ++k) {
-        if (has_draft)
-            r = fmax(r - (double)q, 0.0) * s.scale[k];
-        else
-            r = s.gone[k] == i ? 0.0 : r * s.scale[k];
-    }
-    return r;
+__device__ __forceinline__ bool is_gone(const VerifyShared& s, int x) {
+    for (int k = 0; k < s.rejections; ++k)
+        if (s.gone[k] == x) return true;
+    return false;
+}
+// r at node j's token, of its parent's row
+__device__ __forceinline__ double rest_at(const VerifyShared& s, bool has_draft, int j) {
+    const double p = s.p_at[j];
+    if (s.rejections == 0) return p;
+    if (!has_draft) return is_gone(s, s.token[j]) ? 0.0 : p / s.t;
+    return fmax(p - s.c * (double)s.q_at[j], 0.0) / s.t;
+}
+// without a draft, the node's sum known: token of node j rejected
+__device__ __forceinline__ void take_out(VerifyShared& s, int j, double sum) {
+    if (is_gone(s, s.token[j])) return;
+    const double left = (s.rejections == 0 ? sum : s.t) - (double)s.p_at[j];
+    if (!(left > 0.0)) return;
+    s.t = left;
+    s.gone[s.rejections] = s.token[j];
+    s.gone_p[s.rejections++] = s.p_at[j];
 }
 
-__global__ void __launch_bounds__(kVThreads) verify_tree_kernel(VerifyArgs a) {
+// Sums of eight values a lane over the warp: lane l gets value (l >> 2)'s in
+// nine exchanges, each of the first three halving the values a lane has.
+__device__ __forceinline__ double warp_sums_f64(double (&v)[kVChunks]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = 4; h > 0; h >>= 1) {
+        const bool up = lane & (4 * h);
+#pragma unroll
+        for (int i = 0; i < h; ++i) {
+            const double give = up ? v[i] : v[i + h], keep = up ? v[i + h] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, 4 * h);
+        }
+    }
+    double t = v[0];
+    t += __shfl_xor_sync(0xffffffffu, t, 2);
+    t += __shfl_xor_sync(0xffffffffu, t, 1);
+    return t;
+}
+
+// Sums of fp32 values without a double per value (whose conversions and
+// additions bound the pass): pairs of values added to a sum kept as two fp32
+// parts, each addition's rounding error recovered (Knuth's two-sum) and kept in
+// the second.  n additions lose at most n 2^-48 of the terms' sum.
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t sub2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t r, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+struct TwoPart {
+    uint64_t hi, lo;       // two sums side by side
+    __device__ __forceinline__ void add(uint64_t x) {
+        const uint64_t s = add2(hi, x), b = sub2(s, hi);
+        lo = add2(lo, add2(sub2(hi, sub2(s, b)), sub2(x, b)));
+        hi = s;
+    }
+    // adds (p - q)+ = p - min(p, q): the difference's own rounding error is exact, as p is the larger
+    __device__ __forceinline__ void add_rest(float p0, float p1, float q0, float q1) {
+        const uint64_t p = pair(p0, p1), q = pair(fminf(q0, p0), fminf(q1, p1)), d = sub2(p, q);
+        add(d);
+        lo = add2(lo, sub2(sub2(p, d), q));
+    }
+    __device__ __forceinline__ double sum() const {
+        float a, b, c, d;
+        unpair(hi, a, b);
+        unpair(lo, c, d);
+        return ((double)a + (double)b) + ((double)c + (double)d);
+    }
+};
+
+// Four values of a row from i on, 0 at and past `end`.
+__device__ __forceinline__ float4 four(const float* row, int i, int end, int wide) {
+    if (wide && i + 3 < end) return __ldg(reinterpret_cast<const float4*>(row + i));
+    return make_float4(i < end ? __ldg(row + i) : 0.0f, i + 1 < end ? __ldg(row + i + 1) : 0.0f,
+                       i + 2 < end ? __ldg(row + i + 2) : 0.0f, i + 3 < end ? __ldg(row + i + 3) : 0.0f);
+}
+
+__global__ void __launch_bounds__(kVThreads, 2) verify_tree_kernel(VerifyArgs a) {
     __shared__ VerifyShared s;
-    griddep_launch_dependents();
     griddep_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    griddep_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
     uint32_t rank, ranks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
     const int64_t b = blockIdx.x / ranks;
     const float* target = a.target + b * a.nodes * (int64_t)a.vocab;
     const float* draft = a.draft ? a.draft + b * a.nodes * (int64_t)a.vocab : nullptr;
-    for (int j = tid; j < a.nodes; j += kVThreads) {
-        int parent = a.parents[b * a.parents_bs + j];
+    for (int j = tid; j < a.nodes; j += blockDim.x) {
+        const int parent = a.parents[b * a.parents_bs + j];
         const int64_t x = a.tokens[b * a.nodes + j];
         bool child = j > 0 && parent >= 0 && parent < j;
         if (child && (x < 0 || x >= a.vocab)) {   // no token: never accepted, rejects nothing
@@ -103,13 +196,18 @@ __global__ void __launch_bounds__(kVThreads) verify_tree_kernel(VerifyArgs a) {
     if (tid == 0) {
         s.rejections = 0;
         s.node = 0;
+        s.c = 0.0;
+        s.t = 1.0;
         s.child = 1;
         s.found = -1;
+        s.summed = -1;
     }
+    const double sample_u = (double)a.sample_u[b];
     int accepted = 1, meeting = 0;
-    const int lo = (int)rank * a.per, hi = min(a.vocab, lo + a.per);
-    const int span = a.per / kVWarps;                       // a warp's part of the slice
-    const int wlo = min(hi, lo + warp * span), whi = min(hi, wlo + span);
+    // this warp's values [lo, end), chunk c at lo + c * chunk
+    const int span = kVChunks * a.chunk;
+    const int slice0 = (int)min((int64_t)a.vocab, (int64_t)rank * warps * span);
+    const int lo = (int)min((int64_t)a.vocab, (int64_t)slice0 + (int64_t)warp * span);
     for (;;) {
         __syncthreads();
         if (tid == 0) {
@@ -118,12 +216,18 @@ __global__ void __launch_bounds__(kVThreads) verify_tree_kernel(VerifyArgs a) {
             int j = s.child;
             for (; j < a.nodes; ++j) {
                 if (s.parent[j] != s.node) continue;
-                const double r = rest_at(s, draft != nullptr, s.token[j], s.p_at[j], s.q_at[j]);
+                const double r = rest_at(s, draft != nullptr, j);
                 if ((double)s.u[j] * (double)s.q_at[j] < r) {
                     s.node = j;
                     s.rejections = 0;
+                    s.c = 0.0;
+                    s.t = 1.0;
                     if (rank == 0) a.path[b * a.nodes + accepted] = j;
                     ++accepted;
+                } else if (!draft && s.summed == s.node) {
+                    double sum = 0.0;
+                    for (int c = 0; c < (int)ranks; ++c) sum += s.sum[(meeting & 1) ^ 1][c];
+                    take_out(s, j, sum);
                 } else {
                     s.found = j;
                     break;
@@ -135,39 +239,108 @@ __global__ void __launch_bounds__(kVThreads) verify_tree_kernel(VerifyArgs a) {
         const int node = s.node, rejected = s.found;
         const float* p = target + node * (int64_t)a.vocab;
         const float* q = draft ? draft + node * (int64_t)a.vocab : nullptr;
-        const int x = rejected >= 0 ? s.token[rejected] : -1;
-        // the sum of this slice: of (r - q)+ after a rejection, of r at the end
-        double sum = 0.0;
-        for (int i = wlo + lane; i < whi; i += 32) {
-            const float qi = q ? q[i] : 0.0f;
-            double r = rest_at(s, q != nullptr, i, p[i], qi);
-            if (rejected >= 0) r = q ? fmax(r - (double)qi, 0.0) : i == x ? 0.0 : r;
-            sum += r;
+        const bool known = rejected < 0 && s.summed == node;
+        // what is summed: (p - c q)+, p where c is 0
+        const double c_now = !q ? 0.0 : rejected >= 0 ? s.c + s.t : s.c;
+        auto values = [&](const float4& pi, const float4& qi, double (&r)[4]) {
+            const float pe[4] = {pi.x, pi.y, pi.z, pi.w}, qe[4] = {qi.x, qi.y, qi.z, qi.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = c_now == 0.0 ? (double)pe[e] : fmax((double)pe[e] - c_now * (double)qe[e], 0.0);
+        };
+        double sum[kVChunks];
+#pragma unroll
+        for (int c = 0; c < kVChunks; ++c) sum[c] = 0.0;
+        if (lo < a.vocab && !known) {
+            TwoPart part[kVChunks];
+#pragma unroll
+            for (int c = 0; c < kVChunks; ++c) part[c] = {0, 0};
+            for (int i0 = 4 * lane; i0 < a.chunk; i0 += 128) {
+                float4 pv[kVChunks], qv[kVChunks];
+#pragma unroll
+                for (int c = 0; c < kVChunks; ++c) {
+                    const int i = (int)min((int64_t)a.vocab, (int64_t)lo + (int64_t)c * a.chunk + i0);
+                    pv[c] = four(p, i, a.vocab, a.wide);
+                    qv[c] = c_now != 0.0 ? four(q, i, a.vocab, a.wide) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                if (c_now == 0.0) {
+#pragma unroll
+                    for (int c = 0; c < kVChunks; ++c) {
+                        part[c].add(pair(pv[c].x, pv[c].y));
+                        part[c].add(pair(pv[c].z, pv[c].w));
+                    }
+                } else if (c_now == 1.0) {         // the first rejection
+#pragma unroll
+                    for (int c = 0; c < kVChunks; ++c) {
+                        part[c].add_rest(pv[c].x, pv[c].y, qv[c].x, qv[c].y);
+                        part[c].add_rest(pv[c].z, pv[c].w, qv[c].z, qv[c].w);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kVChunks; ++c) {
+                        double r[4];
+                        values(pv[c], qv[c], r);
+                        sum[c] += (r[0] + r[1]) + (r[2] + r[3]);
+                    }
+                }
+            }
+            if (c_now == 0.0 || c_now == 1.0) {
+#pragma unroll
+                for (int c = 0; c < kVChunks; ++c) sum[c] = part[c].sum();
+            }
         }
-        sum = warp_sum_f64(sum);
-        if (lane == 0) s.warp_sum[warp] = sum;
-        __syncthreads();
-        if (tid < (int)ranks) {
-            double t = 0.0;
-            for (int w = 0; w < kVWarps; ++w) t += s.warp_sum[w];
-            const uint32_t at = mapa_shared(smem_u32(&s.sum[meeting & 1][rank]), tid);
-            asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(t) : "memory");
+        if (!known) {
+            const double all = warp_sums_f64(sum);
+            if ((lane & 3) == 0) s.chunk_sum[warp][lane >> 2] = all;
+            __syncthreads();
+            if (warp == 0) {
+                // the slice's sum, to every CTA of the cluster
+                double t = 0.0;
+                for (int c = lane; c < warps * kVChunks; c += 32) t += s.chunk_sum[c / kVChunks][c % kVChunks];
+                t = warp_sum_f64(t);
+                if (lane < (int)ranks) {
+                    const uint32_t at = mapa_shared(smem_u32(&s.sum[meeting & 1][rank]), lane);
+                    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(t) : "memory");
+                }
+            }
+            if (ranks > 1)
+                cluster_sync();
+            else
+                __syncthreads();
+            ++meeting;
         }
-        cluster_sync();
-        const double* sums = s.sum[meeting & 1];
-        ++meeting;
-        double total = 0.0;
-        for (int c = 0; c < (int)ranks; ++c) total += sums[c];
+        double* sums = s.sum[(meeting & 1) ^ 1];
         if (rejected >= 0) {
-            if (tid == 0 && total > 0.0) {
-                s.scale[s.rejections] = 1.0 / total;
-                s.gone[s.rejections] = x;
-                ++s.rejections;
+            if (tid == 0) {
+                double total = 0.0;
+                for (int c = 0; c < (int)ranks; ++c) total += sums[c];
+                s.summed = node;
+                if (!q) {
+                    take_out(s, rejected, total);
+                } else if (total > 0.0) {
+                    s.c += s.t;
+                    s.t = total;
+                    ++s.rejections;
+                } else {
+                    s.summed = -1;
+                }
             }
             continue;
         }
-        // the next token: the slice, then the warp's part, then the value in which the running sum passes u * total
-        const double want = (double)a.sample_u[b] * total;
+        // the next token: the slice, then the chunk, then the value in which the running sum passes u * total
+        if (!q && s.rejections > 0) {
+            // without the tokens taken out
+            __syncthreads();
+            if (tid == 0)
+                for (int k = 0; k < s.rejections; ++k) {
+                    const int64_t c = s.gone[k] / a.chunk, of = (int64_t)warps * kVChunks;
+                    sums[c / of] -= s.gone_p[k];
+                    if (c / of == rank) s.chunk_sum[c % of / kVChunks][c % kVChunks] -= s.gone_p[k];
+                }
+            __syncthreads();
+        }
+        double total = 0.0;
+        for (int c = 0; c < (int)ranks; ++c) total += sums[c];
+        const double want = sample_u * total;
         double before = 0.0;
         int slice = -1, last = (int)ranks - 1;
         for (int c = 0; c < (int)ranks; ++c) {
@@ -178,30 +351,49 @@ __global__ void __launch_bounds__(kVThreads) verify_tree_kernel(VerifyArgs a) {
         const bool past = slice < 0;                        // u * total at or past the total's rounding: the last value
         if (past) slice = last;
         if (slice == (int)rank && warp == 0) {
-            int part = -1, end = kVWarps - 1;
+            int part = -1, end = warps * kVChunks - 1;
             double base = before;
-            for (int w = 0; w < kVWarps; ++w) {
-                if (s.warp_sum[w] > 0.0) end = w;
-                if (!past && part < 0 && base + s.warp_sum[w] > want) part = w;
-                if (!past && part < 0) base += s.warp_sum[w];
+            for (int c = 0; c < warps * kVChunks && part < 0; ++c) {
+                const double t = s.chunk_sum[c / kVChunks][c % kVChunks];
+                if (t > 0.0) end = c;
+                if (!past && base + t > want) part = c;
+                if (part < 0) base += t;
             }
             const bool over = part < 0;
             if (over) part = end;
-            const int plo = min(hi, lo + part * span), phi = min(hi, plo + span);
+            const int plo = (int)min((int64_t)a.vocab, (int64_t)slice0 + (int64_t)part * a.chunk);
+            const int phi = (int)min((int64_t)a.vocab, (int64_t)plo + a.chunk);
             int token = -1, top = -1;                       // the answer; the last value above 0
-            for (int i0 = plo; i0 < phi && token < 0; i0 += 32) {
-                const int i = i0 + lane;
-                const double r = i < phi ? rest_at(s, q != nullptr, i, p[i], q ? q[i] : 0.0f) : 0.0;
-                double run = r;
+            for (int i0 = plo; i0 < phi && token < 0; i0 += 128) {
+                const int i = i0 + 4 * lane;
+                const float4 pv = four(p, min(i, phi), phi, a.wide);
+                const float4 qv = c_now != 0.0 ? four(q, min(i, phi), phi, a.wide) : make_float4(0.f, 0.f, 0.f, 0.f);
+                double r[4], run = 0.0;
+                values(pv, qv, r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (!q && is_gone(s, i + e)) r[e] = 0.0;
+                    run += r[e];
+                }
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const double v = __shfl_up_sync(0xffffffffu, run, o);
                     if (lane >= o) run += v;
                 }
-                const unsigned hit = __ballot_sync(0xffffffffu, !over && i < phi && base + run > want);
-                const unsigned some = __ballot_sync(0xffffffffu, r > 0.0);
-                if (hit) token = i0 + __ffs(hit) - 1;
-                if (some) top = i0 + 31 - __clz(some);
+                double at = __shfl_up_sync(0xffffffffu, run, 1);
+                at = base + (lane > 0 ? at : 0.0);
+                int hit = -1, some = -1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    at += r[e];
+                    if (i + e < phi) {
+                        if (hit < 0 && !over && at > want) hit = i + e;
+                        if (r[e] > 0.0) some = i + e;
+                    }
+                }
+                const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), somes = __ballot_sync(0xffffffffu, some >= 0);
+                if (hits) token = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
+                if (somes) top = __shfl_sync(0xffffffffu, some, 31 - __clz(somes));
                 base += __shfl_sync(0xffffffffu, run, 31);
             }
             if (lane == 0) a.next[b] = token >= 0 ? token : top >= 0 ? top : a.vocab - 1;
@@ -210,7 +402,7 @@ __global__ void __launch_bounds__(kVThreads) verify_tree_kernel(VerifyArgs a) {
     }
     if (rank == 0 && tid == 0) a.count[b] = accepted;
     // a CTA's shared memory takes the others' sums: none leaves before all have written
-    cluster_sync();
+    if (ranks > 1) cluster_sync();
 }
 
 }  // namespace
@@ -246,14 +438,17 @@ extern "C" int kz_verify_tree_f32(const int64_t* tokens, const int32_t* parents,
     a.nodes = (int)nodes;
     a.vocab = (int)vocab;
     a.status = device_status_ptr();
-    // a cluster for each sequence: 8 CTAs once a slice has 4 values a thread, fewer for small vocabularies
+    // a cluster for each sequence: the CTAs it takes to have 128 values a warp's chunk, 8 at most; a small
+    // vocabulary is one CTA of four warps
+    const int threads = vocab <= 4 * kVChunks * 128 ? 128 : kVThreads, warps = threads / 32;
     int ranks = 1;
-    while (ranks < kVMaxCluster && vocab > (int64_t)ranks * kVThreads * 4) ranks *= 2;
-    const int unit = 32 * kVWarps;
-    a.per = (int)((vocab + (int64_t)ranks * unit - 1) / ((int64_t)ranks * unit)) * unit;
+    while (ranks < kVMaxCluster && vocab > (int64_t)ranks * warps * kVChunks * 128) ranks *= 2;
+    const int64_t chunks = (int64_t)ranks * warps * kVChunks;
+    a.chunk = (int)((vocab + chunks * 128 - 1) / (chunks * 128)) * 128;
+    a.wide = vocab % 4 == 0 && ((reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft)) & 15u) == 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(batch * ranks));
-    cfg.blockDim = dim3(kVThreads);
+    cfg.blockDim = dim3(threads);
     cfg.stream = reinterpret_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeClusterDimension;
