@@ -25,12 +25,11 @@ number or position that a cache does not have is left out and recorded in the
 device status word (quantize.device_status), as NaN/Inf in a written row is.
 """
 import ctypes
-import math
 
 import torch
 
 from . import _lib
-from .tensor import Tensor, _as_device, ptr, require_cuda, stream_handle
+from .tensor import Tensor, _as_device, ptr, require_cuda
 
 
 def _raw(t, what):
@@ -43,16 +42,9 @@ def _raw(t, what):
     return x if x.dtype is torch.float32 else x.float()
 
 
-def _rows(x, what, width):
-    """(x, batch stride, row stride) of a [batch, tokens, width] tensor whose
-    rows a kernel can read in 16-byte pieces; any other is copied first."""
-    bs, rs, fs = x.stride()
-    if (x.data_ptr() & 15) or ((bs | rs) & 3) or fs != 1 or bs < 0 or (rs < width and x.shape[1] > 1):
-        x = x.contiguous()
-        if x.data_ptr() & 15:
-            x = x.clone()
-        bs, rs, _ = x.stride()
-    return x, bs, rs
+def _like(x):
+    """A new contiguous tensor like x (the cheapest allocation torch has)."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _ints(t, what, shape, index, dtype=torch.int32):
@@ -73,13 +65,14 @@ def _parents(parents, batch, nodes, index):
     return _ints(parents, "parents", (batch, nodes), index), nodes
 
 
-def _on(device, name, *args):
-    """Calls libkz with `device` current, on torch's current stream there."""
-    if torch.cuda.current_device() == device.index:
-        _lib.call(name, *args, stream_handle(device))
+def _on(index, name, *args):
+    """Calls libkz with GPU `index` current, on torch's current stream there."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        _lib.call(name, *args, stream)
     else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, stream_handle(device))
+        with torch.cuda.device(index):
+            _lib.call(name, *args, stream)
 
 
 class QCache:
@@ -145,13 +138,23 @@ class QCache:
                 None if counts is None else _ints(counts, "counts", (batch,), self._at))
 
     def _input(self, t, what, heads, batch):
+        """(x, its address, batch stride, row stride) of [batch, tokens, heads *
+        head_dim] rows that a kernel can read in 16-byte pieces; others are copied."""
         x = _raw(t, what)
         width = heads * self.head_dim
         if x.dim() != 3 or x.shape[0] != batch or x.shape[2] != width:
             raise ValueError(f"{what} must be [{batch}, tokens, {width}], not {list(x.shape)}")
         if x.get_device() != self._at:
             raise ValueError(f"{what} is on {x.device}, the cache on {self.device}")
-        return _rows(x, what, width)
+        bs, rs, fs = x.stride()
+        at = x.data_ptr()
+        if (at | bs << 2 | rs << 2) & 15 or fs != 1 or bs < 0 or (rs < width and x.shape[1] > 1):
+            x = x.contiguous()
+            if x.data_ptr() & 15:
+                x = x.clone()
+            bs, rs, _ = x.stride()
+            at = x.data_ptr()
+        return x, at, bs, rs
 
     def write(self, k, v, table, lengths, counts=None, values=False):
         """Quantizes new tokens' k and v [batch, tokens, kv_heads * head_dim]
@@ -159,15 +162,14 @@ class QCache:
         lengths + 0, 1, ...  With ``values``, returns what the codes stand for,
         two Tensors like k and v (0 in padding rows): the K/V a later pass sees."""
         batch, cols, table, lengths, counts = self._sequences(table, lengths, counts)
-        k, kb, kr = self._input(k, "k", self.kv_heads, batch)
-        v, vb, vr = self._input(v, "v", self.kv_heads, batch)
+        k, k_at, kb, kr = self._input(k, "k", self.kv_heads, batch)
+        v, v_at, vb, vr = self._input(v, "v", self.kv_heads, batch)
         if v.shape != k.shape:
             raise ValueError(f"k {list(k.shape)} and v {list(v.shape)} do not match")
-        ko = vo = None
         if values:
-            ko, vo = (torch.empty(k.shape, dtype=torch.float32, device=k.device) for _ in range(2))
-        _on(self.device, "kz_cache_write_f32", self._ref, ptr(k), ptr(v), batch, k.shape[1], kb, kr, vb, vr, ptr(table),
-            cols, ptr(lengths), ptr(counts), ptr(ko), ptr(vo))
+            ko, vo = _like(k), _like(k)
+        _on(self._at, "kz_cache_write_f32", self._ref, k_at, v_at, batch, k.shape[1], kb, kr, vb, vr, table.data_ptr(),
+            cols, lengths.data_ptr(), ptr(counts), ko.data_ptr() if values else None, vo.data_ptr() if values else None)
         return (Tensor(ko), Tensor(vo)) if values else None
 
     def read(self, table, lengths, most):
@@ -178,8 +180,10 @@ class QCache:
         if most < 0:
             raise ValueError(f"read: most must not be negative (got {most})")
         shape = (batch, int(most), self.kv_heads * self.head_dim)
-        k, v = (torch.empty(shape, dtype=torch.float32, device=self.device) for _ in range(2))
-        _on(self.device, "kz_cache_read_f32", self._ref, ptr(table), cols, ptr(lengths), batch, shape[1], ptr(k), ptr(v))
+        k = self.k_scale.new_empty(shape)
+        v = _like(k)
+        _on(self._at, "kz_cache_read_f32", self._ref, table.data_ptr(), cols, lengths.data_ptr(), batch, shape[1],
+            k.data_ptr(), v.data_ptr())
         return Tensor(k), Tensor(v)
 
     def attention(self, q, heads, table, lengths, counts=None, parents=None, scale=None):
@@ -192,22 +196,22 @@ class QCache:
         batch, cols, table, lengths, counts = self._sequences(table, lengths, counts)
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"attention: heads ({heads}) must be a multiple of kv_heads ({self.kv_heads})")
-        q, qb, qr = self._input(q, "q", heads, batch)
+        q, q_at, qb, qr = self._input(q, "q", heads, batch)
         tokens, pb = q.shape[1], 0
         if parents is not None:
             if tokens > _lib.KZ_TREE_MAX_NODES:
                 raise ValueError(f"attention: a tree has at most {_lib.KZ_TREE_MAX_NODES} nodes (got {tokens})")
             parents, pb = _parents(parents, batch, tokens, self._at)
-        out = torch.empty((batch, tokens, heads * self.head_dim), dtype=torch.float32, device=self.device)
+        out = _like(q)
         need = self._scratch.get((tokens, heads, cols))
         if need is None:
             with torch.cuda.device(self.device):
                 need = _lib.load().kz_cache_attention_workspace_bytes(self._ref, tokens, heads, cols)
             self._scratch[tokens, heads, cols] = need
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        _on(self.device, "kz_cache_attention_f32", self._ref, ptr(q), batch, tokens, heads, qb, qr, ptr(table), cols,
-            ptr(lengths), ptr(counts), ptr(parents), pb, 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
-            ptr(out), ptr(work), need)
+        work = self.k_codes.new_empty(need) if need else None
+        _on(self._at, "kz_cache_attention_f32", self._ref, q_at, batch, tokens, heads, qb, qr, table.data_ptr(), cols,
+            lengths.data_ptr(), ptr(counts), ptr(parents), pb, self.head_dim ** -0.5 if scale is None else scale,
+            out.data_ptr(), ptr(work), need)
         return Tensor(out)
 
     def keep(self, table, lengths, path, count):
@@ -220,8 +224,8 @@ class QCache:
         path = _ints(path, "path", (batch, path.shape[1]), self._at)
         if count is None:
             raise ValueError("count must be an int32 tensor [batch]")
-        _on(self.device, "kz_cache_keep", self._ref, ptr(table), cols, ptr(lengths), ptr(path), ptr(count), batch,
-            path.shape[1])
+        _on(self._at, "kz_cache_keep", self._ref, table.data_ptr(), cols, lengths.data_ptr(), path.data_ptr(),
+            count.data_ptr(), batch, path.shape[1])
 
 
 class PagePool:
@@ -296,11 +300,10 @@ def verify_tree(tokens, parents, target, draft, accept_u, sample_u):
     accept_u, sample_u = floats(accept_u, "accept_u", (batch, nodes)), floats(sample_u, "sample_u", (batch,))
     tokens = _ints(tokens, "tokens", (batch, nodes), at, torch.int64)
     parents, pb = _parents(parents, batch, nodes, at)
-    path = torch.empty((batch, nodes), dtype=torch.int32, device=dev)
-    count = torch.empty(batch, dtype=torch.int32, device=dev)
-    token = torch.empty(batch, dtype=torch.int64, device=dev)
-    _on(dev, "kz_verify_tree_f32", ptr(tokens), ptr(parents), pb, ptr(target), ptr(draft), ptr(accept_u), ptr(sample_u),
-        batch, nodes, vocab, ptr(path), ptr(count), ptr(token))
+    path = _like(parents) if pb else parents.new_empty((batch, nodes))
+    count, token = parents.new_empty(batch), tokens.new_empty(batch)
+    _on(at, "kz_verify_tree_f32", tokens.data_ptr(), parents.data_ptr(), pb, target.data_ptr(), ptr(draft),
+        accept_u.data_ptr(), sample_u.data_ptr(), batch, nodes, vocab, path.data_ptr(), count.data_ptr(), token.data_ptr())
     return path, count, token
 
 

@@ -53,7 +53,7 @@ struct Shape {
     static constexpr int CODES = kKT * D, STAGE = 2 * CODES + 2 * kKT * 4;
     static constexpr int PITCH = D + 4;                     // joined rows: float2 stores without conflicts
     static constexpr int QBYTES = RT * D * 4;               // both halves of q, as mma operands
-    static constexpr int UBYTES = KG > 1 && RT * PITCH * 4 > QBYTES ? RT * PITCH * 4 : QBYTES;
+    static constexpr int UBYTES = RT * PITCH * 4 > QBYTES ? RT * PITCH * 4 : QBYTES;
     static constexpr int SMEM = STAGES * STAGE + UBYTES + 1024;
     static constexpr int SLOT = RT * (D + 2);               // floats of a part
 };
@@ -461,56 +461,40 @@ __global__ void __launch_bounds__(kCaThreads, 2)
                 const int R = g.rt * S::RT + r;
                 return out + ((int64_t)(R / a.group) * a.heads + R % a.group) * D;
             };
-            if constexpr (S::KG == 1) {
+            for (int turn = 0; turn < S::KG; ++turn) {
+                if (turn == kg) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int r = (rg * NT + n) * 8 + 2 * tq + j;
-                        const float f = direct ? (l[n][j] == 0.0f ? 0.0f : 1.0f / l[n][j]) : 1.0f;
-                        if (r < rows) {
-                            float* dst = direct ? out_row(r) : slot + r * D;
+                        for (int j = 0; j < 2; ++j) {
+                            const int r = (rg * NT + n) * 8 + 2 * tq + j;
+                            float M = -INFINITY;
 #pragma unroll
-                            for (int i = 0; i < D / 16; ++i)
-                                *reinterpret_cast<float2*>(dst + 16 * i + 2 * gq) = make_float2(o[n][i][j] * f, o[n][i][j + 2] * f);
-                        }
-                    }
-            } else {
-                for (int turn = 0; turn < S::KG; ++turn) {
-                    if (turn == kg) {
+                            for (int k = 0; k < S::KG; ++k) M = fmaxf(M, s_m[k][r]);
+                            const float f = shrink(m[n][j], M);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const int r = (rg * NT + n) * 8 + 2 * tq + j;
-                                float M = -INFINITY;
-#pragma unroll
-                                for (int k = 0; k < S::KG; ++k) M = fmaxf(M, s_m[k][r]);
-                                const float f = shrink(m[n][j], M);
-#pragma unroll
-                                for (int i = 0; i < D / 16; ++i) {
-                                    float2* p = reinterpret_cast<float2*>(joined + r * S::PITCH + 16 * i + 2 * gq);
-                                    const float2 v = turn ? *p : make_float2(0.f, 0.f);
-                                    *p = make_float2(fmaf(o[n][i][j], f, v.x), fmaf(o[n][i][j + 2], f, v.y));
-                                }
+                            for (int i = 0; i < D / 16; ++i) {
+                                float2* p = reinterpret_cast<float2*>(joined + r * S::PITCH + 16 * i + 2 * gq);
+                                const float2 v = turn ? *p : make_float2(0.f, 0.f);
+                                *p = make_float2(fmaf(o[n][i][j], f, v.x), fmaf(o[n][i][j + 2], f, v.y));
                             }
-                    }
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                        }
                 }
-                for (int i = tid; i < rows * (D / 4); i += kConsumers) {
-                    const int r = i / (D / 4), c = i % (D / 4);
-                    float4 v = *reinterpret_cast<const float4*>(joined + r * S::PITCH + 4 * c);
-                    if (direct) {
-                        float M = -INFINITY, L = 0.0f;
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
+            for (int i = tid; i < rows * (D / 4); i += kConsumers) {
+                const int r = i / (D / 4), c = i % (D / 4);
+                float4 v = *reinterpret_cast<const float4*>(joined + r * S::PITCH + 4 * c);
+                if (direct) {
+                    float M = -INFINITY, L = 0.0f;
 #pragma unroll
-                        for (int k = 0; k < S::KG; ++k) M = fmaxf(M, s_m[k][r]);
+                    for (int k = 0; k < S::KG; ++k) M = fmaxf(M, s_m[k][r]);
 #pragma unroll
-                        for (int k = 0; k < S::KG; ++k) L += s_l[k][r] * shrink(s_m[k][r], M);
-                        const float f = L == 0.0f ? 0.0f : 1.0f / L;
-                        v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-                    }
-                    *reinterpret_cast<float4*>((direct ? out_row(r) : slot + r * D) + 4 * c) = v;
+                    for (int k = 0; k < S::KG; ++k) L += s_l[k][r] * shrink(s_m[k][r], M);
+                    const float f = L == 0.0f ? 0.0f : 1.0f / L;
+                    v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
                 }
+                *reinterpret_cast<float4*>((direct ? out_row(r) : slot + r * D) + 4 * c) = v;
             }
             if (!direct && tid < S::RT) {
                 float M = -INFINITY, L = 0.0f;
@@ -624,15 +608,18 @@ __global__ void __launch_bounds__(kConsumers) cache_attention_join_kernel(const 
 
 // ---------------------------------------------------------------- launches
 
-// Rows of a tile: the smallest of 8, 16, 32 and 64 that holds a key head's rows.
-int tile_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// Rows of a tile: the smallest of 8, 16 and 32 that holds a key head's rows.
+int tile_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
 
 // Whether every (sequence, head, row tile) is one CTA's whole work: the table
 // holds no more tiles than a CTA's range has at least.
 bool whole_ranges(int64_t cols, int64_t page) { return cols * page <= (int64_t)kMinTiles * kKT; }
 
-// Whether the rows of a key head are many enough for the tcgen05 kernel.
-bool many_rows(int64_t rows) { return rows > 16; }
+// Whether the rows of a key head are many enough for the tcgen05 kernel, whose
+// time does not depend on them up to 128: at 32 rows (batch 16, 8 key heads of
+// 128, contexts of 1500 and 6000) it takes 45 and 87 us against 37 and 87 here,
+// at 64 rows 51 and 98 against 58 and 150 with tiles of 64 rows.
+bool many_rows(int64_t rows) { return rows > 32; }
 
 int64_t parts_floats(int64_t rows, int64_t d) {
     const int64_t ctas = (many_rows(rows) ? 1 : 2) * (int64_t)sm_count();
@@ -680,8 +667,7 @@ int dispatch_cache_attention(const CacheAttArgs& a, cudaStream_t s) {
     const int64_t row_tiles = (rows + rt - 1) / rt;
     if (rt == 8) return launch_cache_attention<D, 1, 1>(a, row_tiles, s);
     if (rt == 16) return launch_cache_attention<D, 2, 1>(a, row_tiles, s);
-    if (rt == 32) return launch_cache_attention<D, 2, 2>(a, row_tiles, s);
-    return launch_cache_attention<D, 2, 4>(a, row_tiles, s);
+    return launch_cache_attention<D, 2, 2>(a, row_tiles, s);
 }
 
 }  // namespace

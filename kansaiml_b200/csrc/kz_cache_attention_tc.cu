@@ -11,7 +11,7 @@
 // N-major for the second.  Warps 0-7: softmax, two threads a row (64 keys of
 // each tile, and half of the row's sums in registers, to which each tile's O is
 // added); 8-11 convert the next tiles; 12 issues the MMAs, 13 loads the pages
-// (bulk copies).  The MMAs of tile t + 1's scores run while tile t's softmax
+// (bulk copies), 14 and 15 zero the padding's rows.  The MMAs of tile t + 1's scores run while tile t's softmax
 // does, so the tensor cores wait only where a row tile ends.
 //
 // Tensor memory (512 columns): Q halves 0..d-1, S / P of even tiles 128..255,
@@ -61,14 +61,6 @@ __device__ __forceinline__ uint64_t smem_desc_n_sw128(uint32_t addr, uint32_t ne
     d |= static_cast<uint64_t>(1u) << 46;
     d |= static_cast<uint64_t>(2u) << 61;
     return d;
-}
-__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
@@ -127,7 +119,7 @@ __device__ __forceinline__ bool elect_one() {
 
 // The registers of a warpgroup: each of the four starts with what the launch
 // gives it, the two of the softmax take from the others'.
-constexpr int kRegsLaunch = 65536 / kTcThreads, kRegsSoftmax = 176, kRegsConvert = 104, kRegsIssue = 56;
+constexpr int kRegsLaunch = 65536 / kTcThreads, kRegsSoftmax = 192, kRegsConvert = 72, kRegsIssue = 56;
 static_assert(2 * kRegsSoftmax + kRegsConvert + kRegsIssue <= 4 * kRegsLaunch, "an increase would wait for ever");
 template <int N>
 __device__ __forceinline__ void registers_up() {
@@ -192,7 +184,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
         s_s_full[2], s_p_full[2], s_q_full, s_o_full, s_o_empty;
     __shared__ uint32_t s_tmem, s_bad[4];
     __shared__ float s_top[2][2][kTcRows], s_l[2][kTcRows];      // exchanged between a row's two threads
-    __shared__ uint32_t s_q_top[2][kTcRows];
     __shared__ uint32_t s_sees[kTcRows][kTreeWords];
     __shared__ int32_t s_parent[KZ_TREE_MAX_NODES];
     __shared__ int s_sum[4], s_part[128], s_start[2], s_units[2];
@@ -338,26 +329,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
                 for (int half = 0; half < 2; ++half)
 #pragma unroll
                     for (int i = 0; i < kKT / 16; ++i)
-                        tc_mma_f16_ts(tmem + kTmO, p + (i >> 1) * 32 + half * 16 + (i & 1) * 8, smem_desc_n_sw128(v + i * 2048, kKT * 128), id_o,
+                        tc_mma_f16_ts(tmem + kTmO, p + (i >> 1) * 32 + (1 - half) * 16 + (i & 1) * 8, smem_desc_n_sw128(v + i * 2048, kKT * 128), id_o,
                                       half | i);
                 tc_commit(smem_u32(&s_o_full));
                 tc_commit(smem_u32(s_v_empty) + 8 * odd);
             }
             __syncwarp();
         };
-        while (walk.next(a, g)) {
-            for (int t = g.t0; t < g.t1; ++t, ++it) {
-                if (t == g.t0) {
-                    // the rows change: q comes after the last tile's softmax, so its output goes first
-                    if (pending >= 0) {
-                        output(pending);
-                        wait(s_o_full, pending);
+        bool more = true;
+        int t = 0;
+        g.t0 = g.t1 = 0;
+        while (more || pending >= 0) {
+            // the next tile, if there is one; where the rows change, q comes after the last tile's
+            // softmax, so its output goes first
+            bool first = t >= g.t1;
+            while (more && t >= g.t1) {
+                more = walk.next(a, g);
+                t = g.t0;
+            }
+            first = first || !more;
+#pragma unroll 1
+            for (int step = 0; step < 3; ++step) {
+                if (step == (first ? 0 : 2) && pending >= 0) {
+                    output(pending);
+                    if (first) wait(s_o_full, pending);
+                    if (!more) {                         // every commit has arrived before this CTA can end
+                        wait(s_k_empty[pending & 1], pending >> 1);
+                        wait(s_v_empty[pending & 1], pending >> 1);
                     }
                     pending = -1;
-                    wait(s_q_full, segment++);
-                } else if (it >= 2) {
-                    wait(s_o_full, it - 2);              // P(it - 2), in S's place, is used
                 }
+                if (step != 1 || !more) continue;
+                if (first)
+                    wait(s_q_full, segment++);
+                else if (it >= 2)
+                    wait(s_o_full, it - 2);              // P(it - 2), in S's place, is used
                 wait(s_k_full[it & 1], it >> 1);
                 tc_fence_after();
                 const uint32_t odd = __shfl_sync(0xffffffffu, it & 1, 0);
@@ -367,20 +373,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
                     for (int half = 0; half < 2; ++half)
 #pragma unroll
                         for (int i = 0; i < D / 16; ++i)
-                            tc_mma_f16_ts(tmem + kTmS + odd * 128, tmem + half * (D / 2) + i * 8,
+                            tc_mma_f16_ts(tmem + kTmS + odd * 128, tmem + (1 - half) * (D / 2) + i * 8,
                                           smem_desc_k_sw128(k + (i >> 2) * (kKT * 128) + (i & 3) * 32), id_s, half | i);
                     tc_commit(smem_u32(s_s_full) + 8 * odd);
                     tc_commit(smem_u32(s_k_empty) + 8 * odd);
                 }
                 __syncwarp();
-                if (pending >= 0) output(pending);
-                pending = it;
             }
-        }
-        if (pending >= 0) {
-            output(pending);
-            wait(s_k_empty[pending & 1], pending >> 1);      // every commit has arrived before this CTA can end
-            wait(s_v_empty[pending & 1], pending >> 1);
+            if (more) {
+                pending = it++;
+                ++t;
+            }
         }
     } else if (warp < 8) {
         // ---- softmax: threads r and r + 128 have row r of the tile, each 64 of its
@@ -388,13 +391,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
         registers_up<kRegsSoftmax>();
         const int row = tid & 127, half = tid >> 7;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        // the row's two threads are in warps w and w + 4: they exchange by a barrier of those two
+        auto meet_pair = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };
         auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(kSoftmax) : "memory"); };
-        for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {   // rows past a sequence's count are 0
-            const int n = a.counts ? max(0, min(a.counts[b], a.tokens)) : a.tokens;
-            const int64_t width = (int64_t)a.heads * D;
-            float4* o = reinterpret_cast<float4*>(a.out + ((int64_t)b * a.tokens + n) * width);
-            for (int64_t i = tid; i < (a.tokens - n) * (width / 4); i += kSoftmax) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
         int it = 0;
         bool first_segment = true;
         while (walk.next(a, g)) {
@@ -406,29 +405,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
                 // q times scale log2(e), its largest value brought into [2^13, 2^14), as two halves
                 const float* src = a.q + g.b * a.q_bs + (int64_t)token * a.q_rs +
                                    ((int64_t)g.h * a.group + R % a.group) * D + half * (D / 2);
-                const float f = a.scale * 1.4426950408889634f;
-                float x[D / 2];
-                uint32_t top = 0;
+                float4 x[D / 8];
+                float top = 0.0f;
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const float4 v = is_row ? *reinterpret_cast<const float4*>(src + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    x[4 * i] = v.x * f;
-                    x[4 * i + 1] = v.y * f;
-                    x[4 * i + 2] = v.z * f;
-                    x[4 * i + 3] = v.w * f;
-                }
-#pragma unroll
-                for (int i = 0; i < D / 2; ++i) {
-                    const uint32_t bits = __float_as_uint(x[i]) & 0x7FFFFFFFu;
-                    if (bits < 0x7F800000u) top = max(top, bits);
-                }
-                s_q_top[half][row] = top;
+                for (int i = 0; i < D / 8; ++i)
+                    x[i] = is_row ? *reinterpret_cast<const float4*>(src + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
                 if (a.parents)
                     for (int j = tid; j <= g.last_token; j += kSoftmax) s_parent[j] = a.parents[g.b * a.parents_bs + j];
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                    top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+                s_l[half][row] = top;
                 meet();
-                top = max(top, s_q_top[half ^ 1][row]);
-                const int ex = max((int)(top >> 23), 14);
-                const float up = pow2_field(267 - ex);
+                top = fmaxf(top, s_l[half ^ 1][row]);
+                const float f = a.scale * 1.4426950408889634f;
+                const int ex = min(max((int)(__float_as_uint(fabsf(top * f)) >> 23), 30), 254);
+                const float up = f * pow2_field(267 - ex);
                 unit = pow2_field(ex - 13);
                 // 16 values a step: 8 columns of each half
 #pragma unroll
@@ -436,7 +428,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
                     uint32_t hi[8], lo[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float u = x[16 * c + 2 * i] * up, w = x[16 * c + 2 * i + 1] * up;
+                        const float4 v = x[4 * c + i / 2];
+                        const float u = (i & 1 ? v.z : v.x) * up, w = (i & 1 ? v.w : v.y) * up;
                         hi[i] = half2_bits(leading(u), leading(w));
                         lo[i] = half2_bits(u - leading(u), w - leading(w));
                     }
@@ -460,26 +453,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
                 }
             }
             const uint64_t unit2 = pair(unit, unit);
-            float m = -INFINITY, l = 0.0f, corr = 0.0f;
+            float m = -INFINITY, l = 0.0f, corr = 0.0f, corr_next = 0.0f;
             float o[D / 2];
 #pragma unroll
             for (int i = 0; i < D / 2; ++i) o[i] = 0.0f;
-            // the output of tile t joins the row's sums, `corr` the softmax's rescaling since the tile before
-            auto join = [&](int t) {
-                wait(s_o_full, t);
-                tc_fence_after();
+            // a tile's output joins the row's sums, `corr` the softmax's rescaling since the tile before
+            auto join = [&] {
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t r[16];
-                    tmem_ld_32x32b_x16(tmem + lanes + kTmO + half * (D / 2) + 16 * c, r);
+                for (int c = 0; c < D / 32; c += 2) {
+                    uint32_t r[2][16];
+                    tmem_ld_32x32b_x16(tmem + lanes + kTmO + half * (D / 2) + 16 * c, r[0]);
+                    if (c + 1 < D / 32) tmem_ld_32x32b_x16(tmem + lanes + kTmO + half * (D / 2) + 16 * c + 16, r[1]);
                     tc_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[16 * c + i] = fmaf(o[16 * c + i], corr, __uint_as_float(r[i]));
+                    for (int i = 0; i < 32; ++i)
+                        if (16 * c + i < D / 2) o[16 * c + i] = fmaf(o[16 * c + i], corr, __uint_as_float(r[i >> 4][i & 15]));
                 }
-                tc_fence_before();
-                arrive(s_o_empty);
             };
-            for (int t = g.t0; t < g.t1; ++t, ++it) {
+            // a warp none of whose rows are rows keeps the others' pace and computes nothing
+            const bool idle = g.rt * kTcRows + (warp & 3) * 32 >= g.count * a.group;
+            // (one turn more than tiles: the last joins the last tile's output)
+#pragma unroll 1
+            for (int t = g.t0; t < g.t1 || t > g.t0; ++t, ++it) {
+                if (t == g.t1 || idle) {
+                    if (t < g.t1) {
+                        wait(s_s_full[it & 1], it >> 1);
+                        arrive(s_p_full[it & 1]);
+                    }
+                } else {
                 const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(factors + 3 * (it & 3) * kKT + 64 * half);
                 const ulonglong2 *vs = ks + kKT / 4, *lv = vs + kKT / 4;     // pairs of fp32 values
                 const uint32_t s_at = tmem + lanes + kTmS + (it & 1) * 128 + 64 * half;
@@ -512,104 +513,94 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
                     }
                     return s;
                 };
-                // A chunk's 32 scores times ks, and the largest of s + log2 vs; and, from these, its
-                // weights, their sum, and their halves times vs over the chunk's own columns of S (16
-                // of leading halves, 16 of the rest).
-                float top[4] = {m, m, m, m};
-                uint64_t sum[2] = {0, 0};
-                auto scores = [&](int c, auto with_mask, uint32_t sees, const uint32_t (&r)[32], uint64_t* z) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const ulonglong2 f = ks[8 * c + j], e = lv[8 * c + j];
-                        z[2 * j] = mul2(bits_pair(r[4 * j], r[4 * j + 1]), f.x);
-                        z[2 * j + 1] = mul2(bits_pair(r[4 * j + 2], r[4 * j + 3]), f.y);
-                        float x[4];
-                        unpair(fma2(z[2 * j], unit2, e.x), x[0], x[1]);
-                        unpair(fma2(z[2 * j + 1], unit2, e.y), x[2], x[3]);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if (decltype(with_mask)::value && !((sees >> (4 * j + k)) & 1u)) x[k] = -INFINITY;
-                            top[k] = fmaxf(top[k], x[k]);
-                        }
-                    }
-                };
-                auto weights = [&](int c, auto with_mask, uint32_t sees, uint64_t ref2, const uint64_t* z) {
-                    uint32_t hi[16], lo[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        float p0, p1;
-                        unpair(fma2(z[j], unit2, ref2), p0, p1);
-                        p0 = exp2_approx(p0);
-                        p1 = exp2_approx(p1);
-                        const bool s0 = !decltype(with_mask)::value || ((sees >> (2 * j)) & 1u);
-                        const bool s1 = !decltype(with_mask)::value || ((sees >> (2 * j + 1)) & 1u);
-                        if (!s0) p0 = 0.0f;
-                        if (!s1) p1 = 0.0f;
-                        const ulonglong2 f = vs[8 * c + (j >> 1)];
-                        const uint64_t p = pair(p0, p1);
-                        sum[j & 1] = add2(sum[j & 1], p);
-                        unpair(mul2(p, j & 1 ? f.y : f.x), p0, p1);
-                        if (!s0) p0 = 0.0f;              // whatever vs is there
-                        if (!s1) p1 = 0.0f;
-                        const float h0 = leading(p0), h1 = leading(p1);
-                        float l0, l1;
-                        unpair(sub2(pair(p0, p1), pair(h0, h1)), l0, l1);
-                        hi[j] = half2_bits(h0, h1);
-                        lo[j] = half2_bits(l0, l1);
-                    }
-                    tmem_st_32x32b_x16(s_at + 32 * c, hi);
-                    tmem_st_32x32b_x16(s_at + 32 * c + 16, lo);
-                };
-                float m_new = m;
-                auto maximum = [&] {               // over the row's two threads
-                    m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                    s_top[it & 1][half][row] = m_new;
-                    meet();
-                    m_new = fmaxf(m_new, s_top[it & 1][half ^ 1][row]);
-                    const float ref = m_new == -INFINITY ? 0.0f : kLift - m_new;
-                    return pair(ref, ref);
-                };
-                if (!masked) {
+                uint64_t z[32];                      // s * ks
+                {
                     uint32_t r[2][32];
                     tmem_ld_32x32b_x32(s_at, r[0]);
                     tmem_ld_32x32b_x32(s_at + 32, r[1]);
                     tc_wait_ld();
-                    uint64_t z[32];
-                    scores(0, std::false_type{}, 0, r[0], z);
-                    scores(1, std::false_type{}, 0, r[1], z + 16);
-                    const uint64_t ref2 = maximum();
-                    weights(0, std::false_type{}, 0, ref2, z);
-                    weights(1, std::false_type{}, 0, ref2, z + 16);
-                } else {
-                    uint32_t r[32];
-                    uint64_t z[16];
-#pragma unroll 1
-                    for (int c = 0; c < 2; ++c) {
-                        tmem_ld_32x32b_x32(s_at + 32 * c, r);
-                        tc_wait_ld();
-                        scores(c, std::true_type{}, seen(2 * half + c), r, z);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const ulonglong2 f = ks[j];
+                        const int c = j >> 3, i = (4 * j) & 31;
+                        z[2 * j] = mul2(bits_pair(r[c][i], r[c][i + 1]), f.x);
+                        z[2 * j + 1] = mul2(bits_pair(r[c][i + 2], r[c][i + 3]), f.y);
                     }
-                    const uint64_t ref2 = maximum();
-#pragma unroll 1
+                }
+                if (masked) {
+#pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        tmem_ld_32x32b_x32(s_at + 32 * c, r);
-                        tc_wait_ld();
-                        scores(c, std::true_type{}, 0, r, z);
-                        weights(c, std::true_type{}, seen(2 * half + c), ref2, z);
+                        const uint32_t sees = seen(2 * half + c);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            float x0, x1;
+                            unpair(z[16 * c + j], x0, x1);
+                            if (!((sees >> (2 * j)) & 1u)) x0 = -INFINITY;
+                            if (!((sees >> (2 * j + 1)) & 1u)) x1 = -INFINITY;
+                            z[16 * c + j] = pair(x0, x1);
+                        }
                     }
+                }
+                float top[4] = {m, m, m, m};         // the largest of s + log2 vs
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const ulonglong2 e = lv[j];
+                    float x[4];
+                    unpair(fma2(z[2 * j], unit2, e.x), x[0], x[1]);
+                    unpair(fma2(z[2 * j + 1], unit2, e.y), x[2], x[3]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], x[k]);
+                }
+                float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                s_top[it & 1][half][row] = m_new;
+                meet_pair();
+                m_new = fmaxf(m_new, s_top[it & 1][half ^ 1][row]);
+                const float ref = m_new == -INFINITY ? 0.0f : kLift - m_new;
+                const uint64_t ref2 = pair(ref, ref);
+                uint64_t sum[2] = {0, 0};
+                // the weights, and their halves times vs over each 32 keys' own columns of S (16 of
+                // leading halves, 16 of the rest)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        float p0, p1;
+                        unpair(fma2(z[8 * c + j], unit2, ref2), p0, p1);
+                        const uint64_t p = pair(exp2_approx(p0), exp2_approx(p1));
+                        const ulonglong2 f = vs[4 * c + (j >> 1)];
+                        sum[j & 1] = add2(sum[j & 1], p);
+                        const uint64_t w = mul2(p, j & 1 ? f.y : f.x);
+                        unpair(w, p0, p1);
+                        const float h0 = leading(p0), h1 = leading(p1);
+                        float l0, l1;
+                        unpair(sub2(w, pair(h0, h1)), l0, l1);
+                        hi[j] = half2_bits(h0, h1);
+                        lo[j] = half2_bits(l0, l1);
+                    }
+                    tmem_st_32x32b_x8(s_at + 32 * (c >> 1) + 8 * (c & 1), hi);
+                    tmem_st_32x32b_x8(s_at + 32 * (c >> 1) + 16 + 8 * (c & 1), lo);
                 }
                 const float corr_new = shrink(m, m_new);
                 m = m_new;
                 float s0, s1;
                 unpair(add2(sum[0], sum[1]), s0, s1);
                 l = fmaf(l, corr_new, s0 + s1);
-                if (t > g.t0) join(it - 1);
-                corr = corr_new;
                 tc_wait_st();
                 tc_fence_before();
                 arrive(s_p_full[it & 1]);
+                corr_next = corr_new;
+                }
+                if (t > g.t0) {
+                    wait(s_o_full, it - 1);
+                    tc_fence_after();
+                    if (!idle) join();
+                    tc_fence_before();
+                    arrive(s_o_empty);
+                }
+                corr = corr_next;
+                if (t == g.t1) break;
             }
-            if (g.t0 < g.t1) join(it - 1);
             s_l[half][row] = l;
             meet();
             l += s_l[half ^ 1][row];
@@ -643,20 +634,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
                 const float* raw = scales + 2 * (it & 3) * kKT;
                 float* made = factors + 3 * (it & 3) * kKT;
                 const bool out = t * kKT + t128 > g.len + g.last_token || ((s_bad[it & 3] >> (t128 >> a.c.shift)) & 1u);
+                // a vs that is not finite reaches whoever sees the key through its score
                 const float vs = out ? 0.0f : raw[kKT + t128];
-                wait(s_k_empty[it & 1], (it >> 1) + 1);
-                made[t128] = raw[t128];
-                made[kKT + t128] = vs;
-                made[2 * kKT + t128] = log2_vs(vs);
-                convert_tile<D>(codes + 2 * (it & 1) * T::CODES, k_tiles + (it & 1) * T::TILE, t128);
-                fence_proxy_async_smem();
-                arrive(s_k_full[it & 1]);
-                wait(s_v_empty[it & 1], (it >> 1) + 1);
-                convert_tile<D>(codes + (2 * (it & 1) + 1) * T::CODES, v_tiles + (it & 1) * T::TILE, t128);
-                fence_proxy_async_smem();
-                arrive(s_v_full[it & 1]);
+                const bool fine = fabsf(vs) < INFINITY;
+#pragma unroll 1
+                for (int kv = 0; kv < 2; ++kv) {
+                    wait(kv ? s_v_empty[it & 1] : s_k_empty[it & 1], (it >> 1) + 1);
+                    if (kv == 0) {
+                        made[t128] = fine ? raw[t128] : __uint_as_float(0x7FC00000u);
+                        made[kKT + t128] = fine ? vs : 0.0f;
+                        made[2 * kKT + t128] = log2_vs(fine ? vs : 0.0f);
+                    }
+                    convert_tile<D>(codes + (2 * (it & 1) + kv) * T::CODES, (kv ? v_tiles : k_tiles) + (it & 1) * T::TILE, t128);
+                    fence_proxy_async_smem();
+                    arrive(kv ? s_v_full[it & 1] : s_k_full[it & 1]);
+                }
                 arrive(s_code_empty[it & 1]);
             }
+        }
+    }
+    if (warp >= 14) {
+        // rows past a sequence's count are 0
+        for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+            const int n = a.counts ? max(0, min(a.counts[b], a.tokens)) : a.tokens;
+            const int64_t width = (int64_t)a.heads * D;
+            float4* o = reinterpret_cast<float4*>(a.out + ((int64_t)b * a.tokens + n) * width);
+            for (int64_t i = tid - 448; i < (a.tokens - n) * (width / 4); i += 64) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
     }
     // a wait that ran out (recorded): give what is in flight time to end before the memory goes
