@@ -286,13 +286,13 @@ __global__ void __launch_bounds__(kCaThreads, 2)
                     const uint32_t row_at = (kl + (lane & 15)) * D + (lane >> 4) * 16;
 
                     // ---- S^T: 32 keys x 8 NT rows
-                    float s[2][NT][4];
+                    float s[2][NT][4], s_lo[2][NT][4];           // the small halves' products have a sum of their own
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) s[mt][n][j] = 0.0f;
+                            for (int j = 0; j < 4; ++j) s[mt][n][j] = s_lo[mt][n][j] = 0.0f;
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
                         uint32_t ops[2][2][4];
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kCaThreads, 2)
 #pragma unroll
                                 for (int mt = 0; mt < 2; ++mt) mma_16816(s[mt][n], ops[mt][i], b.x, b.y);
 #pragma unroll
-                                for (int mt = 0; mt < 2; ++mt) mma_16816(s[mt][n], ops[mt][i], b.z, b.w);
+                                for (int mt = 0; mt < 2; ++mt) mma_16816(s_lo[mt][n], ops[mt][i], b.z, b.w);
                             }
                     }
 
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kCaThreads, 2)
                         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                z[mt][e] = s[mt][n][e] * ks[mt][e >> 1] * qs[n][e & 1];
+                                z[mt][e] = (s[mt][n][e] + s_lo[mt][n][e]) * ks[mt][e >> 1] * qs[n][e & 1];
                                 float x = z[mt][e] + lv[mt][e >> 1];
                                 if (!((seen >> (4 * mt + e)) & 1u)) z[mt][e] = x = -INFINITY;
                                 mx[e & 1] = fmaxf(mx[e & 1], x);
@@ -417,16 +417,17 @@ __global__ void __launch_bounds__(kCaThreads, 2)
 #pragma unroll
                                 for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.0f;
 #pragma unroll
-                        for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-                            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                                for (int n = 0; n < NT; ++n) mma_16816(acc[i][n], ops[mt][i], w_hi[mt][n][0], w_hi[mt][n][1]);
+                        for (int mt = 0; mt < 2; ++mt)             // the small halves first: their sum is truncated least
 #pragma unroll
                             for (int i = 0; i < 2; ++i)
 #pragma unroll
                                 for (int n = 0; n < NT; ++n) mma_16816(acc[i][n], ops[mt][i], w_lo[mt][n][0], w_lo[mt][n][1]);
-                        }
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) mma_16816(acc[i][n], ops[mt][i], w_hi[mt][n][0], w_hi[mt][n][1]);
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -514,36 +515,51 @@ __global__ void __launch_bounds__(kCaThreads, 2)
 
 // Joins the parts of a (sequence, head, row tile) that several CTAs left: with
 // M the largest of their maxima, o = sum f_c o_c / sum f_c l_c, f_c =
-// 2^(m_c - M).  Latency bounds it (a row's parts are few and far apart), so a
-// block has four rows only, a lane D / 32 of a row's values; up to four parts
-// are a warp's work, more are dealt out to the four warps, each with a maximum
-// of its own, and joined once more.
-constexpr int kJoinRows = 4;
-template <int D, int RT>
-__global__ void __launch_bounds__(kConsumers) cache_attention_join_kernel(const CacheAttArgs a, int ctas) {
-    constexpr int E = D / 32, SLOT = RT * (D + 2), BLOCKS = RT / kJoinRows;
-    __shared__ int s_sum[4];
-    __shared__ float s_part[4][kJoinRows][D], s_m[4][kJoinRows], s_l[4][kJoinRows];
+// 2^(m_c - M).  Latency bounds it (a row's parts are far apart), so a block has
+// few rows, a lane D / 32 of a row's values.  FEW: up to four parts are a
+// warp's work, and a block has four rows and four warps.  Otherwise (more
+// CTAs than four a row tile: few, long sequences) a block has one row, dealt
+// out part by part to eight warps, each with a maximum of its own, and joined
+// once more.  One sequence of 30000 keys, 35 parts a row: 31 us in all with
+// the first, 23 with the second; 32 sequences of 4096 to 8191: 78 and 81.
+template <bool FEW>
+struct Join {
+    static constexpr int ROWS = FEW ? 4 : 1, WARPS = FEW ? 4 : 8;
+};
+template <int D, int RT, bool FEW>
+__global__ void __launch_bounds__(32 * Join<FEW>::WARPS) cache_attention_join_kernel(const CacheAttArgs a, int ctas) {
+    constexpr int E = D / 32, SLOT = RT * (D + 2), ROWS = Join<FEW>::ROWS, WARPS = Join<FEW>::WARPS, BLOCKS = RT / ROWS;
+    __shared__ int s_units[2][WARPS];
+    __shared__ float s_part[WARPS][ROWS][D], s_m[WARPS][ROWS], s_l[WARPS][ROWS];
     griddep_launch_dependents();
     const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // lengths and counts were written before the kernel that left the parts began
     int before = 0, total = 0;
-    for (int i = threadIdx.x; i < a.batch; i += kConsumers) {
+    for (int i = threadIdx.x; i < a.batch; i += 32 * WARPS) {
         const int n = units_of(a, sequence<RT>(a, i));
         total += n;
         if (i < b) before += n;
     }
-    total = sum_128(total, s_sum);
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    before = sum_128(before, s_sum);
-    griddep_wait();
+    total = __reduce_add_sync(0xffffffffu, total);
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (lane == 0) {
+        s_units[0][warp] = total;
+        s_units[1][warp] = before;
+    }
+    __syncthreads();
+    total = before = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        total += s_units[0][w];
+        before += s_units[1][w];
+    }
     const Seq s = sequence<RT>(a, b);
     const int tile = blockIdx.x / BLOCKS, h = tile % a.c.heads, rt = tile / a.c.heads;
-    const int r0 = (blockIdx.x % BLOCKS) * kJoinRows, rows = min(RT, s.count * a.group - rt * RT) - r0;   // of this block
-    if (rt >= s.row_tiles || rows <= 0) return;
+    const int r0 = (blockIdx.x % BLOCKS) * ROWS, rows = min(RT, s.count * a.group - rt * RT) - r0;   // of this block
     const int per = units_a_cta(a, total, ctas);
     const int u0 = before + (h * s.row_tiles + rt) * s.tiles, c0 = u0 / per, c1 = (u0 + s.tiles - 1) / per;
-    if (c0 == c1) return;                                       // one CTA had it all
+    griddep_wait();
+    if (rt >= s.row_tiles || rows <= 0 || c0 == c1) return;     // nothing, or one CTA had it all
     auto slot = [&](int c) {                                    // a CTA's first part is in its first slot
         return a.parts + (2 * (int64_t)c + (c > c0 || c0 * per == u0 ? 0 : 1)) * SLOT;
     };
@@ -556,7 +572,7 @@ __global__ void __launch_bounds__(kConsumers) cache_attention_join_kernel(const 
         for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
         for (int c = first; c <= c1; c += step) {
             const float* p = slot(c);
             const float f = shrink(p[RT * D + r], M);
@@ -574,14 +590,14 @@ __global__ void __launch_bounds__(kConsumers) cache_attention_join_kernel(const 
     };
     float M, L, o[E];
     if (c1 - c0 < 4) {
-        if (warp < rows) {
+        if (warp < min(rows, ROWS)) {
             gather(r0 + warp, c0, 1, M, L, o);
             finish(r0 + warp, L, o);
         }
         return;
     }
-    for (int i = 0; i < min(rows, kJoinRows); ++i) {
-        gather(r0 + i, c0 + warp, 4, M, L, o);
+    for (int i = 0; i < min(rows, ROWS); ++i) {
+        gather(r0 + i, c0 + warp, WARPS, M, L, o);
 #pragma unroll
         for (int e = 0; e < E; ++e) s_part[warp][i][lane + 32 * e] = o[e];
         if (lane == 0) {
@@ -590,13 +606,15 @@ __global__ void __launch_bounds__(kConsumers) cache_attention_join_kernel(const 
         }
     }
     __syncthreads();
-    if (warp < rows) {
-        M = fmaxf(fmaxf(s_m[0][warp], s_m[1][warp]), fmaxf(s_m[2][warp], s_m[3][warp]));
+    if (warp < min(rows, ROWS)) {
+        M = -INFINITY;
         L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w][warp]);
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             const float f = shrink(s_m[w][warp], M);
             L = fmaf(s_l[w][warp], f, L);
 #pragma unroll
@@ -604,6 +622,20 @@ __global__ void __launch_bounds__(kConsumers) cache_attention_join_kernel(const 
         }
         finish(r0 + warp, L, o);
     }
+}
+
+template <int D, int RT, bool FEW>
+int launch_join_as(const CacheAttArgs& a, int64_t row_tiles, int ctas, cudaStream_t s) {
+    using J = Join<FEW>;
+    KZ_CHECK_CUDA(launch_pdl(cache_attention_join_kernel<D, RT, FEW>,
+                             dim3((unsigned)(row_tiles * a.c.heads * (RT / J::ROWS)), (unsigned)a.batch), dim3(32 * J::WARPS),
+                             0, s, a, ctas));
+    return KZ_OK;
+}
+template <int D, int RT>
+int launch_join(const CacheAttArgs& a, int64_t row_tiles, int ctas, cudaStream_t s) {
+    return ctas <= 4 * a.batch * a.c.heads * row_tiles ? launch_join_as<D, RT, true>(a, row_tiles, ctas, s)
+                                                       : launch_join_as<D, RT, false>(a, row_tiles, ctas, s);
 }
 
 // ---------------------------------------------------------------- launches
@@ -645,10 +677,7 @@ int launch_cache_attention(const CacheAttArgs& a, int64_t row_tiles, cudaStream_
     const int64_t most = (int64_t)a.batch * a.c.heads * row_tiles;
     const int grid = (int)std::min<int64_t>(2 * (int64_t)sm_count(), a.parts ? 2 * (int64_t)sm_count() : most);
     KZ_CHECK_CUDA(launch_pdl(cache_attention_kernel<D, NT, RG>, dim3(grid), dim3(kCaThreads), S::SMEM, s, tm_k, tm_v, a));
-    if (a.parts)
-        KZ_CHECK_CUDA(launch_pdl(cache_attention_join_kernel<D, S::RT>,
-                                 dim3((unsigned)(row_tiles * a.c.heads * (S::RT / kJoinRows)), (unsigned)a.batch), dim3(kConsumers), 0, s, a, grid));
-    return KZ_OK;
+    return a.parts ? launch_join<D, S::RT>(a, row_tiles, grid, s) : KZ_OK;
 }
 
 template <int D>
@@ -658,10 +687,7 @@ int dispatch_cache_attention(const CacheAttArgs& a, cudaStream_t s) {
         const int64_t tiles = (rows + kTcRows - 1) / kTcRows;
         const int grid = (int)std::min<int64_t>(sm_count(), a.parts ? sm_count() : a.batch * a.c.heads * tiles);
         const int st = launch_cache_attention_tc(a, D, grid, s);
-        if (!st && a.parts)
-            KZ_CHECK_CUDA(launch_pdl(cache_attention_join_kernel<D, kTcRows>,
-                                     dim3((unsigned)(tiles * a.c.heads * (kTcRows / kJoinRows)), (unsigned)a.batch), dim3(kConsumers), 0, s, a, grid));
-        return st;
+        return st || !a.parts ? st : launch_join<D, kTcRows>(a, tiles, grid, s);
     }
     const int rt = tile_rows(rows);
     const int64_t row_tiles = (rows + rt - 1) / rt;
