@@ -243,7 +243,11 @@ def _attention_64(q, kvals, vvals, length, count, heads, parents, scale):
     2^-23 of the terms' absolute sum, is off by (d + 4) 2^-23 sum |q k|; a
     weight's relative error is twice that (its own and the largest's) plus the
     exponential's and its own 22 bits; the weighted sum of n values adds
-    2^-23 for each 16 keys that a partial sum covers, and 32 for the joining."""
+    2^-23 for each 16 keys that a partial sum covers, and 32 for the joining.
+    The 22 bits are two fp16 values of an operand whose largest is brought to
+    [2^13, 2^14): below 2^-14 fp16 has steps of 2^-24 only, so that a factor is
+    off by 2^-25 at least, 2^-38 of the largest in its row: max|q| 2^-38 a term
+    of a product (doubled, as above), max(w |v|) 2^-38 a term of the sum."""
     tokens, kv, d = q.shape[0], kvals.shape[1], kvals.shape[2]
     out, bound = np.zeros((tokens, heads * d)), np.zeros((tokens, heads * d))
     for t in range(count):
@@ -255,8 +259,10 @@ def _attention_64(q, kvals, vvals, length, count, heads, parents, scale):
             e = np.exp(s - s.max())
             w = e / e.sum()
             out[t, h * d:(h + 1) * d] = w @ v
-            off = 2 * (d + 4) * (np.abs(k) @ np.abs(qq)).max() * scale + 16 + len(seen) / 16 + 32
-            bound[t, h * d:(h + 1) * d] = off * 2.0**-23 * (w @ np.abs(v))
+            size = abs(scale)
+            off = 2 * (d + 4) * (np.abs(k) @ np.abs(qq)).max() * size + 16 + len(seen) / 16 + 32
+            small = 2 * size * np.abs(qq).max() * np.abs(k).sum(1).max() * (w @ np.abs(v)) + len(seen) * (w * np.abs(v).max(1)).max()
+            bound[t, h * d:(h + 1) * d] = off * 2.0**-23 * (w @ np.abs(v)) + 2.0**-38 * small
     return out, bound
 
 
@@ -340,10 +346,24 @@ def test_attention_extreme_scales(cuda_device, tokens, spread, strong):
     _check_attention(book, [401 - tokens, 200 - tokens], None, tokens, 4, spread=spread, strong=strong)
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("spread,strong", [(12.0, 1e-4), (0.5, 12.0), (30.0, 1e-12), (1.0, 0.0), (1.0, 1e-30)])
+def test_attention_extreme_scales_many_rows(cuda_device, d, spread, strong):
+    """The same with more rows a key head than the small kernel takes (40 x 2, and 70 x 4 in three row tiles)."""
+    book = Book([441, 140], 2, d, 32)
+    _check_attention(book, [401, 100], None, 40, 4, spread=spread, strong=strong)
+    book = Book([270], 1, d, 64)
+    _check_attention(book, [200], None, 70, 4, _tree(70, 3), spread=spread, strong=strong)
+
+
 def test_attention_scale_argument(cuda_device):
     book = Book([300], 1, 32, 16)
     _check_attention(book, [299], None, 1, 2, scale=0.03)
     _check_attention(book, [299], None, 1, 2, scale=0.9)
+    book = Book([340], 1, 32, 16)
+    for scale in (0.03, 0.9, -0.2, 0.0):
+        _check_attention(book, [300], None, 40, 2, scale=scale)
+        _check_attention(book, [330], None, 1, 2, scale=scale)
 
 
 @pytest.mark.parametrize("lengths,tokens,heads,kv", [([20000], 1, 8, 1), ([9000, 3, 5000], 1, 2, 2), ([7000], 40, 4, 1)])
@@ -353,13 +373,27 @@ def test_attention_long(cuda_device, lengths, tokens, heads, kv):
     _check_attention(book, lengths, None, tokens, heads)
 
 
-def test_attention_is_repeatable_and_independent_of_the_batch(cuda_device):
+@pytest.mark.parametrize("tokens,heads", [(1, 8), (12, 4), (50, 8)])
+def test_attention_is_repeatable(cuda_device, tokens, heads):
     """The same call gives the same bits."""
     book = Book([3000, 700], 2, 128, 64)
-    lengths = [2999, 699]
-    a = _check_attention(book, lengths, None, 1, 8)
+    lengths = [3000 - tokens, 700 - tokens]
+    a = _check_attention(book, lengths, None, tokens, heads)
     for _ in range(3):
-        assert _check_attention(book, lengths, None, 1, 8).tobytes() == a.tobytes()
+        assert _check_attention(book, lengths, None, tokens, heads).tobytes() == a.tobytes()
+
+
+def test_attention_many_sequences(cuda_device):
+    """More sequences than a block has threads, most of them without tokens."""
+    rs = np.random.RandomState(2)
+    lengths = [int(n) for n in rs.randint(0, 40, 300)]
+    counts = [int(n) for n in rs.randint(0, 2, 300)]
+    lengths[150], counts[150] = 900, 1
+    book = Book([a + b for a, b in zip(lengths, counts)], 1, 32, 16)
+    _check_attention(book, lengths, counts, 1, 1)
+    counts = [3 * c for c in counts]
+    book = Book([a + b for a, b in zip(lengths, counts)], 1, 32, 16)
+    _check_attention(book, lengths, counts, 3, 12)
 
 
 def test_attention_nan_in_a_visible_row_only(cuda_device):
@@ -374,6 +408,53 @@ def test_attention_nan_in_a_visible_row_only(cuda_device):
     want = torch.zeros(6, 4, dtype=torch.bool)
     want[1, 2:] = want[3, 2:] = True
     assert torch.equal(bad, want) and torch.equal(torch.isnan(y).any(-1).cpu(), want)
+
+
+@pytest.mark.parametrize("part", ["k", "v"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_nan_among_many_rows(cuda_device, part, d):
+    """The same in the kernel for many rows: 40 nodes, a NaN or infinite scale
+    at one of them, NaN throughout where no token is."""
+    book = Book([140], 2, d, 32)
+    book.fill([140])
+    parents = _tree(40, 5)
+    q = torch.randn(1, 40, 4 * d, device="cuda")
+    for bad in (math.nan, math.inf):
+        at = 100 + 7
+        scale = book.cache.k_scale if part == "k" else book.cache.v_scale
+        was = scale[book.table_h[0, at // 32], 1, at % 32].clone()
+        scale[book.table_h[0, at // 32], 1, at % 32] = bad
+        y = book.cache.attention(q, 4, book.table, _i32([100]), None, _i32(parents)).data.view(40, 4, d)
+        sees = torch.tensor([7 in _sees(parents, 40, t) for t in range(40)])
+        good = torch.isfinite(y).all(-1).cpu()
+        assert good[:, :2].all() and good[~sees].all()
+        if part == "v" or math.isnan(bad):
+            assert not torch.isfinite(y).any(-1).cpu()[sees][:, 2:].any()
+        scale[book.table_h[0, at // 32], 1, at % 32] = was
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("tokens,parents", [(20, True), (40, True), (40, False), (9, False)])
+def test_bad_pages_among_many_rows(cuda_device, tokens, parents):
+    """Two pages of the context and one of the new tokens' that are none."""
+    from kansaiml_b200 import _lib
+    n = 200 + tokens
+    book = Book([n], 1, 64, 16)
+    kvals, vvals = book.fill([n])
+    table = book.table.clone()
+    for i in (0, 7, 13):
+        table[0, i] = 10 ** 6 if i else -1
+    par = _tree(tokens, 2) if parents else None
+    q = np.random.RandomState(4).standard_normal((1, tokens, 4 * 64)).astype(np.float32)
+    y = book.cache.attention(_dev(q), 4, table, _i32([200]), None, None if par is None else _i32(par)).numpy()[0]
+    assert _status() == _lib.KZ_ERR_INVALID_ARGUMENT
+    there = np.array([p // 16 not in (0, 7, 13) for p in range(n)])
+    for t in range(tokens):
+        seen = [p for p in list(range(200)) + [200 + j for j in _sees(par, tokens, t)] if there[p]]
+        for h in range(4):
+            want, bound = _attention_64(q[0, t:t + 1, h * 64:(h + 1) * 64], kvals[0][seen], vvals[0][seen], len(seen) - 1, 1,
+                                        1, None, 1 / 8)
+            assert np.all(np.abs(y[t, h * 64:(h + 1) * 64] - want[0]) <= bound[0]), (t, h)
 
 
 def test_bad_pages_are_left_out_and_reported(cuda_device):
@@ -419,6 +500,54 @@ def test_empty_calls(cuda_device):
     book.cache.write(z, z, book.table[:0], none)
     assert book.cache.attention(torch.empty(1, 0, 64, device="cuda"), 2, book.table, _i32([4])).shape == [1, 0, 64]
     assert book.cache.read(book.table[:0], none, 5)[0].shape == [0, 5, 64]
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("tokens,parents", [(5, False), (40, True)])
+def test_attention_nan_in_q_stays_in_its_row(cuda_device, tokens, parents):
+    """A NaN or infinity in one row of q, and a very large row beside ordinary ones."""
+    book = Book([150], 1, 64, 16)
+    book.fill([150])
+    par = _i32(_tree(tokens, 6)) if parents else None
+    q = torch.randn(1, tokens, 4 * 64, device="cuda")
+    lengths = _i32([150 - tokens])
+    want = book.cache.attention(q, 4, book.table, lengths, None, par).data.view(tokens, 4, 64)
+    for bad in (math.nan, math.inf, 1e30):
+        x = q.clone()
+        x[0, 2, 64 + 9] = bad
+        y = book.cache.attention(x, 4, book.table, lengths, None, par).data.view(tokens, 4, 64)
+        if bad != 1e30:
+            assert torch.isnan(y[2, 1]).all()
+        y[2, 1] = want[2, 1]
+        assert torch.equal(y, want)
+    assert _status() == 0
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """A pool of more than 2^31 bytes of codes, its last pages used: written,
+    attended over by both kernels, kept and read."""
+    from kansaiml_b200.cache import QCache
+    pages, kv, page, d = 17000, 8, 128, 128
+    cache = QCache(pages, kv, d, page, "cuda")
+    assert cache.k_codes.numel() > 2**31
+    table, zero = _i32([[pages - 1, pages - 3, pages - 2]]), _i32([0])
+    rs = np.random.RandomState(8)
+    k, v = (rs.standard_normal((1, 300, kv * d)).astype(np.float32) for _ in range(2))
+    cache.write(_dev(k), _dev(v), table, zero)
+    stood = []
+    for x in (k, v):
+        codes, scales = _quantized(x.reshape(300, kv, d))
+        stood.append(codes * scales.astype(np.float32).astype(np.float64)[..., None])
+    for tokens in (1, 40):
+        q = rs.standard_normal((1, tokens, kv * d)).astype(np.float32)
+        y = cache.attention(_dev(q), kv, table, _i32([300 - tokens])).numpy()[0]
+        want, bound = _attention_64(q[0], stood[0], stood[1], 300 - tokens, tokens, kv, None, d**-0.5)
+        assert np.all(np.abs(y - want) <= bound)
+    cache.keep(table, _i32([100]), _i32([[0, 50, 199]]), _i32([3]))
+    got = cache.read(table, _i32([103]), 103)
+    for part in range(2):
+        want = stood[part][[*range(101), 150, 299]].reshape(103, kv * d).astype(np.float32)
+        np.testing.assert_array_equal(got[part].numpy()[0], want)
     assert _status() == 0
 
 
