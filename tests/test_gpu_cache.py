@@ -543,7 +543,7 @@ def test_offsets_past_32_bits(cuda_device):
         y = cache.attention(_dev(q), kv, table, _i32([300 - tokens])).numpy()[0]
         want, bound = _attention_64(q[0], stood[0], stood[1], 300 - tokens, tokens, kv, None, d**-0.5)
         assert np.all(np.abs(y - want) <= bound)
-    cache.keep(table, _i32([100]), _i32([[0, 50, 199]]), _i32([3]))
+    cache.keep(table, _i32([100]), _i32([[0, 50, 199] + [-1] * 197]), _i32([3]))     # a path of a tree of 200
     got = cache.read(table, _i32([103]), 103)
     for part in range(2):
         want = stood[part][[*range(101), 150, 299]].reshape(103, kv * d).astype(np.float32)
