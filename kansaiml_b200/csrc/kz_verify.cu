@@ -169,6 +169,8 @@ __device__ __forceinline__ float4 four(const float* row, int i, int end, int wid
 
 __global__ void __launch_bounds__(kVThreads, 2) verify_tree_kernel(VerifyArgs a) {
     __shared__ VerifyShared s;
+    // every CTA of the cluster has begun before the first sum goes into another's shared memory
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     griddep_wait();
     griddep_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
@@ -292,6 +294,7 @@ __global__ void __launch_bounds__(kVThreads, 2) verify_tree_kernel(VerifyArgs a)
             const double all = warp_sums_f64(sum);
             if ((lane & 3) == 0) s.chunk_sum[warp][lane >> 2] = all;
             __syncthreads();
+            if (meeting == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // (the first turn always sums)
             if (warp == 0) {
                 // the slice's sum, to every CTA of the cluster
                 double t = 0.0;
