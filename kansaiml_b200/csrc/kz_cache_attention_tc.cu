@@ -212,7 +212,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
         tmem_relinquish();
     }
     griddep_wait();
-    griddep_launch_dependents();
 
     // ---- this CTA's units, and where they begin
     if (warp < 4) {
@@ -243,6 +242,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    griddep_launch_dependents();           // not before this CTA has its tensor memory: a dependent may take some
     constexpr uint32_t tmem = 0;           // where all 512 columns begin
     Walk<kTcRows> walk;
     walk.at = s_units[0];
