@@ -152,7 +152,7 @@ class QCache:
             x = x.contiguous()
             if x.data_ptr() & 15:
                 x = x.clone()
-            bs, rs, _ = x.stride()
+            bs, rs = x.shape[1] * width, width      # (a single row's own strides may be anything)
             at = x.data_ptr()
         return x, at, bs, rs
 

@@ -14,6 +14,7 @@ import numpy as np
 import torch
 
 from . import nn
+from ._lib import KZ_TREE_MAX_NODES
 from .cache import PagePool, QCache, verify_tree
 from .quantize import QActivation, QLinear
 from .tensor import Tensor, from_numpy
@@ -149,9 +150,13 @@ class Decoder(nn.Module):
         without drafts.  Returns one list of new ids per prompt."""
         device = self.tok.weight.device
         seen = [list(p) for p in prompts]
-        batch, longest = len(seen), max(len(p) for p in seen)
-        if min(len(p) for p in seen) < 1 or not all(0 <= t < self.vocab for p in seen for t in p):
+        batch, longest = len(seen), max((len(p) for p in seen), default=0)
+        if not seen or min(len(p) for p in seen) < 1 or not all(0 <= t < self.vocab for p in seen for t in p):
             raise ValueError(f"Decoder.generate: a prompt is one or more ids below {self.vocab}")
+        if not 0 <= drafts < KZ_TREE_MAX_NODES:
+            raise ValueError(f"Decoder.generate: drafts must be 0 to {KZ_TREE_MAX_NODES - 1} (got {drafts})")
+        if not temperature >= 0:
+            raise ValueError(f"Decoder.generate: temperature must be 0 or above (got {temperature})")
         if new_tokens < 1 or longest + new_tokens > self.ctx:
             raise ValueError(f"Decoder.generate: {longest} + {new_tokens} tokens, the context is {self.ctx}")
         cache = self.new_cache(batch)

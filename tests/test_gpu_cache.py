@@ -167,6 +167,23 @@ def test_write_copies_views_a_kernel_cannot_read(cuda_device):
         assert a.tobytes() == b.tobytes()
 
 
+def test_a_single_row_with_any_strides(cuda_device):
+    """One row of one sequence is contiguous for torch whatever its strides say."""
+    x = torch.randn(1, 1, 128, device="cuda")
+    odd = torch.as_strided(x.reshape(-1), (1, 1, 128), (129, 7, 1))
+    assert odd.stride() == (129, 7, 1) and odd.is_contiguous()
+    books = [Book([5], 2, 64, 16) for _ in range(2)]
+    outs = []
+    for book, y in zip(books, (x, odd)):
+        book.cache.write(y, y, book.table, _i32([4]))
+        book.cache.write(y, y, book.table, _i32([0]))
+        outs.append(book.cache.attention(y, 2, book.table, _i32([0])).numpy())
+    for a, b in zip(books[0].held(), books[1].held()):
+        assert a.tobytes() == b.tobytes()
+    np.testing.assert_array_equal(outs[0], outs[1])
+    assert _status() == 0
+
+
 # --------------------------------------------------------------------- read
 
 @pytest.mark.parametrize("d,kv,page,lengths,most", [
@@ -776,8 +793,15 @@ def test_decoder_generates_through_the_cache(cuda_device):
             assert a == model.generate(prompts, 30, temperature, drafts, seed=7)
     with pytest.raises(ValueError, match="context"):
         model.generate(prompts, 157)
-    with pytest.raises(ValueError, match="prompt"):
-        model.generate([[1], []], 3)
+    for empty in ([[1], []], []):
+        with pytest.raises(ValueError, match="prompt"):
+            model.generate(empty, 3)
+    for drafts in (-1, 256):
+        with pytest.raises(ValueError, match="drafts"):
+            model.generate(prompts, 3, 1.0, drafts)
+    for temperature in (-1.0, math.nan):
+        with pytest.raises(ValueError, match="temperature"):
+            model.generate(prompts, 3, temperature)
     with pytest.raises(ValueError, match="capacity"):
         cache.room(200)
     assert _status() == 0
@@ -812,6 +836,54 @@ def test_captured_steps_replay_with_new_lengths(cuda_device):
         torch.cuda.synchronize()
         assert torch.equal(y1, book.cache.attention(q, 8, book.table, lengths).data)
         assert torch.equal(y2, book.cache.attention(q2, 8, book.table, l2).data)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("nodes,vocab,draft", [(7, 11, False), (40, 9000, True)])
+def test_a_captured_run_of_all(cuda_device, nodes, vocab, draft):
+    """Write, attention over a tree, verification, keep and the new lengths as
+    one graph, with no call before the capture: each replay leaves what the
+    same calls leave one by one."""
+    from kansaiml_b200.cache import verify_tree
+    batch, kv, heads, d = 3, 2, 4, 64
+    rs = np.random.RandomState(31)
+    books = [Book([700, 650, 900], kv, d, 32) for _ in range(2)]
+    for book in books:
+        book.fill([300, 20, 511])
+    lengths = [_i32([300, 20, 511]) for _ in range(2)]
+    k, v, q = (torch.zeros(batch, nodes, n * d, device="cuda") for n in (kv, kv, heads))
+    tokens, parents = torch.zeros(batch, nodes, dtype=torch.int64, device="cuda"), _i32([[-1] * nodes] * batch)
+    target, other = (torch.zeros(batch, nodes, vocab, device="cuda") for _ in range(2))
+    au, su = torch.zeros(batch, nodes, device="cuda"), torch.zeros(batch, device="cuda")
+
+    def step(book, lengths):
+        book.cache.write(k, v, book.table, lengths)
+        y = book.cache.attention(q, heads, book.table, lengths, None, parents).data
+        path, count, token = verify_tree(tokens, parents, target, other if draft else None, au, su)
+        book.cache.keep(book.table, lengths, path, count)
+        lengths += count
+        return y, path, count, token
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(books[0], lengths[0])
+    for turn in range(4):
+        for t in (k, v, q):
+            t.copy_(torch.randn_like(t))
+        tokens.copy_(_dev(rs.randint(0, vocab, (batch, nodes))))
+        parents.copy_(_dev(np.array([_tree(nodes, 10 * turn + b) for b in range(batch)], np.int32)))
+        for t in (target, other):
+            t.copy_(_dev(_softmax(rs, (batch, nodes, vocab), 1.0)))
+        au.copy_(_dev(rs.uniform(size=(batch, nodes)).astype(np.float32) * (1e-4 if turn % 2 else 0.3)))
+        su.copy_(_dev(rs.uniform(size=batch).astype(np.float32)))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, step(books[1], lengths[1])):
+            assert torch.equal(a, b)
+        assert torch.equal(lengths[0], lengths[1])
+    most = int(lengths[0].max())
+    for a, b in zip(*(book.cache.read(book.table, n, most) for book, n in zip(books, lengths))):
+        assert torch.equal(a.data, b.data)
     assert _status() == 0
 
 
