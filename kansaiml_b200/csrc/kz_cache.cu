@@ -20,19 +20,6 @@ namespace {
 
 constexpr int kCacheThreads = 256;
 
-// x / d and x % d for 0 <= x < 2^31 by one multiply-high (the rows of a call
-// are numbered through and split into sequence, token and head by each lane).
-struct FastDiv {
-    uint32_t d, m, l;
-};
-FastDiv fast_div(uint32_t d) {
-    FastDiv f{d, 0, 0};
-    while ((1ull << f.l) < d) ++f.l;
-    f.m = (uint32_t)(((1ull << 32) * ((1ull << f.l) - d)) / d + 1);
-    return f;
-}
-__device__ __forceinline__ uint32_t div_by(uint32_t x, const FastDiv& f) { return (__umulhi(f.m, x) + x) >> f.l; }
-
 struct WriteArgs {
     CacheView c;
     SeqView s;

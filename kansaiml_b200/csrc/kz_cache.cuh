@@ -19,6 +19,18 @@ struct SeqView {
     int cols;
 };
 
+// x / d for 0 <= x < 2^31 by one multiply-high.
+struct FastDiv {
+    uint32_t d, m, l;
+};
+inline FastDiv fast_div(uint32_t d) {
+    FastDiv f{d, 0, 0};
+    while ((1ull << f.l) < d) ++f.l;
+    f.m = (uint32_t)(((1ull << 32) * ((1ull << f.l) - d)) / d + 1);
+    return f;
+}
+__device__ __forceinline__ uint32_t div_by(uint32_t x, const FastDiv& f) { return (__umulhi(f.m, x) + x) >> f.l; }
+
 // Host checks; each returns KZ_OK or records why not (`who`: the entry point).
 int cache_view(const kz_cache* c, const char* who, CacheView* v);
 int seq_view(const int32_t* table, int64_t cols, const int32_t* lengths, int64_t batch, const char* who, SeqView* v);

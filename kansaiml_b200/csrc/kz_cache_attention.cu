@@ -104,9 +104,7 @@ __global__ void __launch_bounds__(kCaThreads, 2)
     __shared__ float s_m[S::KG][S::RT], s_l[S::KG][S::RT];
     __shared__ uint32_t s_sees[S::RT + 1][kTreeWords];
     __shared__ int32_t s_parent[KZ_TREE_MAX_NODES];
-    __shared__ int s_sum[4], s_part[kConsumers];
-    __shared__ int s_start[2];                     // this CTA's first sequence and that one's first unit
-    __shared__ int s_units[2];                     // its units
+    __shared__ RangeShared s_range;
     __shared__ int s_abort;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // uniform: so are the roles' branches
@@ -121,39 +119,9 @@ __global__ void __launch_bounds__(kCaThreads, 2)
     griddep_wait();
     griddep_launch_dependents();
 
-    // ---- this CTA's units, and where they begin
-    if (warp < 4) {
-        const int each = (a.batch + kConsumers - 1) / kConsumers;
-        int mine = 0;
-        for (int b = tid * each; b < min(a.batch, (tid + 1) * each); ++b) mine += units_of(a, sequence<S::RT>(a, b));
-        s_part[tid] = mine;
-        const int total = sum_128(mine, s_sum);
-        if (tid == 0) {
-            const int per = units_a_cta(a, total, gridDim.x);
-            const int u0 = (int)min((int64_t)total, (int64_t)per * blockIdx.x), u1 = (int)min((int64_t)total, (int64_t)u0 + per);
-            s_units[0] = u0;
-            s_units[1] = u1;
-            int base = 0, i = 0, b = 0;
-            if (u0 < u1) {
-                while (i < kConsumers - 1 && base + s_part[i] <= u0) base += s_part[i++];
-                b = i * each;
-                for (; b < a.batch - 1; ++b) {
-                    const int n = units_of(a, sequence<S::RT>(a, b));
-                    if (u0 < base + n) break;
-                    base += n;
-                }
-            }
-            s_start[0] = b;
-            s_start[1] = base;
-        }
-    }
+    if (warp < 4) find_range<S::RT>(a, s_range);
     __syncthreads();
-    Walk<S::RT> walk;
-    walk.at = s_units[0];
-    walk.end = s_units[1];
-    walk.b = s_start[0];
-    walk.base = s_start[1];
-    if (walk.at < walk.end) walk.s = sequence<S::RT>(a, walk.b);
+    Walk<S::RT> walk(a, s_range.range);
     Segment g;
     int it = 0;      // tiles loaded or used so far
 
@@ -527,39 +495,42 @@ struct Join {
     static constexpr int ROWS = FEW ? 4 : 1, WARPS = FEW ? 4 : 8;
 };
 template <int D, int RT, bool FEW>
-__global__ void __launch_bounds__(32 * Join<FEW>::WARPS) cache_attention_join_kernel(const CacheAttArgs a, int ctas) {
+__global__ void __launch_bounds__(32 * Join<FEW>::WARPS) cache_attention_join_kernel(const CacheAttArgs a) {
     constexpr int E = D / 32, SLOT = RT * (D + 2), ROWS = Join<FEW>::ROWS, WARPS = Join<FEW>::WARPS, BLOCKS = RT / ROWS;
-    __shared__ int s_units[2][WARPS];
+    __shared__ Work s_work[WARPS];
+    __shared__ int s_before[WARPS];
     __shared__ float s_part[WARPS][ROWS][D], s_m[WARPS][ROWS], s_l[WARPS][ROWS];
     griddep_launch_dependents();
     const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // lengths and counts were written before the kernel that left the parts began
-    int before = 0, total = 0;
+    Work w{0, 0, 0};
+    int before = 0;
     for (int i = threadIdx.x; i < a.batch; i += 32 * WARPS) {
-        const int n = units_of(a, sequence<RT>(a, i));
-        total += n;
-        if (i < b) before += n;
+        const Seq s = sequence<RT>(a, i);
+        w.add(a, s);
+        if (i < b) before += units_of(a, s, false);
     }
-    total = __reduce_add_sync(0xffffffffu, total);
+    w.add_warp();
     before = __reduce_add_sync(0xffffffffu, before);
     if (lane == 0) {
-        s_units[0][warp] = total;
-        s_units[1][warp] = before;
+        s_work[warp] = w;
+        s_before[warp] = before;
     }
     __syncthreads();
-    total = before = 0;
+    w = s_work[0];
+    before = s_before[0];
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-        total += s_units[0][w];
-        before += s_units[1][w];
+    for (int i = 1; i < WARPS; ++i) {
+        w.add(s_work[i]);
+        before += s_before[i];
     }
     const Seq s = sequence<RT>(a, b);
     const int tile = blockIdx.x / BLOCKS, h = tile % a.c.heads, rt = tile / a.c.heads;
     const int r0 = (blockIdx.x % BLOCKS) * ROWS, rows = min(RT, s.count * a.group - rt * RT) - r0;   // of this block
-    const int per = units_a_cta(a, total, ctas);
+    const int per = max(1, a_cta(a, w.units));
     const int u0 = before + (h * s.row_tiles + rt) * s.tiles, c0 = u0 / per, c1 = (u0 + s.tiles - 1) / per;
     griddep_wait();
-    if (rt >= s.row_tiles || rows <= 0 || c0 == c1) return;     // nothing, or one CTA had it all
+    if (whole_ranges(a, w) || rt >= s.row_tiles || rows <= 0 || c0 == c1) return;     // nothing, or one CTA had it all
     auto slot = [&](int c) {                                    // a CTA's first part is in its first slot
         return a.parts + (2 * (int64_t)c + (c > c0 || c0 * per == u0 ? 0 : 1)) * SLOT;
     };
@@ -625,17 +596,17 @@ __global__ void __launch_bounds__(32 * Join<FEW>::WARPS) cache_attention_join_ke
 }
 
 template <int D, int RT, bool FEW>
-int launch_join_as(const CacheAttArgs& a, int64_t row_tiles, int ctas, cudaStream_t s) {
+int launch_join_as(const CacheAttArgs& a, int64_t row_tiles, cudaStream_t s) {
     using J = Join<FEW>;
     KZ_CHECK_CUDA(launch_pdl(cache_attention_join_kernel<D, RT, FEW>,
                              dim3((unsigned)(row_tiles * a.c.heads * (RT / J::ROWS)), (unsigned)a.batch), dim3(32 * J::WARPS),
-                             0, s, a, ctas));
+                             0, s, a));
     return KZ_OK;
 }
 template <int D, int RT>
-int launch_join(const CacheAttArgs& a, int64_t row_tiles, int ctas, cudaStream_t s) {
-    return ctas <= 4 * a.batch * a.c.heads * row_tiles ? launch_join_as<D, RT, true>(a, row_tiles, ctas, s)
-                                                       : launch_join_as<D, RT, false>(a, row_tiles, ctas, s);
+int launch_join(const CacheAttArgs& a, int64_t row_tiles, cudaStream_t s) {
+    return a.ctas <= 4 * a.batch * a.c.heads * row_tiles ? launch_join_as<D, RT, true>(a, row_tiles, s)
+                                                       : launch_join_as<D, RT, false>(a, row_tiles, s);
 }
 
 // ---------------------------------------------------------------- launches
@@ -643,9 +614,10 @@ int launch_join(const CacheAttArgs& a, int64_t row_tiles, int ctas, cudaStream_t
 // Rows of a tile: the smallest of 8, 16 and 32 that holds a key head's rows.
 int tile_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
 
-// Whether every (sequence, head, row tile) is one CTA's whole work: the table
-// holds no more tiles than a CTA's range has at least.
-bool whole_ranges(int64_t cols, int64_t page) { return cols * page <= (int64_t)kMinTiles * kKT; }
+// Whether a call needs no workspace and no join: its table holds so few tiles
+// of keys that whole_ranges would have every CTA take whole row tiles (but for
+// more of those than CTAs, where it is near).
+bool short_table(int64_t cols, int64_t page) { return cols * page <= 4 * kKT; }
 
 // Whether the rows of a key head are many enough for the tcgen05 kernel, whose
 // time does not depend on them up to 128: at 32 rows (batch 16, 8 key heads of
@@ -659,7 +631,7 @@ int64_t parts_floats(int64_t rows, int64_t d) {
 }
 
 template <int D, int NT, int RG>
-int launch_cache_attention(const CacheAttArgs& a, int64_t row_tiles, cudaStream_t s) {
+int launch_cache_attention(CacheAttArgs a, int64_t row_tiles, cudaStream_t s) {
     using S = Shape<D, NT, RG>;
     static std::atomic<int> attr_set[64];
     int dev = 0;
@@ -675,19 +647,21 @@ int launch_cache_attention(const CacheAttArgs& a, int64_t row_tiles, cudaStream_
     if (!st) st = tensor_map_rows_i8(&tm_v, a.c.codes[1], D, rows, (uint32_t)a.c.page);
     if (st) return st;
     const int64_t most = (int64_t)a.batch * a.c.heads * row_tiles;
-    const int grid = (int)std::min<int64_t>(2 * (int64_t)sm_count(), a.parts ? 2 * (int64_t)sm_count() : most);
-    KZ_CHECK_CUDA(launch_pdl(cache_attention_kernel<D, NT, RG>, dim3(grid), dim3(kCaThreads), S::SMEM, s, tm_k, tm_v, a));
-    return a.parts ? launch_join<D, S::RT>(a, row_tiles, grid, s) : KZ_OK;
+    a.ctas = (int)std::min<int64_t>(2 * (int64_t)sm_count(), a.parts ? 2 * (int64_t)sm_count() : most);
+    a.by_ctas = fast_div((uint32_t)a.ctas);
+    KZ_CHECK_CUDA(launch_pdl(cache_attention_kernel<D, NT, RG>, dim3(a.ctas), dim3(kCaThreads), S::SMEM, s, tm_k, tm_v, a));
+    return a.parts ? launch_join<D, S::RT>(a, row_tiles, s) : KZ_OK;
 }
 
 template <int D>
-int dispatch_cache_attention(const CacheAttArgs& a, cudaStream_t s) {
+int dispatch_cache_attention(CacheAttArgs a, cudaStream_t s) {
     const int64_t rows = (int64_t)a.tokens * a.group;
     if (many_rows(rows)) {
         const int64_t tiles = (rows + kTcRows - 1) / kTcRows;
-        const int grid = (int)std::min<int64_t>(sm_count(), a.parts ? sm_count() : a.batch * a.c.heads * tiles);
-        const int st = launch_cache_attention_tc(a, D, grid, s);
-        return st || !a.parts ? st : launch_join<D, kTcRows>(a, tiles, grid, s);
+        a.ctas = (int)std::min<int64_t>(sm_count(), a.parts ? sm_count() : a.batch * a.c.heads * tiles);
+        a.by_ctas = fast_div((uint32_t)a.ctas);
+        const int st = launch_cache_attention_tc(a, D, s);
+        return st || !a.parts ? st : launch_join<D, kTcRows>(a, tiles, s);
     }
     const int rt = tile_rows(rows);
     const int64_t row_tiles = (rows + rt - 1) / rt;
@@ -704,7 +678,7 @@ using namespace kz;
 extern "C" size_t kz_cache_attention_workspace_bytes(const kz_cache* cache, int64_t tokens, int64_t heads,
                                                      int64_t table_cols) {
     if (!cache || cache->kv_heads <= 0 || tokens <= 0 || heads <= 0 || table_cols < 0) return 0;
-    if (whole_ranges(table_cols, cache->page_size)) return 0;
+    if (short_table(table_cols, cache->page_size)) return 0;
     return sizeof(float) * (size_t)parts_floats(tokens * (heads / cache->kv_heads), cache->head_dim);
 }
 

@@ -9,7 +9,7 @@
 namespace kz {
 
 constexpr int kKT = 128;                    // keys a tile
-constexpr int kMinTiles = 4;                // tiles a CTA's range has at least
+constexpr int kJoinTiles = 5;               // what ranges that end inside a row tile cost, in tiles (see whole_ranges)
 constexpr int kTreeWords = KZ_TREE_MAX_NODES / 32;
 
 struct CacheAttArgs {
@@ -21,8 +21,10 @@ struct CacheAttArgs {
     const int32_t* parents;
     int64_t parents_bs;
     float* out;
-    float* parts;          // two slots a CTA: sums [RT][D], maxima [RT], weights [RT]; NULL: every range is whole
+    float* parts;          // two slots a CTA: sums [RT][D], maxima [RT], weights [RT]; NULL: no range ends inside a row tile
     int batch, tokens, heads, group;
+    int ctas;              // the launch's
+    FastDiv by_ctas;
     float scale;
     int* status;
 };
@@ -43,21 +45,80 @@ __device__ __forceinline__ Seq sequence(const CacheAttArgs& a, int b) {
     s.row_tiles = (int)(((int64_t)s.count * a.group + RT - 1) / RT);
     return s;
 }
-// (the host refuses calls of 2^31 units or more)
-__device__ __forceinline__ int units_of(const CacheAttArgs& a, const Seq& s) {
-    return s.row_tiles * a.c.heads * (a.parts ? s.tiles : 1);            // whole ranges: a unit is a row tile
+// A call's work, summed over sequences (the host refuses calls of 2^31 units or
+// more): its row tiles (of every head), their tiles of keys, and the most that a row tile has.
+struct Work {
+    int row_tiles, units, tiles;
+    __device__ __forceinline__ void add(const CacheAttArgs& a, const Seq& s) {
+        row_tiles += s.row_tiles * a.c.heads;
+        units += s.row_tiles * a.c.heads * s.tiles;
+        if (s.row_tiles) tiles = max(tiles, s.tiles);
+    }
+    __device__ __forceinline__ void add(const Work& o) {
+        row_tiles += o.row_tiles;
+        units += o.units;
+        tiles = max(tiles, o.tiles);
+    }
+    __device__ __forceinline__ void add_warp() {
+        row_tiles = __reduce_add_sync(0xffffffffu, row_tiles);
+        units = __reduce_add_sync(0xffffffffu, units);
+        tiles = __reduce_max_sync(0xffffffffu, tiles);
+    }
+};
+// Whether each CTA takes whole row tiles (a unit of work is then a row tile, not
+// a tile of keys): where the most that one would do that way is not more than in
+// equal ranges, whose CTAs begin and end inside row tiles and need the join.
+__device__ __forceinline__ int a_cta(const CacheAttArgs& a, int units) { return units > 0 ? div_by(units - 1, a.by_ctas) + 1 : 0; }
+__device__ __forceinline__ bool whole_ranges(const CacheAttArgs& a, const Work& w) {
+    return !a.parts || (int64_t)a_cta(a, w.row_tiles) * w.tiles <= (int64_t)a_cta(a, w.units) + kJoinTiles;
 }
-__device__ __forceinline__ int units_a_cta(const CacheAttArgs& a, int total, int ctas) {
-    return max((int)(((int64_t)total + ctas - 1) / ctas), a.parts ? kMinTiles : 1);
+__device__ __forceinline__ int units_of(const CacheAttArgs& a, const Seq& s, bool whole) {
+    return s.row_tiles * a.c.heads * (whole ? 1 : s.tiles);
 }
 
-// Sum of a value over the 128 threads that share `sum` (named barrier 1).
-__device__ __forceinline__ int sum_128(int v, int* sum) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if ((threadIdx.x & 31) == 0) sum[threadIdx.x >> 5] = v;
+// A CTA's units [at, end), and the sequence that holds the first of them with that one's first unit.
+struct Range {
+    int at, end, b, base;
+    bool whole;
+};
+struct RangeShared {
+    Work warp[4];
+    Work part[128];
+    Range range;
+};
+// By 128 threads (named barrier 1); the result is in s.range for whoever syncs with them afterwards.
+template <int RT>
+__device__ __forceinline__ void find_range(const CacheAttArgs& a, RangeShared& s) {
+    const int tid = threadIdx.x, each = (a.batch + 127) / 128;
+    Work w{0, 0, 0};
+    for (int b = tid * each; b < min(a.batch, (tid + 1) * each); ++b) w.add(a, sequence<RT>(a, b));
+    s.part[tid] = w;
+    w.add_warp();
+    if ((tid & 31) == 0) s.warp[tid >> 5] = w;
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    return sum[0] + sum[1] + sum[2] + sum[3];
+    if (tid != 0) return;
+    w = s.warp[0];
+    for (int i = 1; i < 4; ++i) w.add(s.warp[i]);
+    Range r;
+    r.whole = whole_ranges(a, w);
+    const int total = r.whole ? w.row_tiles : w.units, per = a_cta(a, total);
+    r.at = (int)min((int64_t)total, (int64_t)per * blockIdx.x);
+    r.end = (int)min((int64_t)total, (int64_t)r.at + per);
+    r.b = r.base = 0;
+    if (r.at < r.end) {
+        int i = 0;
+        for (; i < 127; ++i) {
+            const int n = r.whole ? s.part[i].row_tiles : s.part[i].units;
+            if (r.at < r.base + n) break;
+            r.base += n;
+        }
+        for (r.b = i * each; r.b < a.batch - 1; ++r.b) {
+            const int n = units_of(a, sequence<RT>(a, r.b), r.whole);
+            if (r.at < r.base + n) break;
+            r.base += n;
+        }
+    }
+    s.range = r;
 }
 
 // A part of one (sequence, head, row tile): key tiles [t0, t1).
@@ -68,20 +129,25 @@ struct Segment {
     bool whole;                    // all of its tiles
 };
 
-// Walks the segments of units [at, end): b0, base: the sequence that holds `at` and its first unit.
+// Walks the segments of a CTA's range.
 template <int RT>
 struct Walk {
-    int at, end, base, b;
+    int at, end, b, base;
+    bool whole;
     Seq s;
+    __device__ __forceinline__ Walk(const CacheAttArgs& a, const Range& r)
+        : at(r.at), end(r.end), b(r.b), base(r.base), whole(r.whole) {
+        if (at < end) s = sequence<RT>(a, b);
+    }
     __device__ __forceinline__ bool next(const CacheAttArgs& a, Segment& g) {
         if (at >= end) return false;
-        while (at >= base + units_of(a, s)) {
+        while (at >= base + units_of(a, s, whole)) {
             if (b + 1 >= a.batch) return false;
-            base += units_of(a, s);
+            base += units_of(a, s, whole);
             s = sequence<RT>(a, ++b);
         }
         const int off = at - base;
-        const int per = a.parts ? s.tiles : 1;
+        const int per = whole ? 1 : s.tiles;
         const int hr = off / per;
         g.b = b;
         g.h = hr / s.row_tiles;
@@ -89,7 +155,7 @@ struct Walk {
         g.t0 = off % per;
         const int take = min(per - g.t0, end - at);
         g.whole = take == per;
-        g.t1 = a.parts ? g.t0 + take : s.tiles;
+        g.t1 = whole ? s.tiles : g.t0 + take;
         at += take;
         g.len = s.len;
         g.count = s.count;
@@ -142,6 +208,6 @@ __device__ __forceinline__ float log2_vs(float vs) {
 // The kernel for many rows (kz_cache_attention_tc.cu): tiles of kTcRows rows,
 // one CTA a SM.
 constexpr int kTcRows = 128;
-int launch_cache_attention_tc(const CacheAttArgs& a, int d, int grid, cudaStream_t s);
+int launch_cache_attention_tc(const CacheAttArgs& a, int d, cudaStream_t s);
 
 }  // namespace kz

@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
     __shared__ float s_top[2][2][kTcRows], s_l[2][kTcRows];      // exchanged between a row's two threads
     __shared__ uint32_t s_sees[kTcRows][kTreeWords];
     __shared__ int32_t s_parent[KZ_TREE_MAX_NODES];
-    __shared__ int s_sum[4], s_part[128], s_start[2], s_units[2];
+    __shared__ RangeShared s_range;
     __shared__ int s_abort;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // uniform: so are the roles' branches
@@ -213,43 +213,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
     }
     griddep_wait();
 
-    // ---- this CTA's units, and where they begin
-    if (warp < 4) {
-        const int each = (a.batch + 127) / 128;
-        int mine = 0;
-        for (int b = tid * each; b < min(a.batch, (tid + 1) * each); ++b) mine += units_of(a, sequence<kTcRows>(a, b));
-        s_part[tid] = mine;
-        const int total = sum_128(mine, s_sum);
-        if (tid == 0) {
-            const int per = units_a_cta(a, total, gridDim.x);
-            const int u0 = (int)min((int64_t)total, (int64_t)per * blockIdx.x), u1 = (int)min((int64_t)total, (int64_t)u0 + per);
-            s_units[0] = u0;
-            s_units[1] = u1;
-            int base = 0, i = 0, b = 0;
-            if (u0 < u1) {
-                while (i < 127 && base + s_part[i] <= u0) base += s_part[i++];
-                b = i * each;
-                for (; b < a.batch - 1; ++b) {
-                    const int n = units_of(a, sequence<kTcRows>(a, b));
-                    if (u0 < base + n) break;
-                    base += n;
-                }
-            }
-            s_start[0] = b;
-            s_start[1] = base;
-        }
-    }
+    if (warp < 4) find_range<kTcRows>(a, s_range);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     griddep_launch_dependents();           // not before this CTA has its tensor memory: a dependent may take some
     constexpr uint32_t tmem = 0;           // where all 512 columns begin
-    Walk<kTcRows> walk;
-    walk.at = s_units[0];
-    walk.end = s_units[1];
-    walk.b = s_start[0];
-    walk.base = s_start[1];
-    if (walk.at < walk.end) walk.s = sequence<kTcRows>(a, walk.b);
+    Walk<kTcRows> walk(a, s_range.range);
     Segment g;
     // bounded as mbar_wait is, with fewer registers
     auto wait = [&](uint64_t& bar, int phase, int sleep = 0) {
@@ -672,7 +642,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
 }
 
 template <int D>
-int launch(const CacheAttArgs& a, int grid, cudaStream_t s) {
+int launch(const CacheAttArgs& a, cudaStream_t s) {
     static std::atomic<int> attr_set[64];
     int dev = 0;
     KZ_CHECK_CUDA(cudaGetDevice(&dev));
@@ -681,14 +651,14 @@ int launch(const CacheAttArgs& a, int grid, cudaStream_t s) {
                                            Tc<D>::SMEM));
         if (dev >= 0 && dev < 64) attr_set[dev] = 1;
     }
-    KZ_CHECK_CUDA(launch_pdl(cache_attention_tc_kernel<D>, dim3(grid), dim3(kTcThreads), Tc<D>::SMEM, s, a));
+    KZ_CHECK_CUDA(launch_pdl(cache_attention_tc_kernel<D>, dim3(a.ctas), dim3(kTcThreads), Tc<D>::SMEM, s, a));
     return KZ_OK;
 }
 
 }  // namespace
 
-int launch_cache_attention_tc(const CacheAttArgs& a, int d, int grid, cudaStream_t s) {
-    return d == 32 ? launch<32>(a, grid, s) : d == 64 ? launch<64>(a, grid, s) : launch<128>(a, grid, s);
+int launch_cache_attention_tc(const CacheAttArgs& a, int d, cudaStream_t s) {
+    return d == 32 ? launch<32>(a, s) : d == 64 ? launch<64>(a, s) : launch<128>(a, s);
 }
 
 }  // namespace kz
