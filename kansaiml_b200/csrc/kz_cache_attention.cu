@@ -483,23 +483,46 @@ __global__ void __launch_bounds__(kCaThreads, 2)
 
 // Joins the parts of a (sequence, head, row tile) that several CTAs left: with
 // M the largest of their maxima, o = sum f_c o_c / sum f_c l_c, f_c =
-// 2^(m_c - M).  Latency bounds it (a row's parts are far apart), so a block has
-// few rows, a lane D / 32 of a row's values.  FEW: up to four parts are a
-// warp's work, and a block has four rows and four warps.  Otherwise (more
-// CTAs than four a row tile: few, long sequences) a block has one row, dealt
-// out part by part to eight warps, each with a maximum of its own, and joined
-// once more.  One sequence of 30000 keys, 35 parts a row: 31 us in all with
-// the first, 23 with the second; 32 sequences of 4096 to 8191: 78 and 81.
+// 2^(m_c - M).  Latency bounds it (a row's parts are far apart), so a lane has D /
+// 32 neighbouring values of a row, one load each.  FEW: up to four parts are a
+// warp's work, every load of two rows in flight at once, and a block has eight
+// rows and four warps.  Otherwise (more CTAs than four a row tile: few, long
+// sequences) a block has one row, dealt out part by part to eight warps, each
+// with a maximum of its own, and joined once more.  One sequence of 30000 keys,
+// 35 parts a row: 31 us in all with the first, 23 with the second; 32 sequences
+// of 4096 to 8191: 78 and 81.
 template <bool FEW>
 struct Join {
-    static constexpr int ROWS = FEW ? 4 : 1, WARPS = FEW ? 4 : 8;
+    static constexpr int ROWS = FEW ? 8 : 1, WARPS = FEW ? 4 : 8;
 };
+template <int E>
+__device__ __forceinline__ void load_values(const float* p, float (&v)[E]) {
+    if constexpr (E == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else if constexpr (E == 2) {
+        const float2 x = *reinterpret_cast<const float2*>(p);
+        v[0] = x.x, v[1] = x.y;
+    } else {
+        v[0] = *p;
+    }
+}
+template <int E>
+__device__ __forceinline__ void store_values(float* p, const float (&v)[E]) {
+    if constexpr (E == 4)
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else if constexpr (E == 2)
+        *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+    else
+        *p = v[0];
+}
 template <int D, int RT, bool FEW>
 __global__ void __launch_bounds__(32 * Join<FEW>::WARPS) cache_attention_join_kernel(const CacheAttArgs a) {
     constexpr int E = D / 32, SLOT = RT * (D + 2), ROWS = Join<FEW>::ROWS, WARPS = Join<FEW>::WARPS, BLOCKS = RT / ROWS;
     __shared__ Work s_work[WARPS];
     __shared__ int s_before[WARPS];
-    __shared__ float s_part[WARPS][ROWS][D], s_m[WARPS][ROWS], s_l[WARPS][ROWS];
+    __shared__ __align__(16) float s_part[WARPS][ROWS][D];
+    __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS];
     griddep_launch_dependents();
     const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // lengths and counts were written before the kernel that left the parts began
@@ -534,64 +557,89 @@ __global__ void __launch_bounds__(32 * Join<FEW>::WARPS) cache_attention_join_ke
     auto slot = [&](int c) {                                    // a CTA's first part is in its first slot
         return a.parts + (2 * (int64_t)c + (c > c0 || c0 * per == u0 ? 0 : 1)) * SLOT;
     };
-    // the sums of row r over the parts first, first + step, ...
-    auto gather = [&](int r, int first, int step, float& M, float& L, float (&o)[E]) {
-        M = -INFINITY;
-        L = 0.0f;
-        for (int c = first + step * lane; c <= c1; c += 32 * step) M = fmaxf(M, slot(c)[RT * D + r]);
+    auto finish = [&](int r, float L, float (&o)[E]) {
+        const float f = L == 0.0f ? 0.0f : 1.0f / L;
+        const int R = rt * RT + r;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] *= f;
+        store_values(a.out + ((int64_t)b * a.tokens + R / a.group) * a.heads * D + ((int64_t)h * a.group + R % a.group) * D + lane * E, o);
+    };
+    if (c1 - c0 < 4) {
+        for (int i = warp; i < min(rows, ROWS); i += 2 * WARPS) {
+            float m[2][4], l[2][4], v[2][4][E];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int r = r0 + i + k * WARPS;
+                    const bool there = c <= c1 - c0 && i + k * WARPS < min(rows, ROWS);
+                    const float* p = slot(there ? c0 + c : c0);
+                    m[k][c] = there ? p[RT * D + r] : -INFINITY;
+                    l[k][c] = there ? p[RT * D + RT + r] : 0.0f;
+                    if (there) load_values(p + r * D + lane * E, v[k][c]);
+                }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (i + k * WARPS >= min(rows, ROWS)) break;
+                const float M = fmaxf(fmaxf(m[k][0], m[k][1]), fmaxf(m[k][2], m[k][3]));
+                float L = 0.0f, o[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (c > c1 - c0) break;
+                    const float f = shrink(m[k][c], M);
+                    L = fmaf(l[k][c], f, L);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[e] = fmaf(v[k][c][e], f, o[e]);
+                }
+                finish(r0 + i + k * WARPS, L, o);
+            }
+        }
+        return;
+    }
+    for (int i = 0; i < min(rows, ROWS); ++i) {
+        // a warp's parts: c0 + warp, c0 + warp + WARPS, ...
+        const int r = r0 + i;
+        float M = -INFINITY, L = 0.0f, o[E];
+        for (int c = c0 + warp + WARPS * lane; c <= c1; c += 32 * WARPS) M = fmaxf(M, slot(c)[RT * D + r]);
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = 0.0f;
 #pragma unroll 8
-        for (int c = first; c <= c1; c += step) {
+        for (int c = c0 + warp; c <= c1; c += WARPS) {
             const float* p = slot(c);
             const float f = shrink(p[RT * D + r], M);
             L = fmaf(p[RT * D + RT + r], f, L);
+            float v[E];
+            load_values(p + r * D + lane * E, v);
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(p[r * D + lane + 32 * e], f, o[e]);
+            for (int e = 0; e < E; ++e) o[e] = fmaf(v[e], f, o[e]);
         }
-    };
-    auto finish = [&](int r, float L, const float (&o)[E]) {
-        const float f = L == 0.0f ? 0.0f : 1.0f / L;
-        const int R = rt * RT + r;
-        float* dst = a.out + ((int64_t)b * a.tokens + R / a.group) * a.heads * D + ((int64_t)h * a.group + R % a.group) * D;
-#pragma unroll
-        for (int e = 0; e < E; ++e) dst[lane + 32 * e] = o[e] * f;
-    };
-    float M, L, o[E];
-    if (c1 - c0 < 4) {
-        if (warp < min(rows, ROWS)) {
-            gather(r0 + warp, c0, 1, M, L, o);
-            finish(r0 + warp, L, o);
-        }
-        return;
-    }
-    for (int i = 0; i < min(rows, ROWS); ++i) {
-        gather(r0 + i, c0 + warp, WARPS, M, L, o);
-#pragma unroll
-        for (int e = 0; e < E; ++e) s_part[warp][i][lane + 32 * e] = o[e];
+        store_values(&s_part[warp][i][lane * E], o);
         if (lane == 0) {
             s_m[warp][i] = M;
             s_l[warp][i] = L;
         }
     }
     __syncthreads();
-    if (warp < min(rows, ROWS)) {
-        M = -INFINITY;
-        L = 0.0f;
+    for (int i = warp; i < min(rows, ROWS); i += WARPS) {
+        float M = -INFINITY, L = 0.0f, o[E];
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w][warp]);
+        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w][i]);
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = 0.0f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            const float f = shrink(s_m[w][warp], M);
-            L = fmaf(s_l[w][warp], f, L);
+            const float f = shrink(s_m[w][i], M);
+            L = fmaf(s_l[w][i], f, L);
+            float v[E];
+            load_values(&s_part[w][i][lane * E], v);
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(s_part[w][warp][lane + 32 * e], f, o[e]);
+            for (int e = 0; e < E; ++e) o[e] = fmaf(v[e], f, o[e]);
         }
-        finish(r0 + warp, L, o);
+        finish(r0 + i, L, o);
     }
 }
 
