@@ -9,7 +9,7 @@
 namespace kz {
 
 constexpr int kKT = 128;                    // keys a tile
-constexpr int kJoinTiles = 5;               // what ranges that end inside a row tile cost, in tiles (see whole_ranges)
+constexpr int kTcRows = 128;                // rows a tile of the kernel for many rows has
 constexpr int kTreeWords = KZ_TREE_MAX_NODES / 32;
 
 struct CacheAttArgs {
@@ -65,12 +65,21 @@ struct Work {
         tiles = __reduce_max_sync(0xffffffffu, tiles);
     }
 };
-// Whether each CTA takes whole row tiles (a unit of work is then a row tile, not
-// a tile of keys): where the most that one would do that way is not more than in
-// equal ranges, whose CTAs begin and end inside row tiles and need the join.
+// The units of each CTA, all having as many.
 __device__ __forceinline__ int a_cta(const CacheAttArgs& a, int units) { return units > 0 ? div_by(units - 1, a.by_ctas) + 1 : 0; }
+
+// Whether each CTA takes whole row tiles (a unit of work is then a row tile, not
+// a tile of keys): where the most tiles that one would do that way are not more
+// than in equal ranges, whose CTAs begin and end inside row tiles and leave parts
+// to be joined, at the time of about three tiles.
+// Measured whole / in ranges, up to 500, 700, 1000 and 2000 keys in 8 key heads
+// of 128: single tokens of one sequence 10.0 / 9.0, 11.8 / 8.9, 14.2 / 8.6 and
+// 21.5 / 9.7 us; of 8, 12.4 / 10.9, 14.6 / 10.4, 17.8 / 12.9 us; of 32, 12.9 /
+// 16.2, -, 19.1 / 22.7, 31.0 / 31.3 us; of 64 (700) 27.2 / 30.4 us; chunks of 20
+// tokens (80 rows) of one sequence 22.3 / 16.6, 24.1 / 16.6, 28.5 / 17.0 us, of
+// 8 22.7 / 24.5, -, 28.9 / 26.4, of 16 24.2 / 33, -, 31 / 39, 47.7 / 50.2 us.
 __device__ __forceinline__ bool whole_ranges(const CacheAttArgs& a, const Work& w) {
-    return !a.parts || (int64_t)a_cta(a, w.row_tiles) * w.tiles <= (int64_t)a_cta(a, w.units) + kJoinTiles;
+    return !a.parts || (int64_t)a_cta(a, w.row_tiles) * w.tiles <= (int64_t)a_cta(a, w.units) + 3;
 }
 __device__ __forceinline__ int units_of(const CacheAttArgs& a, const Seq& s, bool whole) {
     return s.row_tiles * a.c.heads * (whole ? 1 : s.tiles);
@@ -205,9 +214,7 @@ __device__ __forceinline__ float log2_vs(float vs) {
     return r != r ? r : fminf(fmaxf(r, -100.0f), 100.0f);
 }
 
-// The kernel for many rows (kz_cache_attention_tc.cu): tiles of kTcRows rows,
-// one CTA a SM.
-constexpr int kTcRows = 128;
+// The kernel for many rows (kz_cache_attention_tc.cu): one CTA a SM.
 int launch_cache_attention_tc(const CacheAttArgs& a, int d, cudaStream_t s);
 
 }  // namespace kz

@@ -400,6 +400,26 @@ def test_attention_is_repeatable(cuda_device, tokens, heads):
         assert _check_attention(book, lengths, None, tokens, heads).tobytes() == a.tobytes()
 
 
+@pytest.mark.parametrize("d,kv,heads,tokens,spans", [
+    (64, 2, 8, 1, [(40, 600)]), (128, 3, 3, 1, [(1, 1500)]), (32, 1, 4, 2, [(5, 5), (1, 900), (30, 140)]),
+    (64, 2, 16, 20, [(1, 1200), (1, 50)]), (32, 4, 16, 20, [(40, 300)]), (128, 1, 8, 17, [(3, 2400), (20, 130)]),
+    (64, 2, 8, 1, [(600, 9)]), (64, 1, 1, 3, [(7, 0)])])
+def test_attention_in_a_table_wider_than_its_sequences(cuda_device, d, kv, heads, tokens, spans):
+    """The table has room for far more than the sequences hold, so how the keys
+    are dealt out follows from the lengths: few and many sequences, short and
+    long ones together, rows without tokens, and no tokens at all."""
+    rs = np.random.RandomState(tokens * d)
+    most = [n for many, n in spans for _ in range(many)]
+    counts = [int(rs.randint(0, tokens + 1)) if n else 0 for n in most]
+    counts[0] = tokens if most[0] else 0
+    lengths = [int(rs.randint(n // 2, n + 1)) for n in most]
+    book = Book([a + b for a, b in zip(lengths, counts)], kv, d, 16)
+    wide = torch.full((len(most), 300), -1, dtype=torch.int32, device="cuda")
+    wide[:, :book.table.shape[1]] = book.table
+    book.table = wide
+    _check_attention(book, lengths, counts, tokens, heads)
+
+
 def test_attention_many_sequences(cuda_device):
     """More sequences than a block has threads, most of them without tokens."""
     rs = np.random.RandomState(2)
