@@ -15,9 +15,12 @@
 // q is scaled by a power of two per row so that its largest value lies in
 // [2^13, 2^14), and the softmax's exponent is measured from the row's running
 // maximum of s + log2(vs), which puts its largest w * vs there too, so that no
-// half is lost to fp16's range.  Sums are 32-bit; the tensor core's sum of a step of keys is added to
-// the row's sum by an fp32 multiply-add that also carries the softmax's
-// rescaling, so that long contexts do not add up its truncation.
+// half is lost to fp16's range (what is below 2^-38 of a row's largest is).
+// Sums are 32-bit; the tensor core's sum of a step of keys is added to the row's
+// sum by an fp32 multiply-add that also carries the softmax's rescaling, so that
+// long contexts do not add up its truncation.  The small halves' products are
+// summed first, or on their own, where the truncation costs least: 0.6e-6 of the
+// output's size instead of 1.1e-6 at 8000 keys.
 //
 // Work.  The rows of one key head (its `group` query heads times the new
 // tokens) form tiles of RT rows.  S^T = K Q^T and O^T = V^T P^T put the keys
@@ -32,7 +35,14 @@
 // The keys of all sequences are cut into equal ranges, one per CTA, two CTAs
 // a SM, so that ragged batches and long single sequences fill the GPU alike; a
 // (sequence, head, row tile) that spans several ranges leaves its parts in the
-// workspace, and a second kernel joins them.
+// workspace, and a second kernel joins them.  Where that costs more than it
+// gives (whole_ranges) each CTA takes whole row tiles instead.
+//
+// Measured, join included: 32 sequences of 4096 to 8191 keys, 32 heads over 8 key
+// heads of 128, one new token each (416 MB of cache): 76 us = 5.5 TB/s, 0.84 of a
+// plain copy; HBM bounds it but for about 7 us at the start and the join.  32
+// sequences of up to 255 keys, 4 heads of 64: 7.3 us, latency (lengths, table,
+// page, one after another, then a tile's chain).  One sequence of 30000: 23 us.
 #include <algorithm>
 #include <atomic>
 
@@ -488,9 +498,10 @@ __global__ void __launch_bounds__(kCaThreads, 2)
 // warp's work, every load of two rows in flight at once, and a block has eight
 // rows and four warps.  Otherwise (more CTAs than four a row tile: few, long
 // sequences) a block has one row, dealt out part by part to eight warps, each
-// with a maximum of its own, and joined once more.  One sequence of 30000 keys,
-// 35 parts a row: 31 us in all with the first, 23 with the second; 32 sequences
-// of 4096 to 8191: 78 and 81.
+// with a maximum of its own, and joined once more.  The attention with the first
+// and the second: one sequence of 30000 keys (35 parts a row) 31 and 23 us; 32
+// sequences of 4096 to 8191 76 and 80; 2 chunks of 500 tokens, 4 rows a token, 150
+// and 188.
 template <bool FEW>
 struct Join {
     static constexpr int ROWS = FEW ? 8 : 1, WARPS = FEW ? 4 : 8;
@@ -659,7 +670,9 @@ int launch_join(const CacheAttArgs& a, int64_t row_tiles, cudaStream_t s) {
 
 // ---------------------------------------------------------------- launches
 
-// Rows of a tile: the smallest of 8, 16 and 32 that holds a key head's rows.
+// Rows of a tile: the smallest of 8, 16 and 32 that holds a key head's rows.  With
+// tiles of 8, 16 and 32, 4 rows over 32 long sequences: 78, 110 and 197 us; 16
+// rows, 16 sequences of 3000 to 6000: 51 us with 16, 84 with 32.
 int tile_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
 
 // Whether a call needs no workspace and no join: its table holds no more than
@@ -669,8 +682,9 @@ bool short_table(int64_t cols, int64_t page) { return cols * page <= 4 * kKT; }
 
 // Whether the rows of a key head are many enough for the tcgen05 kernel, whose
 // time does not depend on them up to 128: at 32 rows (batch 16, 8 key heads of
-// 128, contexts of 1500 and 6000) it takes 45 and 87 us against 37 and 87 here,
-// at 64 rows 51 and 98 against 58 and 150 with tiles of 64 rows.
+// 128, contexts of 1500 and 6000) it takes 36.6 and 85.6 us against 36.8 and 86.2
+// here, with heads of 64 (20 rows, 32 contexts of 5000) 124 against 87; at 64
+// rows of heads of 128 51 and 98 against 58 and 150 with tiles of 64 rows.
 bool many_rows(int64_t rows) { return rows > 32; }
 
 int64_t parts_floats(int64_t rows, int64_t d) {

@@ -11,8 +11,19 @@
 // N-major for the second.  Warps 0-7: softmax, two threads a row (64 keys of
 // each tile, and half of the row's sums in registers, to which each tile's O is
 // added); 8-11 convert the next tiles; 12 issues the MMAs, 13 loads the pages
-// (bulk copies), 14 and 15 zero the padding's rows.  The MMAs of tile t + 1's scores run while tile t's softmax
-// does, so the tensor cores wait only where a row tile ends.
+// (bulk copies), 14 and 15 zero the padding's rows.  The MMAs of tile t + 1's
+// scores run while tile t's softmax does.
+//
+// Measured, join included: 2 chunks of 500 tokens over 8192 keys, 16 heads over 4
+// key heads of 128: 150 us = 920 TFLOP/s over both halves, 0.56 of the tensor
+// cores' measured rate; trees of 24 tokens (96 rows) over 8 contexts of 2500 to
+// 5000, 8 key heads of 128: 51 us.  What bounds it is the softmax's chain: a tile takes
+// about 3900 cycles, of which the MMAs are 2050 and the exponentials 1024; with
+// neither MMAs nor conversions four fifths of the time remain.  A row a thread
+// with the two warpgroups on alternate tiles took 207 us instead of 157 (S is read
+// twice from tensor memory, at 128 bytes a cycle), joining O between the weights'
+// steps 165 (spills), sums in the converters' warps 192, O kept in tensor memory
+// over 2 or 4 tiles with a CTA-wide vote on rescaling 169 to 172.
 //
 // Tensor memory (512 columns): Q halves 0..d-1, S / P of even tiles 128..255,
 // of odd tiles 256..383, O 384..383+d.  One CTA a SM.
@@ -451,115 +462,115 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
                         arrive(s_p_full[it & 1]);
                     }
                 } else {
-                const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(factors + 3 * (it & 3) * kKT + 64 * half);
-                const ulonglong2 *vs = ks + kKT / 4, *lv = vs + kKT / 4;     // pairs of fp32 values
-                const uint32_t s_at = tmem + lanes + kTmS + (it & 1) * 128 + 64 * half;
-                wait(s_s_full[it & 1], it >> 1);
-                tc_fence_after();
-                const uint32_t bad = s_bad[it & 3];
-                // whether a row of the tile does not see one of the keys
-                const bool masked = t * kKT + kKT > g.len + (a.parents ? 0 : g.first_token + 1) || bad;
-                // the keys of chunk c (32 keys) that this row sees, a bit each
-                auto seen = [&](int c) {
-                    const int first = t * kKT + 32 * c - g.len;      // the chunk's place among the new tokens
-                    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
-                    if (!is_row) return 0u;
-                    uint32_t s;
-                    if (a.parents) {
-                        const uint32_t* mine = s_sees[token - g.first_token];
-                        s = below(-first);
-                        if (first > -32 && first < 0) s |= mine[0] << -first;
-                        if (first >= 0 && first < KZ_TREE_MAX_NODES) {
-                            const int i = first >> 5;
-                            s = mine[i] >> (first & 31);
-                            if ((first & 31) && i + 1 < kTreeWords) s |= mine[i + 1] << (32 - (first & 31));
+                    const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(factors + 3 * (it & 3) * kKT + 64 * half);
+                    const ulonglong2 *vs = ks + kKT / 4, *lv = vs + kKT / 4;     // pairs of fp32 values
+                    const uint32_t s_at = tmem + lanes + kTmS + (it & 1) * 128 + 64 * half;
+                    wait(s_s_full[it & 1], it >> 1);
+                    tc_fence_after();
+                    const uint32_t bad = s_bad[it & 3];
+                    // whether a row of the tile does not see one of the keys
+                    const bool masked = t * kKT + kKT > g.len + (a.parents ? 0 : g.first_token + 1) || bad;
+                    // the keys of chunk c (32 keys) that this row sees, a bit each
+                    auto seen = [&](int c) {
+                        const int first = t * kKT + 32 * c - g.len;      // the chunk's place among the new tokens
+                        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
+                        if (!is_row) return 0u;
+                        uint32_t s;
+                        if (a.parents) {
+                            const uint32_t* mine = s_sees[token - g.first_token];
+                            s = below(-first);
+                            if (first > -32 && first < 0) s |= mine[0] << -first;
+                            if (first >= 0 && first < KZ_TREE_MAX_NODES) {
+                                const int i = first >> 5;
+                                s = mine[i] >> (first & 31);
+                                if ((first & 31) && i + 1 < kTreeWords) s |= mine[i + 1] << (32 - (first & 31));
+                            }
+                        } else {
+                            s = below(token + 1 - first);
                         }
-                    } else {
-                        s = below(token + 1 - first);
-                    }
-                    for (uint32_t left = bad; left; left &= left - 1) {
-                        const int p0 = ((__ffs(left) - 1) << a.c.shift) - 32 * c;   // a missing page's keys
-                        s &= ~(below(p0 + a.c.page) & ~below(p0));
-                    }
-                    return s;
-                };
-                uint64_t z[32];                      // s * ks
-                {
-                    uint32_t r[2][32];
-                    tmem_ld_32x32b_x32(s_at, r[0]);
-                    tmem_ld_32x32b_x32(s_at + 32, r[1]);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const ulonglong2 f = ks[j];
-                        const int c = j >> 3, i = (4 * j) & 31;
-                        z[2 * j] = mul2(bits_pair(r[c][i], r[c][i + 1]), f.x);
-                        z[2 * j + 1] = mul2(bits_pair(r[c][i + 2], r[c][i + 3]), f.y);
-                    }
-                }
-                if (masked) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const uint32_t sees = seen(2 * half + c);
+                        for (uint32_t left = bad; left; left &= left - 1) {
+                            const int p0 = ((__ffs(left) - 1) << a.c.shift) - 32 * c;   // a missing page's keys
+                            s &= ~(below(p0 + a.c.page) & ~below(p0));
+                        }
+                        return s;
+                    };
+                    uint64_t z[32];                      // s * ks
+                    {
+                        uint32_t r[2][32];
+                        tmem_ld_32x32b_x32(s_at, r[0]);
+                        tmem_ld_32x32b_x32(s_at + 32, r[1]);
+                        tc_wait_ld();
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            float x0, x1;
-                            unpair(z[16 * c + j], x0, x1);
-                            if (!((sees >> (2 * j)) & 1u)) x0 = -INFINITY;
-                            if (!((sees >> (2 * j + 1)) & 1u)) x1 = -INFINITY;
-                            z[16 * c + j] = pair(x0, x1);
+                            const ulonglong2 f = ks[j];
+                            const int c = j >> 3, i = (4 * j) & 31;
+                            z[2 * j] = mul2(bits_pair(r[c][i], r[c][i + 1]), f.x);
+                            z[2 * j + 1] = mul2(bits_pair(r[c][i + 2], r[c][i + 3]), f.y);
                         }
                     }
-                }
-                float top[4] = {m, m, m, m};         // the largest of s + log2 vs
+                    if (masked) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const ulonglong2 e = lv[j];
-                    float x[4];
-                    unpair(fma2(z[2 * j], unit2, e.x), x[0], x[1]);
-                    unpair(fma2(z[2 * j + 1], unit2, e.y), x[2], x[3]);
+                        for (int c = 0; c < 2; ++c) {
+                            const uint32_t sees = seen(2 * half + c);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], x[k]);
-                }
-                float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                s_top[it & 1][half][row] = m_new;
-                meet_pair();
-                m_new = fmaxf(m_new, s_top[it & 1][half ^ 1][row]);
-                const float ref = m_new == -INFINITY ? 0.0f : kLift - m_new;
-                const uint64_t ref2 = pair(ref, ref);
-                uint64_t sum[2] = {0, 0};
-                // the weights, and their halves times vs over each 32 keys' own columns of S (16 of
-                // leading halves, 16 of the rest)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t hi[8], lo[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float p0, p1;
-                        unpair(fma2(z[8 * c + j], unit2, ref2), p0, p1);
-                        const uint64_t p = pair(exp2_approx(p0), exp2_approx(p1));
-                        const ulonglong2 f = vs[4 * c + (j >> 1)];
-                        sum[j & 1] = add2(sum[j & 1], p);
-                        const uint64_t w = mul2(p, j & 1 ? f.y : f.x);
-                        unpair(w, p0, p1);
-                        const float h0 = leading(p0), h1 = leading(p1);
-                        float l0, l1;
-                        unpair(sub2(w, pair(h0, h1)), l0, l1);
-                        hi[j] = half2_bits(h0, h1);
-                        lo[j] = half2_bits(l0, l1);
+                            for (int j = 0; j < 16; ++j) {
+                                float x0, x1;
+                                unpair(z[16 * c + j], x0, x1);
+                                if (!((sees >> (2 * j)) & 1u)) x0 = -INFINITY;
+                                if (!((sees >> (2 * j + 1)) & 1u)) x1 = -INFINITY;
+                                z[16 * c + j] = pair(x0, x1);
+                            }
+                        }
                     }
-                    tmem_st_32x32b_x8(s_at + 32 * (c >> 1) + 8 * (c & 1), hi);
-                    tmem_st_32x32b_x8(s_at + 32 * (c >> 1) + 16 + 8 * (c & 1), lo);
-                }
-                const float corr_new = shrink(m, m_new);
-                m = m_new;
-                float s0, s1;
-                unpair(add2(sum[0], sum[1]), s0, s1);
-                l = fmaf(l, corr_new, s0 + s1);
-                tc_wait_st();
-                tc_fence_before();
-                arrive(s_p_full[it & 1]);
-                corr_next = corr_new;
+                    float top[4] = {m, m, m, m};         // the largest of s + log2 vs
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const ulonglong2 e = lv[j];
+                        float x[4];
+                        unpair(fma2(z[2 * j], unit2, e.x), x[0], x[1]);
+                        unpair(fma2(z[2 * j + 1], unit2, e.y), x[2], x[3]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], x[k]);
+                    }
+                    float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    s_top[it & 1][half][row] = m_new;
+                    meet_pair();
+                    m_new = fmaxf(m_new, s_top[it & 1][half ^ 1][row]);
+                    const float ref = m_new == -INFINITY ? 0.0f : kLift - m_new;
+                    const uint64_t ref2 = pair(ref, ref);
+                    uint64_t sum[2] = {0, 0};
+                    // the weights, and their halves times vs over each 32 keys' own columns of S (16 of
+                    // leading halves, 16 of the rest)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            float p0, p1;
+                            unpair(fma2(z[8 * c + j], unit2, ref2), p0, p1);
+                            const uint64_t p = pair(exp2_approx(p0), exp2_approx(p1));
+                            const ulonglong2 f = vs[4 * c + (j >> 1)];
+                            sum[j & 1] = add2(sum[j & 1], p);
+                            const uint64_t w = mul2(p, j & 1 ? f.y : f.x);
+                            unpair(w, p0, p1);
+                            const float h0 = leading(p0), h1 = leading(p1);
+                            float l0, l1;
+                            unpair(sub2(w, pair(h0, h1)), l0, l1);
+                            hi[j] = half2_bits(h0, h1);
+                            lo[j] = half2_bits(l0, l1);
+                        }
+                        tmem_st_32x32b_x8(s_at + 32 * (c >> 1) + 8 * (c & 1), hi);
+                        tmem_st_32x32b_x8(s_at + 32 * (c >> 1) + 16 + 8 * (c & 1), lo);
+                    }
+                    const float corr_new = shrink(m, m_new);
+                    m = m_new;
+                    float s0, s1;
+                    unpair(add2(sum[0], sum[1]), s0, s1);
+                    l = fmaf(l, corr_new, s0 + s1);
+                    tc_wait_st();
+                    tc_fence_before();
+                    arrive(s_p_full[it & 1]);
+                    corr_next = corr_new;
                 }
                 if (t > g.t0) {
                     wait(s_o_full, it - 1);

@@ -25,8 +25,15 @@
 // ends with it, its sums are those that the last token is drawn by.  Without
 // one r is p with the rejected tokens taken out, over what is left: one pass
 // over a node's row gives its sum, from which each rejected token's p is
-// subtracted.  Nothing else of the probabilities is touched.  What bounds it is latency, so a warp loads all of
-// its part of a slice (8 chunks, 128 values of each at a time) before it adds anything up.
+// subtracted.  Nothing else of the probabilities is touched.  What bounds it is
+// latency -- a pass, a meeting, the walk, for each rejection -- so a warp loads
+// all of its part of a slice (8 chunks, 128 values of each at a time) before it
+// adds anything up.
+//
+// Measured: 32 trees of 16 nodes over 128000 tokens with a draft, 30 us (32.8 MB
+// of rows once: 5 us); with clusters of 4 42 us, with blocks of 128 threads 40,
+// with every sum in double 32.  32 trees of 6 nodes over 65 tokens, no draft:
+// 10.4 us (11.5 with every sum in double).
 #include <math.h>
 
 #include <algorithm>
@@ -442,7 +449,7 @@ extern "C" int kz_verify_tree_f32(const int64_t* tokens, const int32_t* parents,
     a.vocab = (int)vocab;
     a.status = device_status_ptr();
     // a cluster for each sequence: the CTAs it takes to have 128 values a warp's chunk, 8 at most; a small
-    // vocabulary is one CTA of four warps
+    // vocabulary is one CTA of four warps (65 tokens: 10.4 us, with eight warps 10.6)
     const int threads = vocab <= 4 * kVChunks * 128 ? 128 : kVThreads, warps = threads / 32;
     int ranks = 1;
     while (ranks < kVMaxCluster && vocab > (int64_t)ranks * warps * kVChunks * 128) ranks *= 2;
