@@ -315,7 +315,9 @@ int kz_gemm_i8_allgather(const int8_t* A, int8_t* const* peer_A, uint32_t* const
  * own: scale = max|x| / 127 in double (1 for zeros), codes rounded half to
  * even; fl32(scale) is kept, and a cached value stands for
  * fl32(code * fl32(scale)).  A row with NaN/Inf keeps codes 0 and scale NaN
- * and sets KZ_ERR_NONFINITE. */
+ * and sets KZ_ERR_NONFINITE.  Several sequences may read a page; a page that a
+ * call writes (kz_cache_write_f32, kz_cache_keep) must be in the table once.
+ * Outputs must not overlap inputs. */
 typedef struct kz_cache {
     int8_t* k_codes;
     float* k_scale;
@@ -360,7 +362,10 @@ int kz_cache_keep(const kz_cache* cache, const int32_t* table, int64_t table_col
  * every one up to itself.  out [batch, tokens, heads * head_dim] contiguous;
  * rows past counts[b], and rows that see no key, are 0.  batch < 65536.
  * `workspace` (16-byte aligned device memory, scratch of this call alone) must
- * hold kz_cache_attention_workspace_bytes(...) bytes, 0 for short tables. */
+ * hold kz_cache_attention_workspace_bytes(...) bytes, 0 for short tables.  The
+ * products keep 22 bits of q and of each weight times V's scale, down to 2^-38
+ * of the row's largest; sums are 32-bit.  Scales are positive; a V scale counts
+ * as within 2^-100 .. 2^100 where the weights are brought into range. */
 size_t kz_cache_attention_workspace_bytes(const kz_cache* cache, int64_t tokens, int64_t heads, int64_t table_cols);
 int kz_cache_attention_f32(const kz_cache* cache, const float* q, int64_t batch, int64_t tokens, int64_t heads,
                            int64_t q_batch_stride, int64_t q_row_stride, const int32_t* table, int64_t table_cols,

@@ -23,6 +23,8 @@ token's parent in its tree (-1: none; a parent comes before its child).  All
 are CUDA tensors, read on the device: nothing here waits for the GPU.  A page
 number or position that a cache does not have is left out and recorded in the
 device status word (quantize.device_status), as NaN/Inf in a written row is.
+Sequences may share pages that are only read; a page that is written to must be
+in the table once.
 """
 import ctypes
 
