@@ -30,10 +30,11 @@
 // all of its part of a slice (8 chunks, 128 values of each at a time) before it
 // adds anything up.
 //
-// Measured: 32 trees of 16 nodes over 128000 tokens with a draft, 30 us (32.8 MB
-// of rows once: 5 us); with clusters of 4 42 us, with blocks of 128 threads 40,
-// with every sum in double 32.  32 trees of 6 nodes over 65 tokens, no draft:
-// 10.4 us (11.5 with every sum in double).
+// Measured: 32 trees of 16 nodes over 128000 tokens with a draft, 27 us (32.8 MB
+// of rows once: 5 us); 32 trees of 6 nodes over 65 tokens, no draft: 10.1 us.
+// Before the walk lost its divisions and the draw its serial sums (30 us) the
+// first took 42 us with clusters of 4, 40 with blocks of 128 threads and 32 with
+// every sum in double.
 #include <math.h>
 
 #include <algorithm>
@@ -88,12 +89,10 @@ __device__ __forceinline__ bool is_gone(const VerifyShared& s, int x) {
         if (s.gone[k] == x) return true;
     return false;
 }
-// r at node j's token, of its parent's row
-__device__ __forceinline__ double rest_at(const VerifyShared& s, bool has_draft, int j) {
-    const double p = s.p_at[j];
-    if (s.rejections == 0) return p;
-    if (!has_draft) return is_gone(s, s.token[j]) ? 0.0 : p / s.t;
-    return fmax(p - s.c * (double)s.q_at[j], 0.0) / s.t;
+// whether node j is accepted, u q < r at its token, of its parent's row (t times it: no division)
+__device__ __forceinline__ bool accepts(const VerifyShared& s, bool has_draft, int j) {
+    const double p = s.p_at[j], q = s.q_at[j], rest = has_draft ? fmax(p - s.c * q, 0.0) : is_gone(s, s.token[j]) ? 0.0 : p;
+    return (double)s.u[j] * q * s.t < rest;
 }
 // without a draft, the node's sum known: token of node j rejected
 __device__ __forceinline__ void take_out(VerifyShared& s, int j, double sum) {
@@ -225,8 +224,7 @@ __global__ void __launch_bounds__(kVThreads, 2) verify_tree_kernel(VerifyArgs a)
             int j = s.child;
             for (; j < a.nodes; ++j) {
                 if (s.parent[j] != s.node) continue;
-                const double r = rest_at(s, draft != nullptr, j);
-                if ((double)s.u[j] * (double)s.q_at[j] < r) {
+                if (accepts(s, draft != nullptr, j)) {
                     s.node = j;
                     s.rejections = 0;
                     s.c = 0.0;
@@ -342,9 +340,9 @@ __global__ void __launch_bounds__(kVThreads, 2) verify_tree_kernel(VerifyArgs a)
             __syncthreads();
             if (tid == 0)
                 for (int k = 0; k < s.rejections; ++k) {
-                    const int64_t c = s.gone[k] / a.chunk, of = (int64_t)warps * kVChunks;
+                    const int c = s.gone[k] / a.chunk, of = warps * kVChunks;
                     sums[c / of] -= s.gone_p[k];
-                    if (c / of == rank) s.chunk_sum[c % of / kVChunks][c % kVChunks] -= s.gone_p[k];
+                    if (c / of == (int)rank) s.chunk_sum[c % of / kVChunks][c % kVChunks] -= s.gone_p[k];
                 }
             __syncthreads();
         }
@@ -361,16 +359,28 @@ __global__ void __launch_bounds__(kVThreads, 2) verify_tree_kernel(VerifyArgs a)
         const bool past = slice < 0;                        // u * total at or past the total's rounding: the last value
         if (past) slice = last;
         if (slice == (int)rank && warp == 0) {
-            int part = -1, end = warps * kVChunks - 1;
-            double base = before;
-            for (int c = 0; c < warps * kVChunks && part < 0; ++c) {
-                const double t = s.chunk_sum[c / kVChunks][c % kVChunks];
-                if (t > 0.0) end = c;
-                if (!past && base + t > want) part = c;
-                if (part < 0) base += t;
+            // running sums over the slice's chunks, two a lane
+            static_assert(kVWarps * kVChunks <= 64, "two chunks a lane");
+            const int n = warps * kVChunks;
+            const double t0 = s.chunk_sum[lane / kVChunks][lane % kVChunks];
+            const double t1 = n > 32 ? s.chunk_sum[lane / kVChunks + 32 / kVChunks][lane % kVChunks] : 0.0;
+            double run0 = t0, run1 = t1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double v0 = __shfl_up_sync(0xffffffffu, run0, o), v1 = __shfl_up_sync(0xffffffffu, run1, o);
+                if (lane >= o) {
+                    run0 += v0;
+                    run1 += v1;
+                }
             }
-            const bool over = part < 0;
-            if (over) part = end;
+            const double first = before + __shfl_sync(0xffffffffu, run0, 31);
+            const unsigned hit0 = past ? 0u : __ballot_sync(0xffffffffu, before + run0 > want);
+            const unsigned hit1 = past ? 0u : __ballot_sync(0xffffffffu, n > 32 && first + run1 > want);
+            const unsigned some0 = __ballot_sync(0xffffffffu, t0 > 0.0), some1 = __ballot_sync(0xffffffffu, t1 > 0.0);
+            const bool over = !(hit0 | hit1);               // rounding: the last chunk that has anything
+            const int part = hit0 ? __ffs(hit0) - 1 : hit1 ? 31 + __ffs(hit1) : some1 ? 63 - __clz(some1) : some0 ? 31 - __clz(some0) : n - 1;
+            const double up0 = __shfl_sync(0xffffffffu, run0, (part - 1) & 31), up1 = __shfl_sync(0xffffffffu, run1, (part - 1) & 31);
+            double base = part == 0 ? before : part <= 32 ? before + up0 : first + up1;
             const int plo = (int)min((int64_t)a.vocab, (int64_t)slice0 + (int64_t)part * a.chunk);
             const int phi = (int)min((int64_t)a.vocab, (int64_t)plo + a.chunk);
             int token = -1, top = -1;                       // the answer; the last value above 0
