@@ -23,7 +23,8 @@
 // with the two warpgroups on alternate tiles took 207 us instead of 157 (S is read
 // twice from tensor memory, at 128 bytes a cycle), joining O between the weights'
 // steps 165 (spills), sums in the converters' warps 192, O kept in tensor memory
-// over 2 or 4 tiles with a CTA-wide vote on rescaling 169 to 172.
+// over 2 or 4 tiles with a CTA-wide vote on rescaling 169 to 172; four threads a
+// row 159 instead of 151 (at d = 64 the same).
 //
 // Tensor memory (512 columns): Q halves 0..d-1, S / P of even tiles 128..255,
 // of odd tiles 256..383, O 384..383+d.  One CTA a SM.
