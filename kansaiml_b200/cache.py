@@ -71,7 +71,9 @@ def _on(index, name, *args):
     """Calls libkz with GPU `index` current, on torch's current stream there."""
     stream = torch._C._cuda_getCurrentRawStream(index)
     if torch._C._cuda_getDevice() == index:
-        _lib.call(name, *args, stream)
+        status = getattr(_lib.load(), name)(*args, stream)
+        if status:
+            _lib.check(status, name)
     else:
         with torch.cuda.device(index):
             _lib.call(name, *args, stream)
@@ -140,23 +142,23 @@ class QCache:
                 None if counts is None else _ints(counts, "counts", (batch,), self._at))
 
     def _input(self, t, what, heads, batch):
-        """(x, its address, batch stride, row stride) of [batch, tokens, heads *
-        head_dim] rows that a kernel can read in 16-byte pieces; others are copied."""
+        """(x, tokens, its address, batch stride, row stride) of [batch, tokens,
+        heads * head_dim] rows that a kernel can read in 16-byte pieces; others are copied."""
         x = _raw(t, what)
-        width = heads * self.head_dim
-        if x.dim() != 3 or x.shape[0] != batch or x.shape[2] != width:
-            raise ValueError(f"{what} must be [{batch}, tokens, {width}], not {list(x.shape)}")
+        shape, width = x.shape, heads * self.head_dim
+        if len(shape) != 3 or shape[0] != batch or shape[2] != width:
+            raise ValueError(f"{what} must be [{batch}, tokens, {width}], not {list(shape)}")
         if x.get_device() != self._at:
             raise ValueError(f"{what} is on {x.device}, the cache on {self.device}")
         bs, rs, fs = x.stride()
-        at = x.data_ptr()
-        if (at | bs << 2 | rs << 2) & 15 or fs != 1 or bs < 0 or (rs < width and x.shape[1] > 1):
+        at, tokens = x.data_ptr(), shape[1]
+        if (at | bs << 2 | rs << 2) & 15 or fs != 1 or bs < 0 or (rs < width and tokens > 1):
             x = x.contiguous()
             if x.data_ptr() & 15:
                 x = x.clone()
-            bs, rs = x.shape[1] * width, width      # (a single row's own strides may be anything)
+            bs, rs = tokens * width, width          # (a single row's own strides may be anything)
             at = x.data_ptr()
-        return x, at, bs, rs
+        return x, tokens, at, bs, rs
 
     def write(self, k, v, table, lengths, counts=None, values=False):
         """Quantizes new tokens' k and v [batch, tokens, kv_heads * head_dim]
@@ -164,14 +166,14 @@ class QCache:
         lengths + 0, 1, ...  With ``values``, returns what the codes stand for,
         two Tensors like k and v (0 in padding rows): the K/V a later pass sees."""
         batch, cols, table, lengths, counts = self._sequences(table, lengths, counts)
-        k, k_at, kb, kr = self._input(k, "k", self.kv_heads, batch)
-        v, v_at, vb, vr = self._input(v, "v", self.kv_heads, batch)
-        if v.shape != k.shape:
+        k, tokens, k_at, kb, kr = self._input(k, "k", self.kv_heads, batch)
+        v, v_tokens, v_at, vb, vr = self._input(v, "v", self.kv_heads, batch)
+        if v_tokens != tokens:
             raise ValueError(f"k {list(k.shape)} and v {list(v.shape)} do not match")
         if values:
             ko, vo = _like(k), _like(k)
-        _on(self._at, "kz_cache_write_f32", self._ref, k_at, v_at, batch, k.shape[1], kb, kr, vb, vr, table.data_ptr(),
-            cols, lengths.data_ptr(), ptr(counts), ko.data_ptr() if values else None, vo.data_ptr() if values else None)
+        _on(self._at, "kz_cache_write_f32", self._ref, k_at, v_at, batch, tokens, kb, kr, vb, vr, table.data_ptr(),
+            cols, lengths.data_ptr(), None if counts is None else counts.data_ptr(), ko.data_ptr() if values else None, vo.data_ptr() if values else None)
         return (Tensor(ko), Tensor(vo)) if values else None
 
     def read(self, table, lengths, most):
@@ -198,8 +200,8 @@ class QCache:
         batch, cols, table, lengths, counts = self._sequences(table, lengths, counts)
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"attention: heads ({heads}) must be a multiple of kv_heads ({self.kv_heads})")
-        q, q_at, qb, qr = self._input(q, "q", heads, batch)
-        tokens, pb = q.shape[1], 0
+        q, tokens, q_at, qb, qr = self._input(q, "q", heads, batch)
+        pb = 0
         if parents is not None:
             if tokens > _lib.KZ_TREE_MAX_NODES:
                 raise ValueError(f"attention: a tree has at most {_lib.KZ_TREE_MAX_NODES} nodes (got {tokens})")
@@ -212,8 +214,8 @@ class QCache:
             self._scratch[tokens, heads, cols] = need
         work = self.k_codes.new_empty(need) if need else None
         _on(self._at, "kz_cache_attention_f32", self._ref, q_at, batch, tokens, heads, qb, qr, table.data_ptr(), cols,
-            lengths.data_ptr(), ptr(counts), ptr(parents), pb, self.head_dim ** -0.5 if scale is None else scale,
-            out.data_ptr(), ptr(work), need)
+            lengths.data_ptr(), None if counts is None else counts.data_ptr(), None if parents is None else parents.data_ptr(),
+            pb, self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), None if work is None else work.data_ptr(), need)
         return Tensor(out)
 
     def keep(self, table, lengths, path, count):
@@ -284,27 +286,29 @@ def verify_tree(tokens, parents, target, draft, accept_u, sample_u):
     [batch], and the next token int64 [batch], drawn from r by sample_u: it is
     distributed as the target's own, whatever was drafted."""
     target = _raw(target, "target")
-    if target.dim() != 3 or target.shape[1] < 1 or target.shape[2] < 1:
-        raise ValueError(f"target must be [batch, nodes, vocab], not {list(target.shape)}")
-    batch, nodes, vocab = target.shape
+    shape = target.shape
+    if len(shape) != 3 or shape[1] < 1 or shape[2] < 1:
+        raise ValueError(f"target must be [batch, nodes, vocab], not {list(shape)}")
+    batch, nodes, vocab = shape
     if nodes > 1024:
         raise ValueError(f"verify_tree: at most 1024 nodes (got {nodes})")
-    dev, at = target.device, target.get_device()
+    at = target.get_device()
 
     def floats(t, what, shape):
         x = _raw(t, what)
         if x.shape != shape or x.get_device() != at:
-            raise ValueError(f"{what} must be {list(shape)} on {dev}, not {list(x.shape)} on {x.device}")
+            raise ValueError(f"{what} must be {list(shape)} on {target.device}, not {list(x.shape)} on {x.device}")
         return x.contiguous()
 
     target = target.contiguous()
-    draft = None if draft is None else floats(draft, "draft", target.shape)
+    draft = None if draft is None else floats(draft, "draft", shape)
     accept_u, sample_u = floats(accept_u, "accept_u", (batch, nodes)), floats(sample_u, "sample_u", (batch,))
     tokens = _ints(tokens, "tokens", (batch, nodes), at, torch.int64)
     parents, pb = _parents(parents, batch, nodes, at)
     path = _like(parents) if pb else parents.new_empty((batch, nodes))
     count, token = parents.new_empty(batch), tokens.new_empty(batch)
-    _on(at, "kz_verify_tree_f32", tokens.data_ptr(), parents.data_ptr(), pb, target.data_ptr(), ptr(draft),
+    _on(at, "kz_verify_tree_f32", tokens.data_ptr(), parents.data_ptr(), pb, target.data_ptr(),
+        None if draft is None else draft.data_ptr(),
         accept_u.data_ptr(), sample_u.data_ptr(), batch, nodes, vocab, path.data_ptr(), count.data_ptr(), token.data_ptr())
     return path, count, token
 
