@@ -26,7 +26,8 @@
 // tokens) form tiles of RT rows.  S^T = K Q^T and O^T = V^T P^T put the keys
 // (the head's width) on the 16-row side of the mma and the query rows on its
 // 8-column side, so that 8 rows, not 16, are the smallest tile and each code
-// is converted once for all of a warp's rows.  The four warps of a CTA split
+// is converted once for all of a warp's rows.  Up to four rows leave half of
+// those columns to the small halves (`halves in the columns`).  The four warps of a CTA split
 // the keys of a tile (KG ways) and the rows (RG ways); each keeps its own
 // running maximum and sum, joined at the end.  A fifth warp streams the pages
 // by TMA (swizzled over the row, so ldmatrix reads without conflicts) into a
@@ -39,9 +40,9 @@
 // gives (whole_ranges) each CTA takes whole row tiles instead.
 //
 // Measured, join included: 32 sequences of 4096 to 8191 keys, 32 heads over 8 key
-// heads of 128, one new token each (416 MB of cache): 76 us = 5.5 TB/s, 0.84 of a
+// heads of 128, one new token each (416 MB of cache): 73 us = 5.7 TB/s, 0.87 of a
 // plain copy; HBM bounds it but for about 7 us at the start and the join.  32
-// sequences of up to 255 keys, 4 heads of 64: 7.3 us, latency (lengths, table,
+// sequences of up to 255 keys, 4 heads of 64: 7.2 us, latency (lengths, table,
 // page, one after another, then a tile's chain).  One sequence of 30000: 23 us.
 #include <algorithm>
 #include <atomic>
@@ -54,10 +55,12 @@ namespace {
 constexpr int kConsumers = 128;             // four warps compute, a fifth loads
 constexpr int kCaThreads = kConsumers + 32;
 
+// NT_ = 0: tiles of four rows, see `halves in the columns`.
 template <int D, int NT_, int RG_>
 struct Shape {
-    static constexpr int NT = NT_, RG = RG_, KG = 4 / RG_;
-    static constexpr int RT = 8 * NT * RG;                  // rows a tile
+    static constexpr bool FOUR = NT_ == 0;
+    static constexpr int NT = FOUR ? 1 : NT_, RG = RG_, KG = 4 / RG_;
+    static constexpr int RT = FOUR ? 4 : 8 * NT * RG;       // rows a tile
     static constexpr int STEPS = kKT / (32 * KG);           // steps of 32 keys a warp takes in a tile
     static constexpr int STAGES = RT <= 16 ? 3 : 2;
     static constexpr int CODES = kKT * D, STAGE = 2 * CODES + 2 * kKT * 4;
@@ -97,13 +100,53 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t off) {   // byte offset in
     return D == 128 ? off ^ ((off >> 3) & 0x70u) : D == 64 ? off ^ ((off >> 3) & 0x30u) : off ^ ((off >> 3) & 0x10u);
 }
 
+// 32 bytes of 16 keys (ldmatrix's order) as the 16-row operands of two mmas: of
+// K with the keys on the rows, of V (transposed) with the head's width there,
+// row x being d 2x and row x + 8 d 2x + 1.
+struct Words {
+    uint32_t r[4];
+};
+__device__ __forceinline__ Words ldsm4_of(uint32_t addr) {
+    Words w;
+    ldsm4(addr, w.r);
+    return w;
+}
+__device__ __forceinline__ Words ldsm4_trans_of(uint32_t addr) {
+    Words w;
+    ldsm4_trans(addr, w.r);
+    return w;
+}
+__device__ __forceinline__ void key_operands(Words w, uint32_t (&ops)[2][4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w.r[j] ^= 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        ops[i][0] = two_codes<0x4140>(w.r[2 * i]);
+        ops[i][1] = two_codes<0x4140>(w.r[2 * i + 1]);
+        ops[i][2] = two_codes<0x4342>(w.r[2 * i]);
+        ops[i][3] = two_codes<0x4342>(w.r[2 * i + 1]);
+    }
+}
+__device__ __forceinline__ void value_operands(Words w, uint32_t (&ops)[2][4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w.r[j] ^= 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        ops[i][0] = two_codes<0x4240>(w.r[2 * i]);
+        ops[i][1] = two_codes<0x4341>(w.r[2 * i]);
+        ops[i][2] = two_codes<0x4240>(w.r[2 * i + 1]);
+        ops[i][3] = two_codes<0x4341>(w.r[2 * i + 1]);
+    }
+}
+
 // ------------------------------------------------------------- the kernel
 
-template <int D, int NT, int RG>
+template <int D, int NT_, int RG>
 __global__ void __launch_bounds__(kCaThreads, 2)
     cache_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                            const CacheAttArgs a) {
-    using S = Shape<D, NT, RG>;
+    using S = Shape<D, NT_, RG>;
+    constexpr int NT = S::NT;
     extern __shared__ uint8_t ca_smem[];
     uint8_t* ring = ca_smem + (-smem_u32(ca_smem) & 1023u);      // an offset, so that accesses stay shared-memory ones
     uint4* q_ops = reinterpret_cast<uint4*>(ring + S::STAGES * S::STAGE);   // [RT / 8][D / 16][32]: hi, hi, lo, lo
@@ -181,8 +224,8 @@ __global__ void __launch_bounds__(kCaThreads, 2)
         while (walk.next(a, g)) {
             const int rows = min(S::RT, g.count * a.group - g.rt * S::RT);   // of this tile
             // ---- q, both halves, as mma operands: lane (gq, tq) of [row / 8][d / 16] holds row gq, d 4 tq .. 4 tq + 3
-            for (int n8 = warp; n8 < S::RT / 8; n8 += 4) {
-                const int r = n8 * 8 + gq, R = g.rt * S::RT + r;
+            for (int n8 = warp; n8 < (S::RT + 7) / 8; n8 += 4) {
+                const int r = S::FOUR ? gq & 3 : n8 * 8 + gq, R = g.rt * S::RT + r;
                 float4 x[D / 16];
                 uint32_t m = 0;
                 const float* src = a.q + g.b * a.q_bs + (int64_t)(R / a.group) * a.q_rs +
@@ -207,11 +250,14 @@ __global__ void __launch_bounds__(kCaThreads, 2)
                     float hi[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) hi[j] = leading(e[j]);
-                    q_ops[(n8 * (D / 16) + i) * 32 + lane] =
-                        make_uint4(half2_bits(hi[0], hi[1]), half2_bits(hi[2], hi[3]),
-                                   half2_bits(e[0] - hi[0], e[1] - hi[1]), half2_bits(e[2] - hi[2], e[3] - hi[3]));
+                    const uint4 both = make_uint4(half2_bits(hi[0], hi[1]), half2_bits(hi[2], hi[3]),
+                                                  half2_bits(e[0] - hi[0], e[1] - hi[1]), half2_bits(e[2] - hi[2], e[3] - hi[3]));
+                    if constexpr (S::FOUR)
+                        reinterpret_cast<uint2*>(q_ops)[i * 32 + lane] = gq < 4 ? make_uint2(both.x, both.y) : make_uint2(both.z, both.w);
+                    else
+                        q_ops[(n8 * (D / 16) + i) * 32 + lane] = both;
                 }
-                if (tq == 0) s_qs[r] = a.scale * 1.4426950408889634f * pow2_field(ex - 13);   // scores in powers of 2
+                if (tq == 0 && (!S::FOUR || gq < 4)) s_qs[r] = a.scale * 1.4426950408889634f * pow2_field(ex - 13);   // scores in powers of 2
             }
             if (a.parents) {
                 // each token's row of the tree: itself and its ancestors, one bit a node
@@ -239,7 +285,7 @@ __global__ void __launch_bounds__(kCaThreads, 2)
                     for (int j = 0; j < 4; ++j) o[n][i][j] = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const int r = (rg * NT + n) * 8 + 2 * tq + j;
+                    const int r = S::FOUR ? 2 * (tq & 1) + j : (rg * NT + n) * 8 + 2 * tq + j;
                     m[n][j] = -INFINITY;
                     l[n][j] = 0.0f;
                     qs[n][j] = s_qs[r];
@@ -263,156 +309,229 @@ __global__ void __launch_bounds__(kCaThreads, 2)
                     // rows of 16 bytes for ldmatrix: keys (lane & 15), 16-byte column (lane >> 4)
                     const uint32_t row_at = (kl + (lane & 15)) * D + (lane >> 4) * 16;
 
-                    // ---- S^T: 32 keys x 8 NT rows
-                    float s[2][NT][4], s_lo[2][NT][4];           // the small halves' products have a sum of their own
+                    if constexpr (S::FOUR) {
+                        // ---- halves in the columns: four rows leave four of the mma's eight columns, which
+                        // carry the small halves of q, then of the weights: half the mmas, and the lanes of
+                        // either half take one 16 of the 32 keys each through the softmax
+                        const bool upper = tq >= 2;                  // this lane's keys are the second 16
+                        float s[2][4];
 #pragma unroll
-                    for (int mt = 0; mt < 2; ++mt)
+                        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
+                            for (int j = 0; j < 4; ++j) s[mt][j] = 0.0f;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) s[mt][n][j] = s_lo[mt][n][j] = 0.0f;
+                        for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t ops[2][2][4];
+                            for (int mt = 0; mt < 2; ++mt) {
+                                uint32_t ops[2][4];
+                                key_operands(ldsm4_of(kt + swizzled<D>(row_at + mt * 16 * D + c * 32)), ops);
 #pragma unroll
-                        for (int mt = 0; mt < 2; ++mt) {
-                            uint32_t r[4];
-                            ldsm4(kt + swizzled<D>(row_at + mt * 16 * D + c * 32), r);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) r[j] ^= 0x80808080u;
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                ops[mt][i][0] = two_codes<0x4140>(r[2 * i]);
-                                ops[mt][i][1] = two_codes<0x4140>(r[2 * i + 1]);
-                                ops[mt][i][2] = two_codes<0x4342>(r[2 * i]);
-                                ops[mt][i][3] = two_codes<0x4342>(r[2 * i + 1]);
+                                for (int i = 0; i < 2; ++i) {
+                                    const uint2 q = reinterpret_cast<const uint2*>(q_ops)[(2 * c + i) * 32 + lane];
+                                    mma_16816(s[mt], ops[i], q.x, q.y);
+                                }
                             }
                         }
+                        const int key0 = kl + (upper ? 16 : 0) + gq;
+                        float z[4], mx[2] = {m[0][0], m[0][1]}, vs[2];
+                        uint32_t seen = 0;
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                const uint4 b = q_ops[((rg * NT + n) * (D / 16) + 2 * c + i) * 32 + lane];
-#pragma unroll
-                                for (int mt = 0; mt < 2; ++mt) mma_16816(s[mt][n], ops[mt][i], b.x, b.y);
-#pragma unroll
-                                for (int mt = 0; mt < 2; ++mt) mma_16816(s_lo[mt][n], ops[mt][i], b.z, b.w);
-                            }
-                    }
-
-                    // ---- scales
-                    float ks[2][2], vs[2][2], lv[2][2];
-#pragma unroll
-                    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            ks[mt][j] = ks_t[kl + mt * 16 + j * 8 + gq];
-                            vs[mt][j] = vs_t[kl + mt * 16 + j * 8 + gq];
-                            lv[mt][j] = log2_vs(vs[mt][j]);
-                        }
-
-                    // ---- softmax, one pass: new maximum, weights, and the weights times vs as two halves
-                    float corr[NT][2];
-                    uint32_t w_hi[2][NT][2], w_lo[2][NT][2];
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        uint32_t seen = 0xFFu;          // bit 4 mt + 2 half + column
-                        if (masked) {
-                            seen = 0;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const int key = kl + (e >> 2) * 16 + ((e >> 1) & 1) * 8 + gq, tok = token[n][e & 1];
-                                const int j = t * kKT + key - g.len;
-                                bool v = !((bad >> (key >> a.c.shift)) & 1u);
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = key0 + (e >> 1) * 8, tok = token[0][e & 1], j = t * kKT + key - g.len;
+                            bool v = true;
+                            if (masked) {
+                                v = !((bad >> (key >> a.c.shift)) & 1u);
                                 if (j >= 0)
                                     v = v && j < g.count && (a.parents ? tok <= g.last_token && ((s_sees[tok - g.first_token][j >> 5] >> (j & 31)) & 1u)
                                                                        : j <= tok);
-                                seen |= (uint32_t)v << e;
                             }
+                            seen |= (uint32_t)v << e;
                         }
-                        float z[2][4];
-                        float mx[2] = {m[n][0], m[n][1]};
 #pragma unroll
-                        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                z[mt][e] = (s[mt][n][e] + s_lo[mt][n][e]) * ks[mt][e >> 1] * qs[n][e & 1];
-                                float x = z[mt][e] + lv[mt][e >> 1];
-                                if (!((seen >> (4 * mt + e)) & 1u)) z[mt][e] = x = -INFINITY;
-                                mx[e & 1] = fmaxf(mx[e & 1], x);
-                            }
+                        for (int e = 0; e < 4; ++e) {
+                            const float other = __shfl_xor_sync(0xffffffffu, upper ? s[0][e] : s[1][e], 2);
+                            const float ks = ks_t[key0 + (e >> 1) * 8];
+                            vs[e >> 1] = vs_t[key0 + (e >> 1) * 8];
+                            z[e] = ((upper ? s[1][e] : s[0][e]) + other) * ks * qs[0][e & 1];
+                            float x = z[e] + log2_vs(vs[e >> 1]);
+                            if (!((seen >> e) & 1u)) z[e] = x = -INFINITY;
+                            mx[e & 1] = fmaxf(mx[e & 1], x);
+                        }
+                        float corr[2];
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
 #pragma unroll
-                            for (int x = 4; x <= 16; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
-                            corr[n][j] = shrink(m[n][j], mx[j]);
-                            m[n][j] = mx[j];
-                            l[n][j] *= corr[n][j];
-                            mx[j] = mx[j] == -INFINITY ? 0.0f : kLift - mx[j];      // -inf: no key yet, every weight is 0
+                            for (int x = 2; x <= 16; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
+                            corr[j] = shrink(m[0][j], mx[j]);
+                            m[0][j] = mx[j];
+                            l[0][j] *= corr[j];
+                            mx[j] = mx[j] == -INFINITY ? 0.0f : kLift - mx[j];
+                        }
+                        float hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float p = exp2_approx(z[e] + mx[e & 1]);
+                            l[0][e & 1] += p;
+                            const float w = (seen >> e) & 1u ? p * vs[e >> 1] : 0.0f;
+                            hi[e] = leading(w);
+                            lo[e] = w - hi[e];
+                        }
+                        uint32_t w[2][2];                            // [16 keys][8 keys]
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const uint32_t h = half2_bits(hi[2 * j], hi[2 * j + 1]), k = half2_bits(lo[2 * j], lo[2 * j + 1]);
+                            const uint32_t other = __shfl_xor_sync(0xffffffffu, upper ? h : k, 2);
+                            w[0][j] = transposed_8x8(upper ? other : h);
+                            w[1][j] = transposed_8x8(upper ? k : other);
                         }
 #pragma unroll
-                        for (int mt = 0; mt < 2; ++mt) {
-                            float hi[4], lo[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float p = exp2_approx(z[mt][e] + mx[e & 1]);
-                                l[n][e & 1] += p;
-                                const float w = (seen >> (4 * mt + e)) & 1u ? p * vs[mt][e >> 1] : 0.0f;
-                                hi[e] = leading(w);
-                                lo[e] = w - hi[e];
-                            }
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {   // keys on the mma's inner side: transposed 8 x 8
-                                w_hi[mt][n][j] = transposed_8x8(half2_bits(hi[2 * j], hi[2 * j + 1]));
-                                w_lo[mt][n][j] = transposed_8x8(half2_bits(lo[2 * j], lo[2 * j + 1]));
-                            }
-                        }
-                    }
-
-                    // ---- O^T: D x 8 NT rows, the step's sum joined to the row's
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t ops[2][2][4];
-#pragma unroll
-                        for (int mt = 0; mt < 2; ++mt) {
-                            uint32_t r[4];
-                            ldsm4_trans(vt + swizzled<D>(row_at + mt * 16 * D + c * 32), r);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) r[j] ^= 0x80808080u;
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {       // mma row x is d 2x, row x + 8 is d 2x + 1
-                                ops[mt][i][0] = two_codes<0x4240>(r[2 * i]);
-                                ops[mt][i][1] = two_codes<0x4341>(r[2 * i]);
-                                ops[mt][i][2] = two_codes<0x4240>(r[2 * i + 1]);
-                                ops[mt][i][3] = two_codes<0x4341>(r[2 * i + 1]);
-                            }
-                        }
-                        float acc[2][NT][4];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.0f;
-#pragma unroll
-                        for (int mt = 0; mt < 2; ++mt)             // the small halves first: their sum is truncated least
+                        for (int c = 0; c < D / 32; ++c) {
+                            float acc[2][4];
 #pragma unroll
                             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                                for (int n = 0; n < NT; ++n) mma_16816(acc[i][n], ops[mt][i], w_lo[mt][n][0], w_lo[mt][n][1]);
+                                for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+#pragma unroll
+                            for (int mt = 0; mt < 2; ++mt) {
+                                uint32_t ops[2][4];
+                                value_operands(ldsm4_trans_of(vt + swizzled<D>(row_at + mt * 16 * D + c * 32)), ops);
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) mma_16816(acc[i], ops[i], w[mt][0], w[mt][1]);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) o[0][2 * c + i][j] = fmaf(o[0][2 * c + i][j], corr[j & 1], acc[i][j]);
+                        }
+                        continue;
+                    } else {
+                        // ---- S^T: 32 keys x 8 NT rows
+                        float s[2][NT][4], s_lo[2][NT][4];           // the small halves' products have a sum of their own
 #pragma unroll
                         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                                for (int n = 0; n < NT; ++n) mma_16816(acc[i][n], ops[mt][i], w_hi[mt][n][0], w_hi[mt][n][1]);
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                                for (int j = 0; j < 4; ++j)
-                                    o[n][2 * c + i][j] = fmaf(o[n][2 * c + i][j], corr[n][j & 1], acc[i][n][j]);
+                                for (int j = 0; j < 4; ++j) s[mt][n][j] = s_lo[mt][n][j] = 0.0f;
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t ops[2][2][4];
+#pragma unroll
+                            for (int mt = 0; mt < 2; ++mt) key_operands(ldsm4_of(kt + swizzled<D>(row_at + mt * 16 * D + c * 32)), ops[mt]);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    const uint4 b = q_ops[((rg * NT + n) * (D / 16) + 2 * c + i) * 32 + lane];
+#pragma unroll
+                                    for (int mt = 0; mt < 2; ++mt) mma_16816(s[mt][n], ops[mt][i], b.x, b.y);
+#pragma unroll
+                                    for (int mt = 0; mt < 2; ++mt) mma_16816(s_lo[mt][n], ops[mt][i], b.z, b.w);
+                                }
+                        }
+
+                        // ---- scales
+                        float ks[2][2], vs[2][2], lv[2][2];
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                ks[mt][j] = ks_t[kl + mt * 16 + j * 8 + gq];
+                                vs[mt][j] = vs_t[kl + mt * 16 + j * 8 + gq];
+                                lv[mt][j] = log2_vs(vs[mt][j]);
+                            }
+
+                        // ---- softmax, one pass: new maximum, weights, and the weights times vs as two halves
+                        float corr[NT][2];
+                        uint32_t w_hi[2][NT][2], w_lo[2][NT][2];
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            uint32_t seen = 0xFFu;          // bit 4 mt + 2 half + column
+                            if (masked) {
+                                seen = 0;
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    const int key = kl + (e >> 2) * 16 + ((e >> 1) & 1) * 8 + gq, tok = token[n][e & 1];
+                                    const int j = t * kKT + key - g.len;
+                                    bool v = !((bad >> (key >> a.c.shift)) & 1u);
+                                    if (j >= 0)
+                                        v = v && j < g.count && (a.parents ? tok <= g.last_token && ((s_sees[tok - g.first_token][j >> 5] >> (j & 31)) & 1u)
+                                                                           : j <= tok);
+                                    seen |= (uint32_t)v << e;
+                                }
+                            }
+                            float z[2][4];
+                            float mx[2] = {m[n][0], m[n][1]};
+#pragma unroll
+                            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    z[mt][e] = (s[mt][n][e] + s_lo[mt][n][e]) * ks[mt][e >> 1] * qs[n][e & 1];
+                                    float x = z[mt][e] + lv[mt][e >> 1];
+                                    if (!((seen >> (4 * mt + e)) & 1u)) z[mt][e] = x = -INFINITY;
+                                    mx[e & 1] = fmaxf(mx[e & 1], x);
+                                }
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                                for (int x = 4; x <= 16; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
+                                corr[n][j] = shrink(m[n][j], mx[j]);
+                                m[n][j] = mx[j];
+                                l[n][j] *= corr[n][j];
+                                mx[j] = mx[j] == -INFINITY ? 0.0f : kLift - mx[j];      // -inf: no key yet, every weight is 0
+                            }
+#pragma unroll
+                            for (int mt = 0; mt < 2; ++mt) {
+                                float hi[4], lo[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float p = exp2_approx(z[mt][e] + mx[e & 1]);
+                                    l[n][e & 1] += p;
+                                    const float w = (seen >> (4 * mt + e)) & 1u ? p * vs[mt][e >> 1] : 0.0f;
+                                    hi[e] = leading(w);
+                                    lo[e] = w - hi[e];
+                                }
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) {   // keys on the mma's inner side: transposed 8 x 8
+                                    w_hi[mt][n][j] = transposed_8x8(half2_bits(hi[2 * j], hi[2 * j + 1]));
+                                    w_lo[mt][n][j] = transposed_8x8(half2_bits(lo[2 * j], lo[2 * j + 1]));
+                                }
+                            }
+                        }
+
+                        // ---- O^T: D x 8 NT rows, the step's sum joined to the row's
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t ops[2][2][4];
+#pragma unroll
+                            for (int mt = 0; mt < 2; ++mt) value_operands(ldsm4_trans_of(vt + swizzled<D>(row_at + mt * 16 * D + c * 32)), ops[mt]);
+                            float acc[2][NT][4];
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.0f;
+#pragma unroll
+                            for (int mt = 0; mt < 2; ++mt)             // the small halves first: their sum is truncated least
+#pragma unroll
+                                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                    for (int n = 0; n < NT; ++n) mma_16816(acc[i][n], ops[mt][i], w_lo[mt][n][0], w_lo[mt][n][1]);
+#pragma unroll
+                            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                    for (int n = 0; n < NT; ++n) mma_16816(acc[i][n], ops[mt][i], w_hi[mt][n][0], w_hi[mt][n][1]);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j)
+                                        o[n][2 * c + i][j] = fmaf(o[n][2 * c + i][j], corr[n][j & 1], acc[i][n][j]);
+                        }
                     }
                 }
                 __syncwarp();
@@ -420,13 +539,20 @@ __global__ void __launch_bounds__(kCaThreads, 2)
             }
 
             // ---- the warps' parts joined
+            if constexpr (S::FOUR) {                               // the small halves' sums to the leading ones'
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[0][i][j] += __shfl_xor_sync(0xffffffffu, o[0][i][j], 2);
+            }
+            const bool holds = !S::FOUR || tq < 2;                 // a lane whose rows are not another's too
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
 #pragma unroll
-                    for (int x = 4; x <= 16; x <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
-                    if (gq == 0) {
+                    for (int x = S::FOUR ? 2 : 4; x <= 16; x <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
+                    if (gq == 0 && holds) {
                         s_m[kg][(rg * NT + n) * 8 + 2 * tq + j] = m[n][j];
                         s_l[kg][(rg * NT + n) * 8 + 2 * tq + j] = l[n][j];
                     }
@@ -441,7 +567,7 @@ __global__ void __launch_bounds__(kCaThreads, 2)
                 return out + ((int64_t)(R / a.group) * a.heads + R % a.group) * D;
             };
             for (int turn = 0; turn < S::KG; ++turn) {
-                if (turn == kg) {
+                if (turn == kg && holds) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -502,9 +628,9 @@ __global__ void __launch_bounds__(kCaThreads, 2)
 // and the second: one sequence of 30000 keys (35 parts a row) 31 and 23 us; 32
 // sequences of 4096 to 8191 76 and 80; 2 chunks of 500 tokens, 4 rows a token, 150
 // and 188.
-template <bool FEW>
+template <bool FEW, int RT>
 struct Join {
-    static constexpr int ROWS = FEW ? 8 : 1, WARPS = FEW ? 4 : 8;
+    static constexpr int ROWS = !FEW ? 1 : RT < 8 ? RT : 8, WARPS = FEW ? 4 : 8;
 };
 template <int E>
 __device__ __forceinline__ void load_values(const float* p, float (&v)[E]) {
@@ -528,8 +654,8 @@ __device__ __forceinline__ void store_values(float* p, const float (&v)[E]) {
         *p = v[0];
 }
 template <int D, int RT, bool FEW>
-__global__ void __launch_bounds__(32 * Join<FEW>::WARPS) cache_attention_join_kernel(const CacheAttArgs a) {
-    constexpr int E = D / 32, SLOT = RT * (D + 2), ROWS = Join<FEW>::ROWS, WARPS = Join<FEW>::WARPS, BLOCKS = RT / ROWS;
+__global__ void __launch_bounds__(32 * Join<FEW, RT>::WARPS) cache_attention_join_kernel(const CacheAttArgs a) {
+    constexpr int E = D / 32, SLOT = RT * (D + 2), ROWS = Join<FEW, RT>::ROWS, WARPS = Join<FEW, RT>::WARPS, BLOCKS = RT / ROWS;
     __shared__ Work s_work[WARPS];
     __shared__ int s_before[WARPS];
     __shared__ __align__(16) float s_part[WARPS][ROWS][D];
@@ -656,7 +782,7 @@ __global__ void __launch_bounds__(32 * Join<FEW>::WARPS) cache_attention_join_ke
 
 template <int D, int RT, bool FEW>
 int launch_join_as(const CacheAttArgs& a, int64_t row_tiles, cudaStream_t s) {
-    using J = Join<FEW>;
+    using J = Join<FEW, RT>;
     KZ_CHECK_CUDA(launch_pdl(cache_attention_join_kernel<D, RT, FEW>,
                              dim3((unsigned)(row_tiles * a.c.heads * (RT / J::ROWS)), (unsigned)a.batch), dim3(32 * J::WARPS),
                              0, s, a));
@@ -670,10 +796,11 @@ int launch_join(const CacheAttArgs& a, int64_t row_tiles, cudaStream_t s) {
 
 // ---------------------------------------------------------------- launches
 
-// Rows of a tile: the smallest of 8, 16 and 32 that holds a key head's rows.  With
-// tiles of 8, 16 and 32, 4 rows over 32 long sequences: 78, 110 and 197 us; 16
-// rows, 16 sequences of 3000 to 6000: 51 us with 16, 84 with 32.
-int tile_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+// Rows of a tile: the smallest of 4, 8, 16 and 32 that holds a key head's rows.  With
+// tiles of 4, 8, 16 and 32, 4 rows over 32 long sequences: 73, 76, 110 and 197 us
+// (4 and 8 for seconds on end, under the power cap: 79 and 86); 16 rows, 16
+// sequences of 3000 to 6000: 51 us with 16, 84 with 32.
+int tile_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
 
 // Whether a call needs no workspace and no join: its table holds no more than
 // four tiles of keys a row tile.  One sequence of 500 keys, 8 key heads: 8.6 us so,
@@ -727,6 +854,7 @@ int dispatch_cache_attention(CacheAttArgs a, cudaStream_t s) {
     }
     const int rt = tile_rows(rows);
     const int64_t row_tiles = (rows + rt - 1) / rt;
+    if (rt == 4) return launch_cache_attention<D, 0, 1>(a, row_tiles, s);
     if (rt == 8) return launch_cache_attention<D, 1, 1>(a, row_tiles, s);
     if (rt == 16) return launch_cache_attention<D, 2, 1>(a, row_tiles, s);
     return launch_cache_attention<D, 2, 2>(a, row_tiles, s);

@@ -373,6 +373,18 @@ def test_attention_extreme_scales_many_rows(cuda_device, d, spread, strong):
     _check_attention(book, [200], None, 70, 4, _tree(70, 3), spread=spread, strong=strong)
 
 
+@pytest.mark.parametrize("d,kv,heads,tokens,tree", [(64, 3, 3, 4, True), (128, 2, 2, 3, False), (32, 1, 2, 2, True),
+                                                    (128, 2, 4, 1, False), (64, 1, 3, 1, False), (32, 2, 2, 4, False)])
+@pytest.mark.parametrize("spread,strong", [(1.0, 1.5), (12.0, 1e-4), (0.5, 12.0), (30.0, 1e-12), (1.0, 0.0)])
+def test_attention_up_to_four_rows(cuda_device, d, kv, heads, tokens, tree, spread, strong):
+    """A key head's rows are one to four: trees, chunks with padding and single
+    tokens, whole and in parts, at ordinary and extreme scales."""
+    lengths, counts = [0, 33, 500, 1700], [tokens, max(tokens - 1, 1), 0, tokens]
+    book = Book([a + b for a, b in zip(lengths, counts)], kv, d, 32, seed=d)
+    parents = [_tree(tokens, b) for b in range(4)] if tree else None
+    _check_attention(book, lengths, counts, tokens, heads, parents, spread=spread, strong=strong)
+
+
 def test_attention_scale_argument(cuda_device):
     book = Book([300], 1, 32, 16)
     _check_attention(book, [299], None, 1, 2, scale=0.03)
