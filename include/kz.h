@@ -365,7 +365,9 @@ int kz_cache_keep(const kz_cache* cache, const int32_t* table, int64_t table_col
  * hold kz_cache_attention_workspace_bytes(...) bytes, 0 for short tables.  The
  * products keep 22 bits of q and of each weight times V's scale, down to 2^-38
  * of the row's largest; sums are 32-bit.  Scales are positive; a V scale counts
- * as within 2^-100 .. 2^100 where the weights are brought into range. */
+ * as within 2^-100 .. 2^100 where the weights are brought into range, for any
+ * number of keys (below, 2^-138 over the scale stands for those 2^-38; from 2^102
+ * up rows can be Inf or NaN, and from a K scale of 2^99 up). */
 size_t kz_cache_attention_workspace_bytes(const kz_cache* cache, int64_t tokens, int64_t heads, int64_t table_cols);
 int kz_cache_attention_f32(const kz_cache* cache, const float* q, int64_t batch, int64_t tokens, int64_t heads,
                            int64_t q_batch_stride, int64_t q_row_stride, const int32_t* table, int64_t table_cols,

@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kCaThreads, 2)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float p = exp2_approx(z[e] + mx[e & 1]);
-                            l[0][e & 1] += p;
+                            l[0][e & 1] = fmaf(p, kSumUnit, l[0][e & 1]);
                             const float w = (seen >> e) & 1u ? p * vs[e >> 1] : 0.0f;
                             hi[e] = leading(w);
                             lo[e] = w - hi[e];
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kCaThreads, 2)
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
                                     const float p = exp2_approx(z[mt][e] + mx[e & 1]);
-                                    l[n][e & 1] += p;
+                                    l[n][e & 1] = fmaf(p, kSumUnit, l[n][e & 1]);
                                     const float w = (seen >> (4 * mt + e)) & 1u ? p * vs[mt][e >> 1] : 0.0f;
                                     hi[e] = leading(w);
                                     lo[e] = w - hi[e];
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(kCaThreads, 2)
 #pragma unroll
                     for (int k = 0; k < S::KG; ++k) L += s_l[k][r] * shrink(s_m[k][r], M);
                     const float f = L == 0.0f ? 0.0f : 1.0f / L;
-                    v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+                    v = make_float4(over_sum(v.x, f), over_sum(v.y, f), over_sum(v.z, f), over_sum(v.w, f));
                 }
                 *reinterpret_cast<float4*>((direct ? out_row(r) : slot + r * D) + 4 * c) = v;
             }
@@ -698,7 +698,7 @@ __global__ void __launch_bounds__(32 * Join<FEW, RT>::WARPS) cache_attention_joi
         const float f = L == 0.0f ? 0.0f : 1.0f / L;
         const int R = rt * RT + r;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] *= f;
+        for (int e = 0; e < E; ++e) o[e] = over_sum(o[e], f);
         store_values(a.out + ((int64_t)b * a.tokens + R / a.group) * a.heads * D + ((int64_t)h * a.group + R % a.group) * D + lane * E, o);
     };
     if (c1 - c0 < 4) {

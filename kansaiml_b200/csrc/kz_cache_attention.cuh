@@ -21,7 +21,7 @@ struct CacheAttArgs {
     const int32_t* parents;
     int64_t parents_bs;
     float* out;
-    float* parts;          // two slots a CTA: sums [RT][D], maxima [RT], weights [RT]; NULL: no range ends inside a row tile
+    float* parts;          // two slots a CTA: sums [RT][D], maxima [RT], weights (kSumUnit times) [RT]; NULL: no range ends inside a row tile
     int batch, tokens, heads, group;
     int ctas;              // the launch's
     FastDiv by_ctas;
@@ -206,8 +206,14 @@ __device__ __forceinline__ float pow2_field(int field) { return __uint_as_float(
 // is brought to 2^kLift by measuring the softmax's exponent from the running
 // maximum of s + log2(vs), not of s alone (the sum of the weights is measured
 // from it too, so it cancels).  vs counts as within 2^-100 .. 2^100 here, which
-// keeps the weights themselves within fp32.
+// keeps a weight within 2^114; their sum is kept in units of 2^20 (an exact
+// factor, taken by the multiply-add that adds a weight up), so that 2^31 of them
+// stay below 2^126.
 constexpr float kLift = 14.0f;
+constexpr float kSumUnit = 9.5367431640625e-7f;         // 2^-20
+// o over the weights' sum, `inverse` that of the sum as it is kept: in this
+// order neither factor leaves fp32 at either end of vs
+__device__ __forceinline__ float over_sum(float o, float inverse) { return (o * kSumUnit) * inverse; }
 __device__ __forceinline__ float log2_vs(float vs) {
     float r;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(vs));

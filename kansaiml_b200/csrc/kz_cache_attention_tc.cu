@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
                     m = m_new;
                     float s0, s1;
                     unpair(add2(sum[0], sum[1]), s0, s1);
-                    l = fmaf(l, corr_new, s0 + s1);
+                    l = fmaf(l, corr_new, (s0 + s1) * kSumUnit);
                     tc_wait_st();
                     tc_fence_before();
                     arrive(s_p_full[it & 1]);
@@ -586,7 +586,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
             s_l[half][row] = l;
             meet();
             l += s_l[half ^ 1][row];
-            const float f = g.whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+            // o over the sum by one factor, which stays a normal number up to a sum of 2^100; past that
+            // (V scales near 2^-100) its 2^-20 is taken afterwards, from what was stored.  A second factor
+            // on o itself, though after the loop, made the loop 7 us of 151 slower (attend_chunk).
+            const bool far = g.whole && l > 1.2676506e30f;
+            const float f = !g.whole ? 1.0f : l == 0.0f ? 0.0f : (far ? 1.0f : kSumUnit) / l;
             float* slot = g.whole ? nullptr
                                   : a.parts + (2 * (int64_t)blockIdx.x + (first_segment ? 0 : 1)) * (kTcRows * (D + 2));
             first_segment = false;
@@ -598,6 +602,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) cache_attention_tc_kernel(const
                 for (int i = 0; i < D / 8; ++i)
                     *reinterpret_cast<float4*>(dst + 4 * i) =
                         make_float4(o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f);
+                if (far)
+#pragma unroll 1
+                    for (int i = 0; i < D / 2; ++i) dst[i] *= kSumUnit;
             }
             if (!g.whole && half == 0) {
                 slot[kTcRows * D + row] = m;

@@ -991,3 +991,59 @@ def test_refusals(cuda_device):
     with pytest.raises(ValueError, match="1024"):
         verify_tree(tok, par, torch.zeros(1, 1025, 2, device="cuda"), None, u, s)
     assert _status() == 0
+
+
+# ------------------------------------------- ends of the range, long contexts, waits
+
+# What even weights over values of one sign may be off by, of the result: no
+# score has an error, a weight has 22 bits (two halves of 11; 2^-22), and the
+# exponential's argument, up to 2^5 where ranges' largest values differ, is off
+# by 2^-20, the ranges then weighing differently by 2^-19 ln 2: 2^-18 for all of
+# these.  A sum is a chain of at most 64 additions each off by 2^-23: the
+# tensor core's 16 keys at a time (2 to 16 in a step), steps of a range (1 to
+# 3 tiles where the keys are dealt out over the GPU), four warps, the ranges
+# by eight (157 of them: 20 and 8).  Without a weight's smaller half: 2^-12 on
+# the mean, twenty times as much.
+EVEN = 64 * 2.0**-23 + 2.0**-18
+
+
+@pytest.mark.parametrize("tokens,heads", [(1, 2), (1, 16), (40, 2)])
+@pytest.mark.parametrize("scale", [1e-34, 1e-30, 1.0, 1e30])
+@pytest.mark.parametrize("n", [40000, 400])
+def test_attention_long_contexts_at_the_ends_of_v(cuda_device, tokens, heads, scale, n):
+    """Keys that weigh the same, in ranges joined and in one, V scales from one
+    end of their range to the other: the sum of the weights, measured against
+    the largest w * vs, stays a number.  q is 0, so the output is the mean."""
+    book = Book([n], 1, 64, 64)
+    book.fill([n])
+    codes = torch.randint(1, 128, book.cache.v_codes.shape, device="cuda").to(torch.int8)
+    book.cache.v_codes.copy_(codes)
+    book.cache.v_scale.fill_(scale)
+    y = book.cache.attention(torch.zeros(1, tokens, heads * 64, device="cuda"), heads, book.table, _i32([n - tokens])).data
+    pos = torch.arange(n, device="cuda")
+    sums = (codes[book.table[0, pos // 64].long(), 0, pos % 64].double() * float(np.float32(scale))).cumsum(0)
+    for t in (0, tokens - 1):
+        seen = n - tokens + 1 + t
+        want = (sums[seen - 1] / seen).repeat(heads)
+        assert ((y[0, t].double() - want).abs() / want).max().item() <= EVEN, t
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("d,kv,heads,tokens,lengths", [
+    (128, 1, 2, 1, [20000]), (64, 2, 16, 1, [17000, 300]), (32, 1, 16, 2, [16500]), (128, 1, 8, 12, [20000, 5]),
+    (64, 1, 4, 40, [20000])])
+def test_attention_keeps_its_halves_over_long_contexts(cuda_device, d, kv, heads, tokens, lengths):
+    """Values of one sign, their scales spread over e^2, under even weights:
+    nothing cancels, so what is lost of a weight or in a join shows."""
+    book = Book([n + tokens for n in lengths], kv, d, 32)
+    _, vvals = book.fill([n + tokens for n in lengths], spread=1.0)
+    book.cache.v_codes.copy_(book.cache.v_codes.abs())
+    y = book.cache.attention(torch.zeros(len(lengths), tokens, heads * d, device="cuda"), heads, book.table,
+                             _i32(lengths)).numpy()
+    for b, n in enumerate(lengths):
+        sums = np.abs(vvals[b]).cumsum(0)
+        for t in range(tokens):
+            want = (sums[n + t] / (n + t + 1)).repeat(heads // kv, 0).reshape(-1)
+            off = np.abs(y[b, t] - want) / want
+            assert off.max() <= EVEN, (b, t, off.max())
+    assert _status() == 0
