@@ -161,15 +161,16 @@ class MultiHeadAttention(Module):
             self.qkv = QLinear(_W(Tensor(qkv)), per_channel=True, activations=activations)
         return self
 
-    def _proj(self, x, i, w):
+    def _proj(self, x, i, w, step=None):
         if self.q_proj is not None:
-            return self.q_proj[i](x)
+            return self.q_proj[i](x if step is None else _step_input(self.q_proj[i], x))
         return x.matmul(w)
 
     def forward(self, query, key, value, mask=None, step=None):
         """With ``step`` (a CacheStep; self-attention only), the inputs are a
         step's new tokens: their keys and values enter the layer's cache and
-        the attention runs over all it holds (mask unused)."""
+        the attention runs over all it holds (mask unused).  What int8
+        projections quantize per tensor they quantize row by row then."""
         if step is not None and not (query is key and key is value):
             raise ValueError("attention over a cache is self-attention: query, key and value must be one input")
         if self.qkv is not None and query is key and key is value:
@@ -177,11 +178,11 @@ class MultiHeadAttention(Module):
         if isinstance(query, QActivation):
             raise ValueError("a pre-quantized input needs the fused self-attention path")
         q_in, k_in, v_in = as_tensor(query), as_tensor(key), as_tensor(value)
-        q = self._proj(q_in, 0, self.w_q).data
-        k = self._proj(k_in, 1, self.w_k).data
-        v = self._proj(v_in, 2, self.w_v).data
+        q = self._proj(q_in, 0, self.w_q, step).data
+        k = self._proj(k_in, 1, self.w_k, step).data
+        v = self._proj(v_in, 2, self.w_v, step).data
         if step is not None:
-            return self._proj(step.attend(q, k, v, self.num_heads), 3, self.w_o)
+            return self._proj(step.attend(q, k, v, self.num_heads), 3, self.w_o, step)
         causal = self._causal(mask, q.shape[1], k.shape[1])
         m = as_tensor(mask).data if mask is not None and not causal else None
         att, _ = attention_device(q, k, v, self.num_heads, mask=m, causal=causal)
@@ -207,9 +208,10 @@ class MultiHeadAttention(Module):
         the key tiles past the diagonal."""
         b, s, _ = x.shape
         d = self.d_model
-        qkv = self.qkv(x).data.reshape(b, s, 3 * d)
+        qkv = self.qkv(x if step is None else _step_input(self.qkv, x)).data.reshape(b, s, 3 * d)
         if step is not None:
-            return self.q_proj[3](step.attend(qkv[:, :, :d], qkv[:, :, d:2 * d], qkv[:, :, 2 * d:], self.num_heads))
+            att = step.attend(qkv[:, :, :d], qkv[:, :, d:2 * d], qkv[:, :, 2 * d:], self.num_heads)
+            return self.q_proj[3](QActivation.rows(att))
         causal = self._causal(mask, s, s)
         m = as_tensor(mask).data if mask is not None and not causal else None
         att, partials = attention_device(qkv[:, :, :d], qkv[:, :, d:2 * d], qkv[:, :, 2 * d:], self.num_heads,
@@ -246,11 +248,12 @@ class TransformerBlock(Module):
         normed = self.ln1(x)
         x = x.add(self.attn(normed, normed, normed, mask=mask, step=step))
         h = self.ln2(x)
+        inner = (lambda layer, h: h) if step is None else _step_input
         if isinstance(self.fc1, QLinear):
-            h = self.fc1(h, act="gelu")
+            h = self.fc1(inner(self.fc1, h), act="gelu")
         else:
             h = self.gelu(self.fc1(h))
-        return x.add(self.fc2(h))
+        return x.add(self.fc2(inner(self.fc2, h)))
 
     def _forward_w8a8(self, x, mask, pending=None, step=None):
         """The same block with every activation quantized where it is made:
@@ -260,23 +263,37 @@ class TransformerBlock(Module):
         residual adds are folded into the LayerNorm that follows each one: the
         block's input is x + pending (pending None: x), and it returns
         (x, pending) with its output x + pending, for the next LayerNorm to
-        add."""
-        ln1, ln2 = self.ln1, self.ln2
+        add.  In a step of generation activations are quantized row by row."""
+        ln1, ln2, rows = self.ln1, self.ln2, step is not None
         if pending is None:
-            qa = QActivation.layernorm(x, ln1.weight, ln1.bias, ln1.eps)
+            qa = QActivation.layernorm(x, ln1.weight, ln1.bias, ln1.eps, rows)
         else:
-            x, qa = QActivation.add_layernorm(x, pending, ln1.weight, ln1.bias, ln1.eps)
-        x, qb = QActivation.add_layernorm(x, self.attn(qa, qa, qa, mask=mask, step=step), ln2.weight, ln2.bias, ln2.eps)
+            x, qa = QActivation.add_layernorm(x, pending, ln1.weight, ln1.bias, ln1.eps, rows)
+        x, qb = QActivation.add_layernorm(x, self.attn(qa, qa, qa, mask=mask, step=step), ln2.weight, ln2.bias, ln2.eps, rows)
+        if rows:
+            return x, self.fc2(QActivation.rows(self.fc1(qb, act="gelu")))
         partials = partials_buffer(x.data.device)
         h = self.fc1(qb, act="gelu", out_partials=partials)
         return x, self.fc2(QActivation.from_partials(h, partials))
+
+
+def _step_input(layer, x):
+    """A layer's input in a step of generation: with a scale for each row where
+    the layer would take one for all of them."""
+    if isinstance(layer, QLinear) and layer.per_tensor_activations and not isinstance(x, QActivation):
+        return QActivation.rows(x)
+    return x
 
 
 class CacheStep:
     """One step of generation as one layer sees it: its QCache, the sequences'
     pages and lengths before the step, how many of the step's rows are tokens
     (counts, None: all) and the tree they form (parents, None: one after
-    another).  See kansaiml_b200.cache for the tensors."""
+    another).  See kansaiml_b200.cache for the tensors.
+
+    A step's rows are unrelated: padding, other sequences, drafts that will not
+    stand.  One scale for all of them would make a token's output depend on the
+    rest, so in a step the layers quantize their activations row by row."""
 
     __slots__ = ("cache", "table", "lengths", "counts", "parents")
 

@@ -246,12 +246,12 @@ def device_status(device=None, clear=True):
 # ------------------------------------------------------------ QTensor
 
 class QActivation:
-    """An activation quantized per tensor for the W8A8 path: int8 codes in the
-    activation's own layout and its scale (float64 and float32, one element
-    each, on the device).  ``qlinear`` accepts it in place of an fp32 input and
-    skips its own quantize step, which lets the producer of the activation
-    supply the absmax: a LayerNorm (``layernorm``) or the epilogue of the
-    previous int8 GEMM (``from_partials``)."""
+    """An activation quantized for the W8A8 path, per tensor or (``rows``) row by
+    row: int8 codes in the activation's own layout and its scale (float64 and
+    float32, one element each or one a row, on the device).  ``qlinear`` accepts
+    it in place of an fp32 input and skips its own quantize step, which lets the
+    producer of the activation supply the absmax: a LayerNorm (``layernorm``) or
+    the epilogue of the previous int8 GEMM (``from_partials``)."""
 
     __slots__ = ("codes", "scale64", "scale_f32")
 
@@ -264,11 +264,24 @@ class QActivation:
 
     @property
     def scale(self):
-        return float(self.scale64.item())
+        """float (per tensor) or list of floats (by row), the exact doubles."""
+        return float(self.scale64.item()) if self.scale64.numel() == 1 else self.scale64.tolist()
 
     @classmethod
     def from_tensor(cls, x):
         return cls(*quantize_tensor_device(_dev_tensor(x, "QActivation")))
+
+    @classmethod
+    def rows(cls, x):
+        """x with a scale for each row (its last axis): no row's codes depend on
+        what else is in x."""
+        x = _dev_tensor(x, "QActivation.rows")
+        K = x.shape[-1]
+        M = x.numel() // K
+        q = torch.empty_like(x, dtype=torch.int8)
+        s64, s32 = torch.empty(M, dtype=torch.float64, device=x.device), torch.empty(M, dtype=torch.float32, device=x.device)
+        _lib.call("kz_quantize_rows_f32", ptr(x), M, K, ptr(q), ptr(s64), ptr(s32), stream_handle(x.device))
+        return cls(q, s64, s32)
 
     @classmethod
     def from_partials(cls, x, partials):
@@ -277,20 +290,22 @@ class QActivation:
         return cls(*quantize_partials_device(_dev_tensor(x, "QActivation"), partials))
 
     @classmethod
-    def layernorm(cls, x, weight=None, bias=None, eps=1e-5):
+    def layernorm(cls, x, weight=None, bias=None, eps=1e-5, rows=False):
         """LayerNorm (nn.py:308-331) of x, quantized per tensor: the LayerNorm
-        kernel emits the absmax partials, so the quantize is a single pass."""
+        kernel emits the absmax partials, so the quantize is a single pass.
+        With ``rows``, quantized row by row."""
         y, partials = layernorm_partials_device(_dev_tensor(x, "QActivation.layernorm"), weight, bias, eps)
-        return cls(*quantize_partials_device(y, partials))
+        return cls.rows(y) if rows else cls(*quantize_partials_device(y, partials))
 
     @classmethod
-    def add_layernorm(cls, x, residual, weight=None, bias=None, eps=1e-5):
+    def add_layernorm(cls, x, residual, weight=None, bias=None, eps=1e-5, rows=False):
         """x + residual (a pre-LN block's residual connection, nn.py:476-477)
-        and the LayerNorm of that sum quantized per tensor, from one LayerNorm
-        kernel that also writes the sum.  Returns (Tensor sum, QActivation)."""
+        and the LayerNorm of that sum quantized per tensor (``rows``: row by
+        row), from one LayerNorm kernel that also writes the sum.  Returns
+        (Tensor sum, QActivation)."""
         y, partials, total = layernorm_partials_device(_dev_tensor(x, "QActivation.add_layernorm"), weight, bias,
                                                        eps, residual=_dev_tensor(residual, "QActivation.add_layernorm"))
-        return Tensor(total), cls(*quantize_partials_device(y, partials))
+        return Tensor(total), cls.rows(y) if rows else cls(*quantize_partials_device(y, partials))
 
 
 class QTensor:
@@ -466,8 +481,8 @@ def qlinear(x, qweight: QTensor, bias=None, activations=None, act=None, out_part
     weight): W8A8 on the tensor cores with the epilogue fused.
     act: optional "relu" / "gelu" applied in the same kernel (the value is the
     same as applying nn.ReLU / nn.GELU afterwards).
-    x may be a QActivation (already quantized per tensor): the W8A8 GEMM then
-    consumes its codes directly.  out_partials (W8A8 only): a KZ_PARTIALS_WORDS
+    x may be a QActivation (already quantized): the W8A8 GEMM then consumes its
+    codes directly.  out_partials (W8A8 only): a KZ_PARTIALS_WORDS
     buffer that receives the absmax partials of the output, for
     QActivation.from_partials.
     """
@@ -533,6 +548,11 @@ class QLinear:
         self.qweight = QTensor.from_tensor(linear.weight, per_channel=per_channel)
         self.bias = as_tensor(linear.bias, device=self.qweight.device) if linear.bias is not None else None
         self.activations = activations
+
+    @property
+    def per_tensor_activations(self):
+        """Whether an fp32 input is quantized with one scale for all its rows."""
+        return (self.activations or ("fp32" if self.qweight.granularity == "tensor" else "int8")) == "int8"
 
     def __call__(self, x, act=None, out_partials=None):
         return qlinear(x, self.qweight, self.bias, activations=self.activations, act=act, out_partials=out_partials)

@@ -104,12 +104,12 @@ class Decoder(nn.Module):
                 pending = None
         return self._logits(x, pending)
 
-    def _logits(self, x, pending):
+    def _logits(self, x, pending, rows=False):
         ln = self.ln
         if pending is None:
-            qa = QActivation.layernorm(x, ln.weight, ln.bias, ln.eps)
+            qa = QActivation.layernorm(x, ln.weight, ln.bias, ln.eps, rows)
         else:
-            _, qa = QActivation.add_layernorm(x, pending, ln.weight, ln.bias, ln.eps)
+            _, qa = QActivation.add_layernorm(x, pending, ln.weight, ln.bias, ln.eps, rows)
         return self.head(qa)
 
     # ------------------------------------------------------------ generation
@@ -126,7 +126,9 @@ class Decoder(nn.Module):
         cache holds; their keys and values enter it behind that (cache.advance
         then makes them part of it).  counts: rows that are tokens (None: all);
         parents (with depths int64 [B, T], a node's distance from the root): the
-        tokens form a tree."""
+        tokens form a tree.  Activations are quantized row by row, so that a
+        token's logits follow from its own sequence (with forward's one scale
+        for all rows they would shift with padding, neighbours and drafts)."""
         cache.room(ids.shape[1])
         where = torch.arange(ids.shape[1], device=ids.device) if depths is None else depths
         where = (cache.lengths[:, None] + where).clamp(max=self.ctx - 1)
@@ -139,15 +141,17 @@ class Decoder(nn.Module):
             else:
                 x = blk(x if pending is None else x.add(pending), step=step)
                 pending = None
-        return self._logits(x, pending)
+        return self._logits(x, pending, rows=True)
 
     def generate(self, prompts, new_tokens, temperature=1.0, drafts=0, seed=0):
         """`new_tokens` more tokens for each prompt (lists of ids), drawn at
         `temperature` (0: the likeliest).  With drafts > 0, each step verifies
         up to that many tokens looked up in the sequence itself -- what followed
         earlier occurrences of its last token, as a tree -- and keeps those that
-        the model's own probabilities accept: the tokens are distributed as
-        without drafts.  Returns one list of new ids per prompt."""
+        the model's own probabilities accept.  These follow from a token's own
+        sequence, so the tokens are distributed as without drafts and as in
+        another batch, but for what the order of the attention's 32-bit sums
+        moves.  Returns one list of new ids per prompt."""
         device = self.tok.weight.device
         seen = [list(p) for p in prompts]
         batch, longest = len(seen), max((len(p) for p in seen), default=0)
