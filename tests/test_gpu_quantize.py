@@ -250,3 +250,29 @@ def test_fused_single_launch_repeated_calls(kq):
         np.testing.assert_array_equal(q.cpu().numpy(), qo)
         assert partials[-2:].cpu().numpy().tolist() == [-(1 << 31) if calls % 2 else 0, 0]
     assert kq.device_status() == 0
+
+
+@pytest.mark.parametrize("M,K", [(1, 4), (9, 128), (33, 132), (5, 256), (17, 260), (3, 512), (40, 1020), (2, 1024), (3, 1028)])
+def test_short_rows_vs_oracle(kq, M, K):
+    """Rows that a warp holds, and their neighbours that it does not: ties, rows
+    of zeros, the ends of the range, a row that is not finite, and inputs off
+    their 16 bytes."""
+    x = np.random.RandomState(M + K).standard_normal((M, K)).astype(np.float32)
+    x[0, :] = np.arange(K) - K / 2 + 0.5 if K <= 254 else 0
+    if M > 4:
+        x[1] *= np.float32(1e-36)
+        x[2] = 0
+        x[3] *= np.float32(1e37)
+    for at in (0, 1):
+        wide = torch.empty(M * K + 1, device="cuda")
+        wide[at:at + M * K] = dev(x).reshape(-1)
+        q, s64, s32 = kq.quantize_rows_device(wide[at:at + M * K].view(M, K))
+        qo, so = ocpu.quantize_rows(x)
+        np.testing.assert_array_equal(q.cpu().numpy(), qo)
+        np.testing.assert_array_equal(s64.cpu().numpy(), so)
+        np.testing.assert_array_equal(s32.cpu().numpy(), so.astype(np.float32))
+    assert kq.device_status() == 0
+    bad = dev(x)
+    bad[M - 1, K - 1] = float("nan")
+    q, s64, _ = kq.quantize_rows_device(bad)
+    assert kq.device_status() == 2 and torch.isnan(s64).nonzero().tolist() == [[M - 1]] and not q[M - 1].any()
