@@ -385,7 +385,10 @@ int kz_cache_attention_f32(const kz_cache* cache, const float* q, int64_t batch,
  * r = (r - q)+ / sum (r - q)+ (r unchanged where that sum is 0).  path
  * [batch, nodes]: the accepted nodes from the root on, then -1; count[batch];
  * next[batch]: the smallest token whose running sum of r passes
- * sample_u * sum r.  All decisions in double.  nodes 1 to 1024, vocab below 2^24. */
+ * sample_u * sum r.  All decisions in double.  A row that a token is drawn from
+ * or a child rejected by and that holds NaN or Inf sets KZ_ERR_NONFINITE (next is
+ * then some token of the vocabulary; of a row of zeros it is the last).  nodes 1
+ * to 1024, vocab below 2^24. */
 int kz_verify_tree_f32(const int64_t* tokens, const int32_t* parents, int64_t parents_batch_stride,
                        const float* target, const float* draft, const float* accept_u, const float* sample_u,
                        int64_t batch, int64_t nodes, int64_t vocab, int32_t* path, int32_t* count, int64_t* next,

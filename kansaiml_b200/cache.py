@@ -284,7 +284,8 @@ def verify_tree(tokens, parents, target, draft, accept_u, sample_u):
     goes on there; else r = (r - q)+ / sum (r - q)+.  Returns path int32
     [batch, nodes] (the accepted nodes from the root on, then -1), count int32
     [batch], and the next token int64 [batch], drawn from r by sample_u: it is
-    distributed as the target's own, whatever was drafted."""
+    distributed as the target's own, whatever was drafted.  NaN or Inf in a row
+    that this takes a sum of is recorded in the device status word."""
     target = _raw(target, "target")
     shape = target.shape
     if len(shape) != 3 or shape[1] < 1 or shape[2] < 1:

@@ -9,6 +9,8 @@
 //     u[j] * q(x[j]) < r(x[j])   accept: j becomes the current node, r = p[j]
 //     otherwise                  reject: r = (r - q)+ / sum (r - q)+  (unchanged where that sum is 0)
 // and the next token is the smallest i with r(0) + .. + r(i) > u * sum r.
+// A row that a decision takes a sum of and that is not finite is recorded in the
+// status word; the sequence's answers then are some nodes and some token.
 // Everything is computed in double from the fp32 rows (or in two fp32 parts
 // that keep as much), so that the decisions do not depend on how the work is
 // split.
@@ -84,6 +86,13 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
     return v;
 }
 
+// x+, and NaN where x is: a row that is no distribution must not become one
+__device__ __forceinline__ double rest_of(double x) { return x < 0.0 ? 0.0 : x; }
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 __device__ __forceinline__ bool is_gone(const VerifyShared& s, int x) {
     for (int k = 0; k < s.rejections; ++k)
         if (s.gone[k] == x) return true;
@@ -91,7 +100,7 @@ __device__ __forceinline__ bool is_gone(const VerifyShared& s, int x) {
 }
 // whether node j is accepted, u q < r at its token, of its parent's row (t times it: no division)
 __device__ __forceinline__ bool accepts(const VerifyShared& s, bool has_draft, int j) {
-    const double p = s.p_at[j], q = s.q_at[j], rest = has_draft ? fmax(p - s.c * q, 0.0) : is_gone(s, s.token[j]) ? 0.0 : p;
+    const double p = s.p_at[j], q = s.q_at[j], rest = has_draft ? rest_of(p - s.c * q) : is_gone(s, s.token[j]) ? 0.0 : p;
     return (double)s.u[j] * q * s.t < rest;
 }
 // without a draft, the node's sum known: token of node j rejected
@@ -154,7 +163,7 @@ struct TwoPart {
     }
     // adds (p - q)+ = p - min(p, q): the difference's own rounding error is exact, as p is the larger
     __device__ __forceinline__ void add_rest(float p0, float p1, float q0, float q1) {
-        const uint64_t p = pair(p0, p1), q = pair(fminf(q0, p0), fminf(q1, p1)), d = sub2(p, q);
+        const uint64_t p = pair(p0, p1), q = pair(min_nan(q0, p0), min_nan(q1, p1)), d = sub2(p, q);
         add(d);
         lo = add2(lo, sub2(sub2(p, d), q));
     }
@@ -252,7 +261,7 @@ __global__ void __launch_bounds__(kVThreads, 2) verify_tree_kernel(VerifyArgs a)
         auto values = [&](const float4& pi, const float4& qi, double (&r)[4]) {
             const float pe[4] = {pi.x, pi.y, pi.z, pi.w}, qe[4] = {qi.x, qi.y, qi.z, qi.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) r[e] = c_now == 0.0 ? (double)pe[e] : fmax((double)pe[e] - c_now * (double)qe[e], 0.0);
+            for (int e = 0; e < 4; ++e) r[e] = c_now == 0.0 ? (double)pe[e] : rest_of((double)pe[e] - c_now * (double)qe[e]);
         };
         double sum[kVChunks];
 #pragma unroll
@@ -322,6 +331,7 @@ __global__ void __launch_bounds__(kVThreads, 2) verify_tree_kernel(VerifyArgs a)
                 double total = 0.0;
                 for (int c = 0; c < (int)ranks; ++c) total += sums[c];
                 s.summed = node;
+                if (rank == 0 && !(fabs(total) < INFINITY)) record_status(a.status, KZ_ERR_NONFINITE);
                 if (!q) {
                     take_out(s, rejected, total);
                 } else if (total > 0.0) {
@@ -349,6 +359,7 @@ __global__ void __launch_bounds__(kVThreads, 2) verify_tree_kernel(VerifyArgs a)
         double total = 0.0;
         for (int c = 0; c < (int)ranks; ++c) total += sums[c];
         const double want = sample_u * total;
+        if (rank == 0 && tid == 0 && !(fabs(want) < INFINITY)) record_status(a.status, KZ_ERR_NONFINITE);
         double before = 0.0;
         int slice = -1, last = (int)ranks - 1;
         for (int c = 0; c < (int)ranks; ++c) {

@@ -1047,3 +1047,44 @@ def test_attention_keeps_its_halves_over_long_contexts(cuda_device, d, kv, heads
             off = np.abs(y[b, t] - want) / want
             assert off.max() <= EVEN, (b, t, off.max())
     assert _status() == 0
+
+
+@pytest.mark.parametrize("vocab", [65, 3000, 50001])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("draft", [False, True])
+def test_verify_reports_rows_that_are_not_finite(cuda_device, vocab, value, draft):
+    """NaN or Inf in a row that a token is drawn from or a draft rejected by:
+    the status word says so, the token is one of the vocabulary, and the other
+    sequences are answered as ever."""
+    from kansaiml_b200 import _lib
+    from kansaiml_b200.cache import verify_tree
+    rs = np.random.RandomState(vocab)
+    batch, nodes = 4, 3
+    target, q = _softmax(rs, (batch, nodes, vocab), 1.0), _softmax(rs, (batch, nodes, vocab), 1.0)
+    parents, tokens = np.array([[-1, 0, 1]] * batch, np.int32), rs.randint(0, vocab, (batch, nodes)).astype(np.int64)
+    # accepted down to the leaf: sequences 0 and 1; rejected at once: 2 and 3
+    au = np.array([[0, 0, 0]] * 2 + [[0, 0.999, 0]] * 2, np.float32)
+    q[2:, 0, tokens[2:, 1]] = 1
+    su = rs.uniform(size=batch).astype(np.float32)
+
+    def run(target, q):
+        out = verify_tree(_dev(tokens), _dev(parents), _dev(target), _dev(q) if draft else None, _dev(au), _dev(su))
+        return [x.cpu().numpy() for x in out]
+
+    want = run(target, q)
+    assert _status() == 0 and want[1].tolist() == [3, 3, 1, 1]
+    at = int(tokens[2, 1] + 1) % vocab                     # not the drafted token's own
+    for rows, b, node in ((target, 0, 2), (target, 2, 0)) + (((q, 2, 0),) if draft else ()):
+        bad = rows.copy()
+        bad[b, node, at] = value
+        if rows is q and value == math.inf:
+            continue                                       # (p - inf)+ is 0: a number
+        got = run(*((bad, q) if rows is target else (target, bad)))
+        assert _status() == _lib.KZ_ERR_NONFINITE
+        assert 0 <= got[2][b] < vocab
+        for x, y in zip(got, want):
+            np.testing.assert_array_equal(np.delete(x, b, 0), np.delete(y, b, 0))
+    bad = target.copy()
+    bad[1, 0, (tokens[1, 1] + 1) % vocab] = value          # a row that only its child's own value is read of
+    got = run(bad, q)
+    assert _status() == 0 and all(np.array_equal(x, y) for x, y in zip(got, want))
