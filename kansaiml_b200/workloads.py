@@ -169,7 +169,9 @@ class Decoder(nn.Module):
         def step(ids, counts, parents=None, depths=None):
             logits = self.extend(ids, cache, counts, parents, depths).data
             if temperature > 0:
-                return torch.softmax(logits / temperature, -1)
+                # from the largest logit, which stays 0 however small the temperature; one below 1e-30 is its
+                # limit already (logits that differ do so by more), and its reciprocal might be infinite
+                return torch.softmax((logits - logits.amax(-1, keepdim=True)) / max(temperature, 1e-30), -1)
             return torch.nn.functional.one_hot(logits.argmax(-1), self.vocab).float()
 
         def verified(ids, parents, probs):

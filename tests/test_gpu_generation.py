@@ -201,3 +201,14 @@ def test_a_blocks_rows_do_not_meet_in_a_step(cuda_device, quantize):
     else:
         assert all(torch.equal(a, b) for a, b in zip(*out))
     assert _status() == 0
+
+
+def test_generate_at_the_smallest_temperatures(cuda_device, model):
+    """A temperature below what a division by it survives is the limit that it
+    stands for: the likeliest token."""
+    prompts = [[1, 2, 3], [60]]
+    want = model.generate(prompts, 8, 0.0)
+    for temperature in (1e-300, 1e-40, 1e-38, 1e-20):
+        assert model.generate(prompts, 8, temperature) == want
+    assert all(0 <= t < 65 for o in model.generate(prompts, 8, math.inf) for t in o)
+    assert _status() == 0
