@@ -14,9 +14,9 @@ import numpy as np
 import torch
 
 from . import nn
-from ._lib import KZ_TREE_MAX_NODES
+from ._lib import KZ_ERR_NONFINITE, KZ_TREE_MAX_NODES, KzError
 from .cache import PagePool, QCache, verify_tree
-from .quantize import QActivation, QLinear
+from .quantize import QActivation, QLinear, device_status
 from .tensor import Tensor, from_numpy
 
 
@@ -151,7 +151,9 @@ class Decoder(nn.Module):
         the model's own probabilities accept.  These follow from a token's own
         sequence, so the tokens are distributed as without drafts and as in
         another batch, but for what the order of the attention's 32-bit sums
-        moves.  Returns one list of new ids per prompt."""
+        moves.  Returns one list of new ids per prompt; raises ValueError where
+        something on the way was NaN or Inf (a model whose weights are), and
+        KzError for any other error that the device recorded."""
         device = self.tok.weight.device
         seen = [list(p) for p in prompts]
         batch, longest = len(seen), max((len(p) for p in seen), default=0)
@@ -164,6 +166,7 @@ class Decoder(nn.Module):
         if new_tokens < 1 or longest + new_tokens > self.ctx:
             raise ValueError(f"Decoder.generate: {longest} + {new_tokens} tokens, the context is {self.ctx}")
         cache = self.new_cache(batch)
+        earlier = device_status(device, clear=False)         # an error of another call's stays for its caller
         random = torch.Generator(device=device).manual_seed(seed)
 
         def step(ids, counts, parents=None, depths=None):
@@ -208,6 +211,11 @@ class Decoder(nn.Module):
                 s += new
                 o += new
             cache.advance(count, max(len(s) - 1 for s, on in zip(seen, live) if on))
+        code = 0 if earlier else device_status(device)
+        if code:
+            if code == KZ_ERR_NONFINITE:
+                raise ValueError("Decoder.generate: the logits, or keys and values on the way to them, contain NaN or Inf")
+            raise KzError(code, f"Decoder.generate: the device recorded error {code}")
         return [o[:new_tokens] for o in out]
 
 

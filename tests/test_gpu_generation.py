@@ -212,3 +212,21 @@ def test_generate_at_the_smallest_temperatures(cuda_device, model):
         assert model.generate(prompts, 8, temperature) == want
     assert all(0 <= t < 65 for o in model.generate(prompts, 8, math.inf) for t in o)
     assert _status() == 0
+
+
+def test_generate_reports_what_the_device_recorded(cuda_device):
+    """A model whose logits are not finite raises instead of returning ids, and
+    an error recorded before the call is left to whoever caused it."""
+    from kansaiml_b200 import _lib, workloads
+    model = workloads.Decoder(seed=3, layers=1)
+    torch.cuda.synchronize()
+    model.pos.weight.data[2] = math.nan
+    with pytest.raises(ValueError, match="NaN or Inf"):
+        model.generate([[1, 2, 3]], 4)
+    assert _status() == 0
+    model.generate([[1]], 1)                           # does not reach the row
+    broken = torch.full((1, 1, 5), math.nan, device="cuda")
+    from kansaiml_b200.cache import verify_tree
+    verify_tree(_ids([[0]]), _i32([-1]), broken, None, torch.zeros(1, 1, device="cuda"), torch.zeros(1, device="cuda"))
+    model.generate([[1]], 1)
+    assert _status() == _lib.KZ_ERR_NONFINITE
