@@ -129,6 +129,8 @@ class Decoder(nn.Module):
         tokens form a tree.  Activations are quantized row by row, so that a
         token's logits follow from its own sequence (with forward's one scale
         for all rows they would shift with padding, neighbours and drafts)."""
+        if parents is not None and depths is None:
+            raise ValueError("Decoder.extend: parents need the nodes' depths, from which their positions follow")
         cache.room(ids.shape[1])
         where = torch.arange(ids.shape[1], device=ids.device) if depths is None else depths
         where = (cache.lengths[:, None] + where).clamp(max=self.ctx - 1)

@@ -159,3 +159,11 @@ def test_cache_is_importable_under_the_reference_name():
     import kansai.cache
     import kansaiml_b200.cache
     assert kansai.cache is kansaiml_b200.cache
+
+
+def test_a_step_of_a_tree_needs_its_nodes_depths():
+    """Decoder.extend: parents without depths would take node numbers for positions."""
+    from kansaiml_b200.workloads import Decoder
+    ids, ints = torch.zeros(1, 3, dtype=torch.int64), torch.zeros(1, 3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="depths"):
+        Decoder.extend(None, ids, None, parents=ints)
