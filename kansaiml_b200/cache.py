@@ -235,7 +235,8 @@ class QCache:
 class PagePool:
     """Hands out page numbers 0 .. pages - 1 to ``batch`` sequences.  ``table``
     (int32 [batch, columns] on the device, -1 where a sequence has no page) is
-    what every layer's QCache takes; a change is one small copy to the device."""
+    what every layer's QCache takes; a change is one small copy to the device,
+    on the current stream, that the host does not wait for."""
 
     def __init__(self, pages, batch, columns, page_size=64, device=None):
         self.page_size, self.columns = int(page_size), int(columns)
@@ -253,16 +254,22 @@ class PagePool:
         need = -(-int(tokens) // self.page_size)
         if need > self.columns:
             raise ValueError(f"PagePool: {tokens} tokens need {need} pages a sequence, the table has {self.columns}")
-        which = range(len(self._held)) if sequence is None else [sequence]
+        which = range(len(self._held))
+        which = which if sequence is None else [which[sequence]]
         short = sum(max(0, need - len(self._held[i])) for i in which)
         if short > len(self._free):
             raise RuntimeError(f"PagePool: {short} pages needed, {len(self._free)} free")
-        for i in which:
-            at = len(self._held[i])
-            if need > at:
-                new = [self._free.pop() for _ in range(need - at)]
-                self._held[i] += new
-                self.table[i, at:need] = torch.tensor(new, dtype=torch.int32)
+        if not short:
+            return
+        at = [(i, c) for i in which for c in range(len(self._held[i]), need)]
+        new = self._free[:-short - 1:-1]
+        # from pinned memory, whose owner keeps it until the copy has run
+        change = torch.tensor([[i * self.columns + c for i, c in at], new], pin_memory=self.table.is_cuda)
+        change = change.to(self.table.device, non_blocking=True)
+        self.table.view(-1).scatter_(0, change[0], change[1].int())
+        del self._free[-short:]
+        for (i, _), page in zip(at, new):
+            self._held[i].append(page)
 
     def release(self, sequence):
         """Gives a sequence's pages back."""

@@ -1088,3 +1088,30 @@ def test_verify_reports_rows_that_are_not_finite(cuda_device, vocab, value, draf
     bad[1, 0, (tokens[1, 1] + 1) % vocab] = value          # a row that only its child's own value is read of
     got = run(bad, q)
     assert _status() == 0 and all(np.array_equal(x, y) for x, y in zip(got, want))
+
+
+def test_pages_are_handed_out_without_waiting(cuda_device):
+    """PagePool.reserve and release, sequences that cross pages together and
+    alone, make no call that waits for the GPU."""
+    from kansaiml_b200.cache import PagePool
+    pool, host = PagePool(300, 32, 12, 16, "cuda"), PagePool(300, 32, 12, 16, "cpu")
+    for p in (host, pool):
+        if p is pool:
+            torch.cuda.set_sync_debug_mode("error")
+        try:
+            p.reserve(1)
+            p.reserve(33)
+            p.reserve(100, 7)
+            p.release(3)
+            p.reserve(50, -1)
+            p.reserve(60)
+            p.reserve(60)
+            with pytest.raises(IndexError):
+                p.reserve(100, 32)
+            with pytest.raises(RuntimeError, match="pages needed"):
+                p.reserve(12 * 16)
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+    assert torch.equal(pool.table.cpu(), host.table) and pool.free == host.free
+    held = pool.table[pool.table >= 0].tolist()
+    assert len(set(held)) == len(held) == 300 - pool.free
