@@ -790,7 +790,7 @@ int launch_join_as(const CacheAttArgs& a, int64_t row_tiles, cudaStream_t s) {
 }
 template <int D, int RT>
 int launch_join(const CacheAttArgs& a, int64_t row_tiles, cudaStream_t s) {
-    return a.ctas <= 4 * a.batch * a.c.heads * row_tiles ? launch_join_as<D, RT, true>(a, row_tiles, s)
+    return a.ctas <= 4 * (int64_t)a.batch * a.c.heads * row_tiles ? launch_join_as<D, RT, true>(a, row_tiles, s)
                                                        : launch_join_as<D, RT, false>(a, row_tiles, s);
 }
 
@@ -814,9 +814,12 @@ bool short_table(int64_t cols, int64_t page) { return cols * page <= 4 * kKT; }
 // rows of heads of 128 51 and 98 against 58 and 150 with tiles of 64 rows.
 bool many_rows(int64_t rows) { return rows > 32; }
 
+int64_t tile_of(int64_t rows) { return many_rows(rows) ? kTcRows : tile_rows(rows); }
+int64_t row_tiles_of(int64_t rows) { return (rows + tile_of(rows) - 1) / tile_of(rows); }
+
 int64_t parts_floats(int64_t rows, int64_t d) {
     const int64_t ctas = (many_rows(rows) ? 1 : 2) * (int64_t)sm_count();
-    return 2 * ctas * (many_rows(rows) ? kTcRows : tile_rows(rows)) * (d + 2);
+    return 2 * ctas * tile_of(rows) * (d + 2);
 }
 
 template <int D, int NT, int RG>
@@ -844,16 +847,14 @@ int launch_cache_attention(CacheAttArgs a, int64_t row_tiles, cudaStream_t s) {
 
 template <int D>
 int dispatch_cache_attention(CacheAttArgs a, cudaStream_t s) {
-    const int64_t rows = (int64_t)a.tokens * a.group;
+    const int64_t rows = (int64_t)a.tokens * a.group, row_tiles = row_tiles_of(rows);
     if (many_rows(rows)) {
-        const int64_t tiles = (rows + kTcRows - 1) / kTcRows;
-        a.ctas = (int)std::min<int64_t>(sm_count(), a.parts ? sm_count() : a.batch * a.c.heads * tiles);
+        a.ctas = (int)std::min<int64_t>(sm_count(), a.parts ? sm_count() : (int64_t)a.batch * a.c.heads * row_tiles);
         a.by_ctas = fast_div((uint32_t)a.ctas);
         const int st = launch_cache_attention_tc(a, D, s);
-        return st || !a.parts ? st : launch_join<D, kTcRows>(a, tiles, s);
+        return st || !a.parts ? st : launch_join<D, kTcRows>(a, row_tiles, s);
     }
     const int rt = tile_rows(rows);
-    const int64_t row_tiles = (rows + rt - 1) / rt;
     if (rt == 4) return launch_cache_attention<D, 0, 1>(a, row_tiles, s);
     if (rt == 8) return launch_cache_attention<D, 1, 1>(a, row_tiles, s);
     if (rt == 16) return launch_cache_attention<D, 2, 1>(a, row_tiles, s);
@@ -890,7 +891,7 @@ extern "C" int kz_cache_attention_f32(const kz_cache* cache, const float* q, int
     KZ_REQUIRE(table_cols * cache->page_size < (int64_t)INT32_MAX - (1 << 25),
                "kz_cache_attention_f32: table_cols * page_size out of range");
     const int64_t most_tiles = (table_cols * cache->page_size + tokens) / kKT + 1;
-    KZ_REQUIRE(batch * cache->kv_heads * (tokens * (heads / cache->kv_heads) / 8 + 1) < (int64_t)INT32_MAX / most_tiles,
+    KZ_REQUIRE(batch * cache->kv_heads * row_tiles_of(tokens * (heads / cache->kv_heads)) < (int64_t)INT32_MAX / most_tiles,
                "kz_cache_attention_f32: the call's work is out of range");
     if (batch * tokens == 0) return KZ_OK;
     KZ_REQUIRE(q && out, "kz_cache_attention_f32: q or out is NULL");

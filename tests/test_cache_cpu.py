@@ -167,3 +167,20 @@ def test_a_step_of_a_tree_needs_its_nodes_depths():
     ids, ints = torch.zeros(1, 3, dtype=torch.int64), torch.zeros(1, 3, dtype=torch.int32)
     with pytest.raises(ValueError, match="depths"):
         Decoder.extend(None, ids, None, parents=ints)
+
+
+def test_attention_work_is_counted_in_the_kernels_own_tiles():
+    """Row tiles of 128 above 32 rows a key head, one tile below: long chunks
+    over long tables are refused only where the units of work pass 31 bits."""
+    lib = _lib.load()
+    c = _cache()
+
+    def attend(batch, tokens, heads, cols):
+        return lib.kz_cache_attention_f32(ctypes.byref(c), None, batch, tokens, heads, tokens * heads * 128, heads * 128,
+                                          P(16), cols, P(16), None, None, 0, 1.0, P(16), P(16), 1 << 40, None)
+
+    for batch, tokens, heads, cols in ((64, 4096, 4, 40000), (8, 60000, 4, 60000), (60000, 4, 16, 20000)):
+        _said(attend(batch, tokens, heads, cols), "q or out is NULL")
+    # 64 sequences x 2 heads x 64 row tiles x 300001 tiles of keys
+    _said(attend(64, 4096, 4, 600000), "work is out of range")
+    _said(attend(60000, 4, 16, 40000), "work is out of range")

@@ -1115,3 +1115,28 @@ def test_pages_are_handed_out_without_waiting(cuda_device):
     assert torch.equal(pool.table.cpu(), host.table) and pool.free == host.free
     held = pool.table[pool.table >= 0].tolist()
     assert len(set(held)) == len(held) == 300 - pool.free
+
+
+def test_attention_of_long_chunks_in_a_wide_table(cuda_device):
+    """4096 rows a sequence in a table of 2.5 million positions: 164 million
+    units of work, which 31 bits hold with room."""
+    d, kv, heads, tokens = 32, 8, 32, 4096
+    lengths, counts = [300, 9000, 0, 77, 1, 5000, 0, 128], [4096, 17, 0, 130, 1, 1000, 4000, 0]
+    book = Book([a + b for a, b in zip(lengths, counts)], kv, d, 64)
+    wide = torch.full((8, 40000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :book.table.shape[1]] = book.table
+    kvals, vvals = book.fill([a + b for a, b in zip(lengths, counts)])
+    q = torch.randn(8, tokens, heads * d, device="cuda")
+    y = book.cache.attention(q, heads, wide, _i32(lengths), _i32(counts)).data
+    for b, (n, m) in enumerate(zip(lengths, counts)):
+        assert not y[b, m:].any()
+        hidden = torch.ones(m, n + m, dtype=torch.bool, device="cuda").triu(n + 1)
+        for h in range(0, heads, 5):
+            k, v = (_dev(x[b][:, h * kv // heads]) for x in (kvals, vvals))
+            qq = q[b, :m, h * d:(h + 1) * d].double()
+            w = torch.softmax((qq @ k.T / math.sqrt(d)).masked_fill(hidden, -math.inf), -1)
+            # as in _attention_64, with the largest product of the whole sequence
+            size = (qq.abs() @ k.abs().T).max().item() / math.sqrt(d) if m else 0.0
+            bound = (2 * (d + 4) * size + 16 + (n + m) / 16 + 32) * 2.0**-23 * (w @ v.abs())
+            assert ((y[b, :m, h * d:(h + 1) * d].double() - w @ v).abs() <= bound).all(), (b, h)
+    assert _status() == 0
