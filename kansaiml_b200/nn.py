@@ -237,6 +237,10 @@ class TransformerBlock(Module):
         self.fc2 = QLinear(self.fc2, per_channel=per_channel, activations=activations)
         return self
 
+    def _attend(self, x, mask, step):
+        """Self-attention; a module of the user's in its place need not know of steps."""
+        return self.attn(x, x, x, mask=mask) if step is None else self.attn(x, x, x, mask=mask, step=step)
+
     def _w8a8(self):
         return isinstance(self.fc1, QLinear) and self.attn.qkv is not None
 
@@ -246,7 +250,7 @@ class TransformerBlock(Module):
             x, pending = self._forward_w8a8(x, mask, step=step)
             return x.add(pending)
         normed = self.ln1(x)
-        x = x.add(self.attn(normed, normed, normed, mask=mask, step=step))
+        x = x.add(self._attend(normed, mask, step))
         h = self.ln2(x)
         inner = (lambda layer, h: h) if step is None else _step_input
         if isinstance(self.fc1, QLinear):
@@ -269,7 +273,7 @@ class TransformerBlock(Module):
             qa = QActivation.layernorm(x, ln1.weight, ln1.bias, ln1.eps, rows)
         else:
             x, qa = QActivation.add_layernorm(x, pending, ln1.weight, ln1.bias, ln1.eps, rows)
-        x, qb = QActivation.add_layernorm(x, self.attn(qa, qa, qa, mask=mask, step=step), ln2.weight, ln2.bias, ln2.eps, rows)
+        x, qb = QActivation.add_layernorm(x, self._attend(qa, mask, step), ln2.weight, ln2.bias, ln2.eps, rows)
         if rows:
             return x, self.fc2(QActivation.rows(self.fc1(qb, act="gelu")))
         partials = partials_buffer(x.data.device)

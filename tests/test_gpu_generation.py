@@ -230,3 +230,24 @@ def test_generate_reports_what_the_device_recorded(cuda_device):
     verify_tree(_ids([[0]]), _i32([-1]), broken, None, torch.zeros(1, 1, device="cuda"), torch.zeros(1, device="cuda"))
     model.generate([[1]], 1)
     assert _status() == _lib.KZ_ERR_NONFINITE
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_an_attention_of_a_users_own(cuda_device, quantized):
+    """A block whose attention takes query, key, value and mask, as the
+    reference's does, runs without a cache as it always has."""
+    from kansaiml_b200 import nn as knn
+    from kansaiml_b200.tensor import Tensor
+
+    class Own(knn.MultiHeadAttention):
+        def forward(self, query, key, value, mask=None):
+            return super().forward(query, key, value, mask)
+
+    blk = knn.TransformerBlock(64, 2, 128, seed=1, device="cuda")
+    own = knn.TransformerBlock(64, 2, 128, seed=1, device="cuda")
+    own.attn = Own(64, 2, seed=1, device="cuda")
+    if quantized:
+        blk.quantize()
+        own.quantize()
+    x, mask = Tensor(torch.randn(2, 9, 64, device="cuda")), knn.causal_mask(9, device="cuda")
+    assert torch.equal(own(x, mask).data, blk(x, mask).data)
