@@ -40,8 +40,16 @@ def _as_device(device):
 
 
 def stream_handle(device):
-    """The raw cudaStream_t of torch's current stream on `device`."""
-    index = device.index
+    """The raw cudaStream_t of torch's current stream on `device` (a torch.device,
+    its name or number, or None: the current one)."""
+    if isinstance(device, int):
+        index = device
+    else:
+        if isinstance(device, str):
+            device = torch.device(device)
+        index = None if device is None else device.index
+        if device is not None and device.type != "cuda":
+            raise ValueError(f"stream_handle: expected a cuda device, not {device}")
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 

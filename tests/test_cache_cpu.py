@@ -184,3 +184,14 @@ def test_attention_work_is_counted_in_the_kernels_own_tiles():
     # 64 sequences x 2 heads x 64 row tiles x 300001 tiles of keys
     _said(attend(64, 4096, 4, 600000), "work is out of range")
     _said(attend(60000, 4, 16, 40000), "work is out of range")
+
+
+def test_stream_handle_takes_what_torch_calls_a_device(monkeypatch):
+    """A device, a name, a number or None (the current device)."""
+    from kansaiml_b200.tensor import stream_handle
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 1000 + index, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    for device, index in ((torch.device("cuda", 1), 1), ("cuda:2", 2), (2, 2), (None, 3), ("cuda", 3), (torch.device("cuda"), 3)):
+        assert stream_handle(device) == 1000 + index
+    with pytest.raises(ValueError, match="cuda"):
+        stream_handle("cpu")
