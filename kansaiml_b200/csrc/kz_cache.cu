@@ -51,8 +51,9 @@ __device__ __forceinline__ float4 codes_times(uint32_t w, float s) {
 // row and back by shuffles, so a warp divides once for all its rows.  Bound by
 // HBM: 16 prompts of up to 2000 tokens, 8 heads of 128, values returned (509
 // MB), 88 us = 5.8 TB/s, 0.89 of a plain copy; a row at a time, every row
-// finding its own place and dividing for itself, took 208 us.  One token of 32
-// sequences, 4 heads of 64: 3.0 us, the launch.
+// finding its own place and dividing for itself, took 208 us.  Without values (247
+// MB) 57 us = 4.3 TB/s, 0.66: there the quantizing, which those writes hid, shows.
+// One token of 32 sequences, 4 heads of 64: 3.0 us, the launch.
 template <int D, int kU>
 __global__ void __launch_bounds__(kCacheThreads, 4) cache_write_kernel(WriteArgs a) {
     constexpr int L = D / 4, G = 32 / L, N = 2 * kU * G;   // lanes a row, groups a warp, rows a warp
@@ -259,7 +260,11 @@ __global__ void __launch_bounds__(kCacheThreads) cache_keep_kernel(KeepArgs a) {
 
 // Row sets a warp holds: as many as the heads fill, four at most.  With 1, 2
 // and 4 sets, heads of 128, 16 x 2000 tokens: 1 head 14.6, 16.1, 20.5 us; 2
-// heads 29.0, 24.2, 27.2 us; 8 heads 111, 88.9, 87.6 us.
+// heads 29.0, 24.2, 27.2 us; 8 heads 111, 88.9, 87.6 us (without values 66.3 with 2
+// and 57.2 with 4).  Heads of 64 and 32, whose four sets spill 44 bytes a thread,
+// with 2 and 4: 8 of 64 45.2 and 46.9 us (without values 33.9, 33.1), 16 of 64 88.9,
+// 91.6 (65.7, 62.4), 16 of 32 45.8, 50.0 (33.8, 35.2).  32 single tokens, 8 heads of
+// any width, are the other way round: 3.0 us with 2 sets, 4.3 with 4.
 template <int D>
 int launch_write(WriteArgs a, int64_t batch, cudaStream_t s) {
     constexpr int G = 128 / D;

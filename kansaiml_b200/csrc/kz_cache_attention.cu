@@ -811,7 +811,12 @@ bool short_table(int64_t cols, int64_t page) { return cols * page <= 4 * kKT; }
 // time does not depend on them up to 128: at 32 rows (batch 16, 8 key heads of
 // 128, contexts of 1500 and 6000) it takes 36.6 and 85.6 us against 36.8 and 86.2
 // here, with heads of 64 (20 rows, 32 contexts of 5000) 124 against 87; at 64
-// rows of heads of 128 51 and 98 against 58 and 150 with tiles of 64 rows.
+// rows of heads of 128 51 and 98 against 58 and 150 with tiles of 64 rows.  Both at
+// each width, 16 contexts of up to 6000, 4 key heads (there, here): of 128 20 rows
+// 49.6, 54.4, 32 50.2, 55.8, 36 50.3, 67.8, 64 53.8, 87.7 us; of 64 44.2, 36.8, 44.4,
+// 37.7, 44.3, 47.0, 45.3, 55.9; of 32 37.3, 29.9, 37.7, 30.7, 37.6, 39.1, 38.5, 44.2.
+// Of up to 300 the other way round for 36 to 64 rows: of 64 12.2 and 10.8, of 32 11.2
+// and 9.0 us, which one rule for all lengths costs.
 bool many_rows(int64_t rows) { return rows > 32; }
 
 int64_t tile_of(int64_t rows) { return many_rows(rows) ? kTcRows : tile_rows(rows); }

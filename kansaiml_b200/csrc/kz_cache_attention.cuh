@@ -78,6 +78,10 @@ __device__ __forceinline__ int a_cta(const CacheAttArgs& a, int units) { return 
 // 16.2, -, 19.1 / 22.7, 31.0 / 31.3 us; of 64 (700) 27.2 / 30.4 us; chunks of 20
 // tokens (80 rows) of one sequence 22.3 / 16.6, 24.1 / 16.6, 28.5 / 17.0 us, of
 // 8 22.7 / 24.5, -, 28.9 / 26.4, of 16 24.2 / 33, -, 31 / 39, 47.7 / 50.2 us.
+// Heads of 64 and 32 (1, 8 and 32 sequences of up to 700, 1500 and 4000 keys, 4 key
+// heads; 1, 4, 7 and 64 rows): what it chooses is the better, or within 12% of it
+// (32 of 700, one row, 64 wide 10.6 / 11.2, 32 wide 9.6 / 10.6), but for 64 rows over
+// 32 of 1500: 31.6 / 36.5 and 28.7 / 31.1, where it takes ranges.
 __device__ __forceinline__ bool whole_ranges(const CacheAttArgs& a, const Work& w) {
     return !a.parts || (int64_t)a_cta(a, w.row_tiles) * w.tiles <= (int64_t)a_cta(a, w.units) + 3;
 }

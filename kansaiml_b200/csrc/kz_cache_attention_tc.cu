@@ -15,9 +15,11 @@
 // scores run while tile t's softmax does.
 //
 // Measured, join included: 2 chunks of 500 tokens over 8192 keys, 16 heads over 4
-// key heads of 128: 150 us = 920 TFLOP/s over both halves, 0.56 of the tensor
-// cores' measured rate; trees of 24 tokens (96 rows) over 8 contexts of 2500 to
-// 5000, 8 key heads of 128: 51 us.  What bounds it is the softmax's chain: a tile takes
+// key heads of 128: 152 us = 910 TFLOP/s over both halves, 0.55 of the tensor
+// cores' measured rate (heads of 64: 130 us, of 32: 111); trees of 24 tokens (96
+// rows) over 8 contexts of 2500 to 5000, 8 key heads of 128: 51 us, of which the 13
+// tiles a CTA are 27, the start and the changes of row tile about 14, the rest the
+// join and the tail.  What bounds the tiles is the softmax's chain: one takes
 // about 3900 cycles, of which the MMAs are 2050 and the exponentials 1024; with
 // neither MMAs nor conversions four fifths of the time remain.  A row a thread
 // with the two warpgroups on alternate tiles took 207 us instead of 157 (S is read

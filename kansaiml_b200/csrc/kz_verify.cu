@@ -27,14 +27,18 @@
 // ends with it, its sums are those that the last token is drawn by.  Without
 // one r is p with the rejected tokens taken out, over what is left: one pass
 // over a node's row gives its sum, from which each rejected token's p is
-// subtracted.  Nothing else of the probabilities is touched.  What bounds it is
-// latency -- a pass, a meeting, the walk, for each rejection -- so a warp loads
-// all of its part of a slice (8 chunks, 128 values of each at a time) before it
-// adds anything up.
+// subtracted.  Nothing else of the probabilities is touched.  What bounds it: for
+// each rejection a pass, a meeting and the walk, one after another.  The passes
+// of a whole batch run at the memory's rate (33 MB in 4.4 us, the first from HBM, the
+// later ones from L2), on values that an earlier pass at the node had in registers
+// already; meetings and walk (2 to 3 us) are latency.  A warp loads all of its
+// part of a slice (8 chunks, 128 values of each at a time) before it adds anything
+// up.
 //
-// Measured: 32 trees of 16 nodes over 128000 tokens with a draft, 27 us (32.8 MB
-// of rows once: 5 us); 32 trees of 6 nodes over 65 tokens, no draft: 10.1 us.
-// Before the walk lost its divisions and the draw its serial sums (30 us) the
+// Measured: 32 trees of 16 nodes over 128000 tokens with a draft, 26 to 28 us (32.8
+// MB of rows once: 5 us); 32 trees of 6 nodes over 65 tokens, no draft: 10.1 us.
+// Rows that do not start on 16 bytes are read by the word: 32 trees of 16 over 50257
+// tokens 20.0 us, over 50256 16.0; without a draft 13.2 and 12.1.  Before the walk lost its divisions and the draw its serial sums (30 us) the
 // first took 42 us with clusters of 4, 40 with blocks of 128 threads and 32 with
 // every sum in double.
 #include <math.h>
