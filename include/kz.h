@@ -385,7 +385,8 @@ int kz_cache_attention_f32(const kz_cache* cache, const float* q, int64_t batch,
  * r = (r - q)+ / sum (r - q)+ (r unchanged where that sum is 0).  path
  * [batch, nodes]: the accepted nodes from the root on, then -1; count[batch];
  * next[batch]: the smallest token whose running sum of r passes
- * sample_u * sum r.  All decisions in double.  A row that a token is drawn from
+ * sample_u * sum r.  All decisions in double (draft NULL: what is left beside
+ * rejected tokens, where that is below 2^-50 of their mass, may count as none).  A row that a token is drawn from
  * or a child rejected by and that holds NaN or Inf sets KZ_ERR_NONFINITE (next is
  * then some token of the vocabulary; of a row of zeros it is the last).  nodes 1
  * to 1024, vocab below 2^24. */

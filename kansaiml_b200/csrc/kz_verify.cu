@@ -36,7 +36,7 @@
 // up.
 //
 // Measured: 32 trees of 16 nodes over 128000 tokens with a draft, 26 to 28 us (32.8
-// MB of rows once: 5 us); 32 trees of 6 nodes over 65 tokens, no draft: 10.1 us.
+// MB of rows once: 5 us); 32 trees of 6 nodes over 65 tokens, no draft: 10.5 us.
 // Rows that do not start on 16 bytes are read by the word: 32 trees of 16 over 50257
 // tokens 20.0 us, over 50256 16.0; without a draft 13.2 and 12.1.  Before the walk lost its divisions and the draw its serial sums (30 us) the
 // first took 42 us with clusters of 4, 40 with blocks of 128 threads and 32 with
@@ -350,14 +350,21 @@ __global__ void __launch_bounds__(kVThreads, 2) verify_tree_kernel(VerifyArgs a)
         }
         // the next token: the slice, then the chunk, then the value in which the running sum passes u * total
         if (!q && s.rejections > 0) {
-            // without the tokens taken out
+            // without the tokens taken out.  n subtractions leave up to n^2 2^-53 of the largest of them where
+            // there is nothing left, which u = 0 would take for mass: as little is none
             __syncthreads();
-            if (tid == 0)
-                for (int k = 0; k < s.rejections; ++k) {
-                    const int c = s.gone[k] / a.chunk, of = warps * kVChunks;
-                    sums[c / of] -= s.gone_p[k];
-                    if (c / of == (int)rank) s.chunk_sum[c % of / kVChunks][c % kVChunks] -= s.gone_p[k];
-                }
+            if (tid == 0) {
+                const int of = warps * kVChunks;
+                const double lim = 2.220446049250313e-16 * s.rejections * s.rejections;
+                for (int turn = 0; turn < 2; ++turn)
+                    for (int k = 0; k < s.rejections; ++k) {
+                        const int c = s.gone[k] / a.chunk;
+                        const double p = s.gone_p[k];
+                        auto take = [&](double& x) { x = turn == 0 ? x - p : x > lim * p ? x : 0.0; };
+                        take(sums[c / of]);
+                        if (c / of == (int)rank) take(s.chunk_sum[c % of / kVChunks][c % kVChunks]);
+                    }
+            }
             __syncthreads();
         }
         double total = 0.0;

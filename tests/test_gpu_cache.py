@@ -1140,3 +1140,23 @@ def test_attention_of_long_chunks_in_a_wide_table(cuda_device):
             bound = (2 * (d + 4) * size + 16 + (n + m) / 16 + 32) * 2.0**-23 * (w @ v.abs())
             assert ((y[b, :m, h * d:(h + 1) * d].double() - w @ v).abs() <= bound).all(), (b, h)
     assert _status() == 0
+
+
+@pytest.mark.parametrize("vocab", [3000, 128000])
+def test_verify_draws_nothing_that_was_taken_out(cuda_device, vocab):
+    """Without draft rows: two rejected tokens that are all there is of a
+    stretch of the row, one far smaller than the other, and the smallest u: what
+    rounding leaves of that stretch's sum is no token's."""
+    from kansaiml_b200.cache import verify_tree
+    batch, y = 64, 2 * vocab // 3
+    small = np.random.RandomState(3).uniform(1e-12, 1e-10, batch).astype(np.float32)
+    p = np.zeros((batch, 3, vocab), np.float32)
+    p[:, 0, 3] = 0.9
+    p[:, 0, 5] = small
+    p[:, 0, y] = 0.1
+    tokens, parents = np.array([[0, 3, 5]] * batch, np.int64), np.array([-1, 0, 0], np.int32)
+    au, su = np.array([[0, 0.95, 0.5]] * batch, np.float32), np.zeros(batch, np.float32)
+    su[1::2] = np.float32(2.0**-60)
+    path, count, token = verify_tree(_dev(tokens), _dev(parents), _dev(p), None, _dev(au), _dev(su))
+    assert count.tolist() == [1] * batch and token.tolist() == [y] * batch
+    assert _status() == 0
