@@ -309,7 +309,8 @@ int kz_gemm_i8_allgather(const int8_t* A, int8_t* const* peer_A, uint32_t* const
  * the call; counts[b] (int32, device, NULL: all) the number of its rows that
  * are tokens, the rest being padding.  A page number outside the pool, or a
  * position the table has no column for, is not read or written: the row is
- * left out and the device status word set to KZ_ERR_INVALID_ARGUMENT.
+ * left out and the device status word set to KZ_ERR_INVALID_ARGUMENT, as for a
+ * negative length (no tokens).
  *
  * A row (one token, one head) is quantized by quantize.py:66-70's rule on its
  * own: scale = max|x| / 127 in double (1 for zeros), codes rounded half to

@@ -156,7 +156,9 @@ __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(ReadArgs a) {
     const uint32_t b = div_by(bc, a.by_chunks), chunk = bc - b * a.by_chunks.d;
     const int64_t first = (int64_t)chunk * a.c.page;
     const int rows = (int)min((int64_t)a.c.page, (int64_t)a.most - first);          // output rows of this page
-    int held = (int)min((int64_t)rows, max((int64_t)0, (int64_t)a.s.lengths[b] - first));
+    const int length = a.s.lengths[b];
+    int held = (int)min((int64_t)rows, max((int64_t)0, (int64_t)length - first));
+    if (length < 0 && lane == 0) record_status(a.status, KZ_ERR_INVALID_ARGUMENT);
     int64_t base = 0;
     if (held > 0) {
         const int page = page_of(a.c, a.s, b, first);

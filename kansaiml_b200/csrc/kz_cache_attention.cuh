@@ -104,7 +104,10 @@ template <int RT>
 __device__ __forceinline__ void find_range(const CacheAttArgs& a, RangeShared& s) {
     const int tid = threadIdx.x, each = (a.batch + 127) / 128;
     Work w{0, 0, 0};
-    for (int b = tid * each; b < min(a.batch, (tid + 1) * each); ++b) w.add(a, sequence<RT>(a, b));
+    for (int b = tid * each; b < min(a.batch, (tid + 1) * each); ++b) {
+        w.add(a, sequence<RT>(a, b));
+        if (blockIdx.x == 0 && a.s.lengths[b] < 0) record_status(a.status, KZ_ERR_INVALID_ARGUMENT);
+    }
     s.part[tid] = w;
     w.add_warp();
     if ((tid & 31) == 0) s.warp[tid >> 5] = w;

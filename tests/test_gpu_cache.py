@@ -1160,3 +1160,22 @@ def test_verify_draws_nothing_that_was_taken_out(cuda_device, vocab):
     path, count, token = verify_tree(_dev(tokens), _dev(parents), _dev(p), None, _dev(au), _dev(su))
     assert count.tolist() == [1] * batch and token.tolist() == [y] * batch
     assert _status() == 0
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_a_negative_length_is_reported(cuda_device, tokens):
+    """By every entry point that takes lengths; the other sequences' rows are as ever."""
+    from kansaiml_b200 import _lib
+    book = Book([100, 100, 300], 1, 64, 32)
+    book.fill([100, 100, 300])
+    x, q = torch.randn(3, tokens, 64, device="cuda"), torch.randn(3, tokens, 128, device="cuda")
+    good, bad = _i32([50, 20, 200]), _i32([50, -3, 200])
+    want = book.cache.attention(q, 2, book.table, good).data
+    path, count = _i32([[0] + [-1] * 6] * 3), _i32([1, 1, 1])
+    for call in (lambda: book.cache.attention(q, 2, book.table, bad).data, lambda: book.cache.read(book.table, bad, 200)[0].data,
+                 lambda: book.cache.keep(book.table, bad, path, count), lambda: book.cache.write(x, x, book.table, bad)):
+        assert _status() == 0
+        got = call()
+        assert _status() == _lib.KZ_ERR_INVALID_ARGUMENT
+        if got is not None and got.shape == want.shape:
+            assert torch.equal(got[::2], want[::2])
