@@ -173,11 +173,13 @@ class Decoder(nn.Module):
 
         def step(ids, counts, parents=None, depths=None):
             logits = self.extend(ids, cache, counts, parents, depths).data
+            top = logits.amax(-1, keepdim=True)
             if temperature > 0:
                 # from the largest logit, which stays 0 however small the temperature; one below 1e-30 is its
                 # limit already (logits that differ do so by more), and its reciprocal might be infinite
-                return torch.softmax((logits - logits.amax(-1, keepdim=True)) / max(temperature, 1e-30), -1)
-            return torch.nn.functional.one_hot(logits.argmax(-1), self.vocab).float()
+                return torch.softmax((logits - top) / max(temperature, 1e-30), -1)
+            likeliest = torch.nn.functional.one_hot(logits.argmax(-1), self.vocab)
+            return likeliest + (top - top)                   # NaN where a logit is, for the verification to see
 
         def verified(ids, parents, probs):
             nodes = ids.shape[1]

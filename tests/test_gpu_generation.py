@@ -251,3 +251,14 @@ def test_an_attention_of_a_users_own(cuda_device, quantized):
         own.quantize()
     x, mask = Tensor(torch.randn(2, 9, 64, device="cuda")), knn.causal_mask(9, device="cuda")
     assert torch.equal(own(x, mask).data, blk(x, mask).data)
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_generate_refuses_logits_that_are_none(cuda_device, temperature):
+    """NaN that enters behind the last cached layer, in the logits alone."""
+    from kansaiml_b200 import workloads
+    model = workloads.Decoder(seed=3, layers=1)
+    model.head.bias.data[7] = math.nan
+    with pytest.raises(ValueError, match="NaN or Inf"):
+        model.generate([[1, 2, 3], [4]], 3, temperature)
+    assert _status() == 0
