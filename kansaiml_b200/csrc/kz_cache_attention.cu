@@ -799,7 +799,8 @@ int launch_join(const CacheAttArgs& a, int64_t row_tiles, cudaStream_t s) {
 // Rows of a tile: the smallest of 4, 8, 16 and 32 that holds a key head's rows.  With
 // tiles of 4, 8, 16 and 32, 4 rows over 32 long sequences: 73, 76, 110 and 197 us
 // (4 and 8 for seconds on end, under the power cap: 79 and 86); 16 rows, 16
-// sequences of 3000 to 6000: 51 us with 16, 84 with 32.
+// sequences of 3000 to 6000: 51 us with 16, 84 with 32 (which spills 152 bytes a
+// thread at heads of 128).
 int tile_rows(int64_t rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
 
 // Whether a call needs no workspace and no join: its table holds no more than
